@@ -304,6 +304,82 @@ KVQ_API int kvq_test_attention_timeout(const void* q, int64_t q_token_stride,
                                        int64_t wait_cycles, void* stream);
 
 /*
+ * ------------------------------------------------------------------ paged cache
+ * The same quantized rows in pages, for batches of sequences of different lengths
+ * (grouped query heads, causal or not). No counterpart in the reference, whose
+ * cache is one contiguous tensor per layer.
+ *
+ * k_pages / v_pages: uint8 [n_pages][n_heads][page_size / 16][16 * (CW + 2 G)],
+ * CW = 64 code bytes per row (int4) or 128 (int8), G = n_groups. A block of 16
+ * tokens of one head is 16 rows of codes, then 16 rows of G bf16 scales, codes and
+ * scales as kvq_quantize() writes them. page_size is 16, 32, 64 or 128; head_dim is
+ * 128; (k_bits, v_bits) is (4, 4), (8, 4) or (8, 8); the group map is one of the
+ * five specialised ones. Both arrays are 16-byte aligned.
+ */
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  int64_t n_pages;
+  int32_t page_size, n_heads, head_dim, k_bits, v_bits, n_groups;
+  const int32_t* chan_band; /* HOST int32[head_dim] */
+} kvq_paged_cache;
+
+/* One sequence (device array): kv_len cached tokens, the last q_len of them new;
+ * q_first / kv_first: sums of the q_len / kv_len before it; q_block / kv_block:
+ * sums of the 16-token storage blocks that the new tokens / all tokens of the
+ * sequences before it touch. q_len may exceed kv_len only for attention: queries
+ * before position 0 see nothing. */
+typedef struct {
+  int32_t kv_len, q_len, q_first, kv_first, q_block, kv_block, reserved0, reserved1;
+} kvq_paged_seq;
+
+/* table: device int32 [n_seqs][table_stride], the pages of each sequence in order,
+ * entries in [0, n_pages) wherever the sequence has tokens (an entry outside reads
+ * page 0 and writes nothing). n_new, n_tokens, n_new_blocks, n_blocks: the sums over
+ * all sequences that kvq_paged_seq counts. */
+typedef struct {
+  const int32_t* table;
+  int64_t table_stride;
+  const kvq_paged_seq* seqs;
+  int64_t n_new, n_tokens, n_new_blocks, n_blocks;
+  int32_t n_seqs, reserved;
+} kvq_paged_batch;
+
+/*
+ * Quantizes the new tokens' K and V rows into their pages, one launch.
+ *   k, v   bf16 [n_new][n_heads][head_dim], token strides in elements; 16-byte
+ *          aligned rows
+ * Codes and scales are those of kvq_quantize(), except that stored values are always
+ * finite: NaN counts as 0 and magnitudes above 3e38 count as 3e38, so a page never
+ * poisons the queries that do not see it. Two tokens must not share a slot.
+ */
+KVQ_API int kvq_paged_append(const void* k, int64_t k_token_stride, const void* v, int64_t v_token_stride,
+                             const kvq_paged_cache* cache, const kvq_paged_batch* batch, void* stream);
+
+/*
+ * Reads the sequences' tokens (new_only: their new tokens) back as bf16
+ * [n_tokens or n_new][n_heads][head_dim], sequence after sequence: the exact product
+ * code * scale rounded once, as kvq_dequantize().
+ */
+KVQ_API int kvq_paged_read(const kvq_paged_cache* cache, const kvq_paged_batch* batch, int new_only, void* k_out,
+                           int64_t k_out_token_stride, void* v_out, int64_t v_out_token_stride, void* stream);
+
+/*
+ * Attention of the new tokens' queries over their sequences' cached tokens:
+ * query i of a sequence stands at position p = kv_len - q_len + i and sees tokens
+ *   j < kv_len,  j <= p if causal,  j > p - window or j < sink if window > 0;
+ * out = sum_j w_j V_j, w = softmax(q . K_j * softmax_scale) over the tokens it sees
+ * (softmax_scale <= 0: 1/sqrt(head_dim)); 0 (lse -inf) where it sees none.
+ *   q, out  bf16 [n_new][n_q_heads][head_dim], token strides in elements; query head
+ *           h reads KV head h / (n_q_heads / n_heads)
+ *   lse     fp32 [n_new][n_q_heads] or NULL: natural log of the sum of exponentials
+ */
+KVQ_API int kvq_paged_attention(const void* q, int64_t q_token_stride, const kvq_paged_cache* cache,
+                                const kvq_paged_batch* batch, void* out, int64_t out_token_stride, float* lse,
+                                int n_q_heads, int causal, int64_t window, int64_t sink, float softmax_scale,
+                                void* stream);
+
+/*
  * Synchronizes the current device and returns the library's device status word:
  * 0 = no kernel gave up, 1 = a kernel's bounded wait timed out (its output is
  * invalid). reset != 0 clears it. No counterpart in the reference (its Triton

@@ -45,7 +45,24 @@ SIGNATURES = {
     "kvq_test_attention_timeout": (_i32, [_p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _i32,
                                           _i64, _i32, _i32, _p, _i32, _i32, _i32, _f32, _i32, _i64, _p]),
     "kvq_device_status": (_i32, [_i32]),
+    "kvq_paged_append": (_i32, [_p, _i64, _p, _i64, _p, _p, _p]),
+    "kvq_paged_read": (_i32, [_p, _p, _i32, _p, _i64, _p, _i64, _p]),
+    "kvq_paged_attention": (_i32, [_p, _i64, _p, _p, _p, _i64, _p, _i32, _i32, _i64, _i64, _f32, _p]),
 }
+
+
+class PagedCacheArgs(ctypes.Structure):
+    """kvq_paged_cache"""
+    _fields_ = [("k_pages", _p), ("v_pages", _p), ("n_pages", _i64), ("page_size", _i32), ("n_heads", _i32),
+                ("head_dim", _i32), ("k_bits", _i32), ("v_bits", _i32), ("n_groups", _i32), ("chan_band", _p)]
+
+
+class PagedBatchArgs(ctypes.Structure):
+    """kvq_paged_batch"""
+    _fields_ = [("table", _p), ("table_stride", _i64), ("seqs", _p), ("n_new", _i64), ("n_tokens", _i64),
+                ("n_new_blocks", _i64), ("n_blocks", _i64), ("n_seqs", _i32), ("reserved", _i32)]
+
+
 ABI_VERSION = 3
 IPC_HANDLE_BYTES = 64
 

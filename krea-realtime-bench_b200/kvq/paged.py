@@ -1,0 +1,298 @@
+"""Paged, quantized KV cache for batches of sequences of different lengths.
+
+    cache = PagedKVCache(n_pages, page_size, n_kv_heads, k_bits=4, v_bits=4, group_mode="bands4", device="cuda")
+    batch = PagedBatch(block_table, kv_lens, q_lens, page_size, device="cuda")   # once per step, for all layers
+    cache.append(k, v, batch)                  # quantize the step's new tokens into their pages
+    out = attention(q, cache, batch)           # their queries over everything cached, causal
+    k, v = cache.read(batch)                   # bf16 values of the sequences' tokens
+
+One layer's K and V live in pages of 16 to 128 tokens; a sequence owns pages through
+its row of the block table, so sequences grow, share a prefix, or drop their oldest
+pages (an eviction that moves and requantizes nothing) by editing that row. Rows are
+stored as QuantKVTensor stores them: int4 or int8 codes with one bf16 scale per
+(token, head, channel group). There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import torch
+
+import quant_kv_kernels as _kern
+
+from . import _lib
+from .ops import _ptr, _require_cuda, _stream
+
+BLOCK = 16  # tokens of one storage block
+PAGE_SIZES = (16, 32, 64, 128)
+HEAD_DIM = 128
+
+
+def _cuda_device(device) -> torch.device:
+    dev = torch.device(device)
+    if dev.type != "cuda":
+        raise RuntimeError(f"the paged cache needs a CUDA (sm_100) device, got {device}; "
+                           "the B200 build has no CPU path")
+    return torch.device("cuda", torch.cuda.current_device()) if dev.index is None else dev
+
+
+def _host_ints(x, name: str, ndim: int) -> np.ndarray:
+    if isinstance(x, torch.Tensor):
+        if x.device.type != "cpu":
+            raise TypeError(f"{name} must be host data (a list, a numpy array or a CPU tensor): the step is planned "
+                            "on the host")
+        x = x.numpy()
+    a = np.asarray(x)
+    if a.size == 0:
+        a = a.astype(np.int64)
+    if a.ndim != ndim or a.dtype.kind not in "iu":
+        raise ValueError(f"{name} must be a {ndim}-D array of whole numbers")
+    return a.astype(np.int64)
+
+
+class PagedBatch:
+    """The sequences of one step: which pages they own, how many tokens they hold
+    (new ones included) and how many of those are new. Shared by all layers and by
+    append, read and attention. block_table [B, most pages], kv_lens [B] and q_lens
+    [B] are host data; row b's first ceil(kv_lens[b] / page_size) entries are used.
+    Tensors with one row per new token are ordered sequence after sequence."""
+
+    def __init__(self, block_table, kv_lens, q_lens, page_size: int, device="cuda"):
+        dev = _cuda_device(device)
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+        kv, ql = _host_ints(kv_lens, "kv_lens", 1), _host_ints(q_lens, "q_lens", 1)
+        table = _host_ints(block_table, "block_table", 2)
+        n = len(kv)
+        if len(ql) != n or table.shape[0] != n:
+            raise ValueError(f"block_table, kv_lens and q_lens describe {table.shape[0]}, {n} and {len(ql)} sequences")
+        if n and (kv.min() < 0 or ql.min() < 0):
+            raise ValueError("kv_lens and q_lens must be >= 0")
+        if kv.sum() >= 2 ** 31 - 256 or ql.sum() >= 2 ** 31 - 256:
+            raise ValueError("a batch holds fewer than 2^31 tokens")
+        pages = -(-kv // page_size)
+        if n and pages.max() > table.shape[1]:
+            raise ValueError(f"a sequence of {int(kv[pages.argmax()])} tokens needs {int(pages.max())} pages, "
+                             f"block_table has {table.shape[1]} per sequence")
+        used = np.arange(table.shape[1])[None] < pages[:, None]
+        ids = table[used]
+        if ids.size and (ids.min() < 0 or ids.max() >= 2 ** 31):
+            raise ValueError("block_table has a page id that is not a page of any pool")
+        self.device, self.page_size, self.n_seqs = dev, int(page_size), n
+        self.kv_lens, self.q_lens = kv, ql
+        self.n_new, self.n_tokens = int(ql.sum()), int(kv.sum())
+        self.n_pages_needed = int(ids.max()) + 1 if ids.size else 0
+        # append: every new token has a position, and its page is written by it alone
+        start = kv - ql
+        self._append_error = None
+        if n and start.min() < 0:
+            self._append_error = "append needs q_lens <= kv_lens: every new token has a position"
+        else:
+            col = np.arange(table.shape[1])[None]
+            fresh = used & (col >= (start // page_size)[:, None]) & (ql > 0)[:, None]
+            written = table[fresh]
+            listed = np.sort(ids)
+            times = np.searchsorted(listed, written, side="right") - np.searchsorted(listed, written, side="left")
+            if times.size and times.max() > 1:
+                self._append_error = "append would write a page that the block table lists more than once"
+        new_blocks = np.where(ql > 0, -(-kv // BLOCK) - np.maximum(start, 0) // BLOCK, 0)
+        blocks = -(-kv // BLOCK)
+        seqs = np.zeros((n, 8), dtype=np.int32)
+        for col, x in enumerate((kv, ql)):
+            seqs[:, col] = x
+        for col, x in enumerate((ql, kv, new_blocks, blocks)):
+            seqs[1:, 2 + col] = np.cumsum(x)[:-1]
+        self.n_new_blocks, self.n_blocks = int(new_blocks.sum()), int(blocks.sum())
+        # unused entries point at page 0, which any pool has
+        width = int(pages.max()) if n else 0
+        rows = np.where(used, table, 0)[:, :width].astype(np.int32)
+        self._upload(seqs, rows)
+
+    def _upload(self, seqs: np.ndarray, rows: np.ndarray) -> None:
+        flat = np.concatenate((seqs.ravel(), rows.ravel()))
+        with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("make the PagedBatch before the capture: its upload cannot be replayed")
+            self._dev = torch.empty(max(flat.size, 8), dtype=torch.int32, device=self.device)
+            if flat.size:
+                self._dev.copy_(torch.from_numpy(flat).pin_memory(), non_blocking=True)
+            self._ready = torch.cuda.Event()
+            self._ready.record()
+            self._made_on = torch.cuda.current_stream(self.device).cuda_stream
+        base = self._dev.data_ptr()
+        self._args = _lib.PagedBatchArgs(base + seqs.size * 4, rows.shape[1], base, self.n_new, self.n_tokens,
+                                         self.n_new_blocks, self.n_blocks, self.n_seqs, 0)
+
+    def _on_stream(self):
+        """The C arguments, safe to use on the current stream: another stream than the one
+        that uploaded them waits for the upload, and the allocator is told of it."""
+        st = torch.cuda.current_stream(self.device)
+        # a capture begins with a synchronization, so the upload before it has completed
+        if st.cuda_stream != self._made_on and not torch.cuda.is_current_stream_capturing():
+            st.wait_event(self._ready)
+            self._dev.record_stream(st)
+        return ctypes.byref(self._args)
+
+
+class PagedKVCache:
+    """One layer's pool of pages. k_pages / v_pages: uint8 [n_pages, n_heads,
+    page_size / 16, 16 * (code bytes + 2 * groups)], a block of 16 tokens of one head
+    being its 16 rows of codes and then its 16 rows of bf16 scales; k_codes, k_scales,
+    v_codes, v_scales are views of them."""
+
+    def __init__(self, n_pages: int, page_size: int, n_heads: int, head_dim: int = HEAD_DIM, k_bits: int = 4,
+                 v_bits: int = 4, group_mode: str = "bands", device="cuda"):
+        from quant_kv import _band_edges
+        dev = _cuda_device(device)
+        if head_dim != HEAD_DIM:
+            raise ValueError(f"the paged cache supports head_dim {HEAD_DIM}, got {head_dim}")
+        if (k_bits, v_bits) not in ((4, 4), (8, 4), (8, 8)):
+            raise ValueError(f"the paged cache holds K/V in 4/4, 8/4 or 8/8 bits, got {k_bits}/{v_bits}")
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+        if group_mode not in ("bands", "bands1", "bands2", "bands4", "blind32", "blind64"):
+            raise ValueError("the paged cache supports the bands, bands2, bands4, blind32 and blind64 group modes, "
+                             f"got {group_mode}")
+        if n_pages < 1 or n_heads < 1:
+            raise ValueError("n_pages and n_heads must be >= 1")
+        self.device, self.n_pages, self.page_size = dev, int(n_pages), int(page_size)
+        self.n_heads, self.head_dim = int(n_heads), int(head_dim)
+        self.k_bits, self.v_bits, self.group_mode = int(k_bits), int(v_bits), group_mode
+        self.bands = _band_edges(head_dim, group_mode)
+        self._map = np.ascontiguousarray(_kern.host_chan_band(_kern.build_chan_band(self.bands, head_dim, "cpu")),
+                                         dtype=np.int32)
+        self.k_pages, self.v_pages = (
+            torch.zeros((n_pages, n_heads, page_size // BLOCK, BLOCK * self._row_bytes(b)), dtype=torch.uint8,
+                        device=dev) for b in (k_bits, v_bits))
+
+    def _row_bytes(self, bits: int) -> int:
+        return self._code_bytes(bits) + 2 * len(self.bands)
+
+    def _code_bytes(self, bits: int) -> int:
+        return self.head_dim // 2 if bits == 4 else self.head_dim
+
+    def _codes(self, pages, bits):
+        return pages[..., :BLOCK * self._code_bytes(bits)].unflatten(-1, (BLOCK, self._code_bytes(bits)))
+
+    def _scales(self, pages, bits):
+        return pages[..., BLOCK * self._code_bytes(bits):].view(torch.bfloat16).unflatten(-1, (BLOCK, len(self.bands)))
+
+    # [n_pages, n_heads, page_size / 16, 16, code bytes or groups]
+    k_codes = property(lambda self: self._codes(self.k_pages, self.k_bits))
+    v_codes = property(lambda self: self._codes(self.v_pages, self.v_bits))
+    k_scales = property(lambda self: self._scales(self.k_pages, self.k_bits))
+    v_scales = property(lambda self: self._scales(self.v_pages, self.v_bits))
+
+    def storage_bytes(self) -> int:
+        return self.k_pages.numel() + self.v_pages.numel()
+
+    def _args(self):
+        for t in (self.k_pages, self.v_pages):
+            _require_cuda(t)
+        return ctypes.byref(_lib.PagedCacheArgs(
+            self.k_pages.data_ptr(), self.v_pages.data_ptr(), self.n_pages, self.page_size, self.n_heads,
+            self.head_dim, self.k_bits, self.v_bits, len(self.bands), self._map.ctypes.data))
+
+    def _check(self, batch: PagedBatch) -> None:
+        if not isinstance(batch, PagedBatch):
+            raise TypeError(f"expected a PagedBatch, got {type(batch).__name__}")
+        if batch.device != self.device:
+            raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
+        if batch.page_size != self.page_size:
+            raise ValueError(f"the batch has pages of {batch.page_size} tokens, the cache of {self.page_size}")
+        if batch.n_pages_needed > self.n_pages:
+            raise ValueError(f"the block table names page {batch.n_pages_needed - 1}, the cache has {self.n_pages}")
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch) -> None:
+        """Quantize the step's new tokens, k and v [n_new, n_heads, 128] bf16, into
+        their pages (kvq_paged_append): codes and scales are those of QuantKVTensor's
+        slice write; NaN is stored as 0 and infinities as the group's largest value."""
+        self._check(batch)
+        if batch._append_error:
+            raise ValueError(batch._append_error)
+        k, v = (_rows(t, (batch.n_new, self.n_heads, self.head_dim), self.device, n) for t, n in ((k, "k"), (v, "v")))
+        with torch.cuda.device(self.device):
+            rc = _lib.load().kvq_paged_append(_ptr(k), _row_stride(k), _ptr(v), _row_stride(v), self._args(),
+                                              batch._on_stream(), _stream(self.device))
+        _lib.check(rc, "kvq_paged_append")
+
+    def read(self, batch: PagedBatch, new_only: bool = False):
+        """(k, v) bf16 [n, n_heads, 128]: the values held for the sequences' tokens, or
+        for their new tokens only, sequence after sequence (kvq_paged_read)."""
+        self._check(batch)
+        if new_only and batch._append_error and (batch.q_lens > batch.kv_lens).any():
+            raise ValueError("new_only needs q_lens <= kv_lens: every new token has a position")
+        n = batch.n_new if new_only else batch.n_tokens
+        k, v = (torch.empty((n, self.n_heads, self.head_dim), dtype=torch.bfloat16, device=self.device)
+                for _ in range(2))
+        with torch.cuda.device(self.device):
+            rc = _lib.load().kvq_paged_read(self._args(), batch._on_stream(), 1 if new_only else 0, _ptr(k),
+                                            _row_stride(k), _ptr(v), _row_stride(v), _stream(self.device))
+        _lib.check(rc, "kvq_paged_read")
+        return k, v
+
+    def __repr__(self):
+        return (f"<PagedKVCache {self.n_pages} pages of {self.page_size} tokens, {self.n_heads} heads, "
+                f"int{self.k_bits}/int{self.v_bits} groups={self.group_mode} ({len(self.bands)}) on {self.device}: "
+                f"{self.storage_bytes() / 2**30:.2f} GiB resident>")
+
+
+def _rows(t, shape, device, name: str) -> torch.Tensor:
+    if _require_cuda(t) != device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]) or t.data_ptr() % 16
+                      or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1] * t.shape[2]))):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def attention(q: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, causal: bool = True, window: int = 0,
+              sink: int = 0, softmax_scale: float | None = None, out: torch.Tensor | None = None,
+              return_lse: bool = False):
+    """Attention of the new tokens' queries, q [n_new, n_q_heads, 128] bf16, over their
+    sequences' cached tokens (append the step's k and v first): bf16 like q, and with
+    return_lse also fp32 [n_new, n_q_heads], the natural log of the sum of exponentials.
+
+    Query i of a sequence stands at position p = kv_len - q_len + i; it sees tokens
+    j <= p if causal (else all), of those the last `window` (0: all) and the first
+    `sink`. A query that sees nothing gives 0, and -inf. Query head h reads KV head
+    h / (n_q_heads / n_heads); softmax_scale defaults to 1 / sqrt(128)."""
+    if not isinstance(cache, PagedKVCache):
+        raise TypeError(f"expected a PagedKVCache, got {type(cache).__name__}")
+    cache._check(batch)
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise TypeError("q must be a [n_new, n_q_heads, 128] bfloat16 tensor")
+    heads = q.shape[1]
+    if heads < 1 or heads % cache.n_heads:
+        raise ValueError(f"{heads} query heads are not a multiple of {cache.n_heads} KV heads")
+    window, sink = int(window), int(sink)
+    if window < 0 or sink < 0:
+        raise ValueError("window and sink must be >= 0")
+    if sink and not window:
+        raise ValueError("sink keeps the first tokens of a window: give window too")
+    scale = 0.0 if softmax_scale is None else float(softmax_scale)
+    if softmax_scale is not None and not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"softmax_scale must be a positive number, got {softmax_scale}")
+    shape = (batch.n_new, heads, cache.head_dim)
+    q = _rows(q, shape, cache.device, "q")
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+    elif _rows(out, shape, cache.device, "out") is not out:
+        raise ValueError("out must have contiguous [heads, channels] blocks, 16-byte aligned rows")
+    lse = torch.empty(shape[:2], dtype=torch.float32, device=cache.device) if return_lse else None
+    with torch.cuda.device(cache.device):
+        rc = _lib.load().kvq_paged_attention(_ptr(q), _row_stride(q), cache._args(), batch._on_stream(), _ptr(out),
+                                             _row_stride(out), _ptr(lse), heads, 1 if causal else 0, window, sink,
+                                             scale, _stream(cache.device))
+    _lib.check(rc, "kvq_paged_attention")
+    return (out, lse) if return_lse else out
