@@ -365,6 +365,34 @@ KVQ_API int kvq_paged_read(const kvq_paged_cache* cache, const kvq_paged_batch* 
                            int64_t k_out_token_stride, void* v_out, int64_t v_out_token_stride, void* stream);
 
 /*
+ * How one attention step over a batch is cut into work, from the host's copy of its
+ * lengths; the same for every layer of the step.
+ *
+ * Rows of a sequence and KV head are its (query, grouped head) pairs, row = query *
+ * (n_q_heads / n_heads) + grouped head, taken in row tiles; a (sequence, KV head, row
+ * tile) is a unit, which one item covers whole or several items cover in parts along
+ * the 16-token blocks that the unit sees. Parts leave partial sums in a workspace and
+ * the part that ends last joins them, in part order.
+ */
+typedef struct {
+  int32_t n_row_items, n_row_ctas; /* items of the kernel for few rows, and its blocks */
+  int32_t n_tile_items;            /* items of the kernel for many rows */
+  int32_t row_tile;                /* rows per row tile of the kernel for few rows */
+  int32_t n_units, n_slots;        /* split units (counters), parts of them */
+  int64_t words;                   /* int32 words of the plan */
+  int64_t workspace_bytes;
+} kvq_paged_plan_info;
+
+/*
+ * Writes the plan to out (HOST int32[capacity], to be copied to the device; NULL:
+ * only *info is filled). kv_lens, q_lens: HOST int32[n_seqs]. n_sms: SMs of the
+ * device that will run it. KVQ_ERR_ARG where capacity < info->words.
+ */
+KVQ_API int kvq_paged_plan(const int32_t* kv_lens, const int32_t* q_lens, int n_seqs, int n_heads, int n_q_heads,
+                           int causal, int64_t window, int64_t sink, int n_sms, int32_t* out, int64_t capacity,
+                           kvq_paged_plan_info* info);
+
+/*
  * Attention of the new tokens' queries over their sequences' cached tokens:
  * query i of a sequence stands at position p = kv_len - q_len + i and sees tokens
  *   j < kv_len,  j <= p if causal,  j > p - window or j < sink if window > 0;
@@ -373,11 +401,18 @@ KVQ_API int kvq_paged_read(const kvq_paged_cache* cache, const kvq_paged_batch* 
  *   q, out  bf16 [n_new][n_q_heads][head_dim], token strides in elements; query head
  *           h reads KV head h / (n_q_heads / n_heads)
  *   lse     fp32 [n_new][n_q_heads] or NULL: natural log of the sum of exponentials
+ *   info, plan   kvq_paged_plan() of the batch's lengths and these masks; plan is its
+ *           device copy, 16-byte aligned
+ *   workspace    device memory of info->workspace_bytes, 256-byte aligned
+ *   counters     device uint32[info->n_units], 0 before the first call that uses them;
+ *           a launch leaves them 0. Launches that may overlap need workspaces and
+ *           counters of their own.
  */
 KVQ_API int kvq_paged_attention(const void* q, int64_t q_token_stride, const kvq_paged_cache* cache,
                                 const kvq_paged_batch* batch, void* out, int64_t out_token_stride, float* lse,
                                 int n_q_heads, int causal, int64_t window, int64_t sink, float softmax_scale,
-                                void* stream);
+                                const kvq_paged_plan_info* info, const int32_t* plan, void* workspace,
+                                uint32_t* counters, void* stream);
 
 /*
  * Synchronizes the current device and returns the library's device status word:

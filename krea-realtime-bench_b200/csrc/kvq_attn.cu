@@ -1464,6 +1464,23 @@ extern "C" int kvq_test_attention_timeout(const void* q, int64_t q_token_stride,
                         stall_tile);
 }
 
+int kvq::status_word(int** ptr) {
+  static std::mutex mu;
+  static void* addr[64];
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  KVQ_REQUIRE(e == cudaSuccess, KVQ_ERR_CUDA, "cudaGetDevice failed: %s", cudaGetErrorString(e));
+  KVQ_REQUIRE(dev >= 0 && dev < 64, KVQ_ERR_DEVICE, "device %d out of range", dev);
+  std::lock_guard<std::mutex> g(mu);
+  if (!addr[dev]) {
+    e = cudaGetSymbolAddress(&addr[dev], g_attn_status);
+    KVQ_REQUIRE(e == cudaSuccess && addr[dev], KVQ_ERR_CUDA, "looking up the device status word failed: %s",
+                cudaGetErrorString(e));
+  }
+  *ptr = static_cast<int*>(addr[dev]);
+  return KVQ_OK;
+}
+
 extern "C" int kvq_device_status(int reset) {
   clear_error();
   int v = 0;

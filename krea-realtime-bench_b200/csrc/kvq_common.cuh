@@ -31,6 +31,10 @@ int check_launch(const char* what);
 // KVQ_ERR_DEVICE unless the current device is compute capability 10.x.
 int require_sm100();
 
+// Device address of the current device's status word (kvq_device_status()), looked up
+// once per device.
+int status_word(int** ptr);
+
 // ---------------------------------------------------------------- group layouts
 // The channel-group maps the reference uses (quant_kv.py:62-82), head_dim 128.
 // Each is a run of contiguous groups given by its G+1 edges.

@@ -62,6 +62,59 @@ __device__ __forceinline__ int find_seq(const Pages& p, int i) {
   return lo;
 }
 
+// One piece of attention work: rows [row0, row0 + n_rows) of a sequence and KV head
+// over entries [jb, je) of the list of storage blocks the rows see: blocks [0, n_sink),
+// then first, first + 1, ... ; part `part` of `parts`, its partial result in workspace
+// slot `slot` + part, its unit counted in counter `unit`. (kvq_paged_plan)
+struct alignas(16) Item {
+  int32_t seq, head, row0, n_rows, n_sink, first, jb, je, part, parts, unit, slot;
+  __host__ __device__ __forceinline__ int block_at(int j) const { return j < n_sink ? j : first + (j - n_sink); }
+};
+static_assert(sizeof(Item) == 48, "the plan's layout");
+
+// Workspace of one part: O [rows][128] unnormalised, then m, l per row (fp32).
+__host__ __device__ constexpr int slot_floats(int rows) { return rows * (D + 2); }
+// Most parts of a unit: joining them is serial work of one block.
+constexpr int kMaxParts = 128;
+constexpr int kRowCtasPerSm = 3;  // resident blocks of the kernel for few rows
+
+// What both attention kernels take.
+struct AttnArgs {
+  Pages p;
+  const uint16_t* q;
+  int64_t q_stride;
+  const uint8_t* k_pages;
+  const uint8_t* v_pages;
+  uint16_t* out;
+  int64_t out_stride;
+  float* lse;
+  int group, n_q_heads;
+  int causal;
+  int64_t window, sink;
+  float scale_log2;
+  const Item* items;
+  const int32_t* cta_first;
+  float* ws;
+  unsigned* ctr;
+  int* status;  // the device status word (kvq_device_status)
+  long long wait_cycles;
+};
+
+// Tokens [lo, hi) and [0, kept) that the query at position pos sees.
+struct Seen {
+  int lo, hi, kept;
+};
+__device__ __forceinline__ Seen seen_by(const AttnArgs& a, int pos, int kv_len) {
+  Seen s;
+  s.hi = a.causal ? min(pos + 1, kv_len) : kv_len;
+  const int64_t lo = a.window > 0 ? static_cast<int64_t>(pos) + 1 - a.window : 0;
+  s.lo = static_cast<int>(lo > 0 ? lo : 0);
+  s.kept = a.window > 0 ? static_cast<int>(min(a.sink, static_cast<int64_t>(s.hi > 0 ? s.hi : 0))) : 0;
+  return s;
+}
+
+int launch_rows(const AttnArgs& a, int layout, int k_bits, int v_bits, int row_tile, int n_ctas, cudaStream_t st);
+
 // Checks that hold for every entry point; fills the group layout.
 int check_cache(const kvq_paged_cache* c, const kvq_paged_batch* b, int* layout);
 Pages make_pages(const kvq_paged_cache* c, const kvq_paged_batch* b);

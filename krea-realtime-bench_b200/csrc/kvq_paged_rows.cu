@@ -1,0 +1,513 @@
+// Attention of few query rows per KV head over the paged quantized cache (sm_100a):
+// single tokens, drafts, short chunks. Memory-bound: every K and V record of a KV
+// head is read once for all its rows.
+//
+// A CTA of four warps streams its pieces of the plan (kvq_paged_plan) one after the
+// other; warp w takes every fourth 16-token storage block of a piece. A block's K and
+// V records are contiguous, so a stage of the warp's ring is filled by two bulk copies
+// (no tensor map), kStages - 1 ahead; the warps never wait for each other inside a
+// piece. Per block (tokens j, rows n, channels c; mma.sync m16n8k16, bf16 in, fp32 out):
+//   S^T[j, n] = sum_c K[j, c] q[n, c]      A = K from registers, B = q held in registers
+//   p = 2^(S^T scale - m_n)                m_n lags the true maximum by at most 8: it moves
+//                                          (and O, l are rescaled) only when some logit
+//                                          exceeds it by more, one vote per block otherwise
+//   O^T[c, n] += sum_j V[j, c] p[j, n]     A = V from registers, B = p (transposed, movmatrix)
+// Tokens are the M side, so 8 rows cost one N = 8 instruction. tcgen05 would need
+// the dequantized tile in shared memory (2 x 256 bytes per row through the shared-
+// memory port, more than it moves at memory speed); mma.sync takes it from registers.
+// Codes become values in registers, two per instruction: code bits are ored into the
+// mantissa of bf16 128 and the offset subtracted (exact), then times the bf16 scale
+// with one rounding, the value that kvq_paged_read returns. The order of channels and
+// of tokens inside a fragment is free as long as A and B agree: lane (g, t) = (lane /
+// 4, lane % 4) holds channels 32t..32t+31 of K rows and channels 16g..16g+15 of V
+// rows, 8 or 16 contiguous bytes of shared memory.
+// The warps' (m, l, O) are joined in shared memory, parts of a unit in the workspace.
+#include <cuda_bf16.h>
+
+#include <cmath>
+
+#include "kvq_paged.cuh"
+#include "kvq_sm100.cuh"
+
+namespace kvq {
+namespace paged {
+using namespace sm100;
+
+constexpr int kWarps = 4;
+constexpr int kRowThreads = 32 * kWarps;
+
+template <class L, int KB, int VB, int NT>
+struct RowGeo {
+  static constexpr int kRecK = Rec<L, KB>::kBytes, kRecV = Rec<L, VB>::kBytes;
+  static constexpr int kStage = kRecK + kRecV;
+  static constexpr int kStages = kStage <= 3072 ? 5 : kStage <= 4096 ? 4 : 3;
+  static constexpr int kRing = kStages * kStage;  // one warp's
+  static constexpr int kOffO = 0;  // the join reuses each warp's ring: 8 NT rows of 128 floats
+  static constexpr int kOffML = kWarps * kRing;
+  static constexpr int kOffBar = kOffML + kWarps * 8 * NT * 8;
+  static constexpr int kOffMisc = kOffBar + kWarps * kStages * 8;
+  static constexpr int kSmemBytes = kOffMisc + 16;
+  static_assert(kRing >= 8 * NT * D * 4, "the join fits a warp's ring");
+  static_assert(kRecK % 16 == 0 && kStage % 16 == 0, "bulk copies");
+  static_assert(kRowCtasPerSm * (kSmemBytes + 1024) <= 228 * 1024, "resident blocks");
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Nibbles at bits 0-3 and 16-19 (code = q + 8) -> bf16x2 (q, q): 128 + code - 136.
+__device__ __forceinline__ uint32_t int4_pair(uint32_t x) { return hsub2((x & 0x000F000Fu) | 0x43004300u, 0x43084308u); }
+// Bytes at bits 0-7 and 16-23 (code = q + 128) -> bf16x2 (q, q). The low seven bits give
+// 128 + code % 128, from which 256 is taken, or 128 where the top bit is set.
+__device__ __forceinline__ uint32_t int8_pair(uint32_t x) {
+  return hsub2((x & 0x007F007Fu) | 0x43004300u, (x & 0x00800080u) ^ 0x43804380u);
+}
+
+// Most channel groups that an aligned run of N channels meets.
+template <class L, int N>
+__host__ __device__ constexpr int most_groups() {
+  int most = 0;
+  for (int c = 0; c < D; c += N) {
+    int n = 0;
+    for (int g = 0; g < L::G; ++g) n += L::E[g] < c + N && L::E[g + 1] > c;
+    most = n > most ? n : most;
+  }
+  return most;
+}
+
+template <class L, int KB, int VB, int NT>
+__global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) rows_kernel(const __grid_constant__ AttnArgs a) {
+  using GEO = RowGeo<L, KB, VB, NT>;
+  constexpr int S = GEO::kStages, G = L::G;
+  constexpr int KG = most_groups<L, 32>(), VG = most_groups<L, 16>();
+  static_assert(KG <= 4 && VG <= 3, "group selection");
+  constexpr int kRows = 8 * NT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + GEO::kOffBar) + warp * S;
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + GEO::kOffMisc);
+  volatile int* last = abort + 1;
+  uint8_t* ring = smem + warp * GEO::kRing;
+  float* sm_ml = reinterpret_cast<float*>(smem + GEO::kOffML);  // [warp][row][2]
+  if (lane == 0) {
+    for (int i = 0; i < S; ++i) mbar_init(&bars[i], 1);
+    fence_mbar_init();
+  }
+  if (tid == 0) *abort = 0;
+  __syncthreads();
+
+  // this lane's channel groups: K channels 32t.., V channels 16g..
+  const int kbase = group_at<L>(32 * t), vbase = group_at<L>(16 * g);
+  uint32_t ksel[KG == 1 ? 1 : 16];
+  if constexpr (KG > 1) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int c = 32 * t + 8 * (i >> 2) + (i & 3);
+      const uint32_t la = 2 * (group_at<L>(c) - kbase), lb = 2 * (group_at<L>(c + 4) - kbase);
+      ksel[i] = la | (la + 1) << 4 | lb << 8 | (lb + 1) << 12;
+    }
+  }
+  // first channel pair of this lane's second and third V group (8: none)
+  int ve1 = 8, ve2 = 8;
+  if constexpr (VG > 1) {
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+      const int l = group_at<L>(16 * g + 2 * i) - vbase;
+      if (l >= 1) ve1 = i;
+      if (l >= 2) ve2 = i;
+    }
+  }
+  // physical token of S row r: a permutation that spreads both K and V reads over the banks
+  auto token_of = [](int r) { return r ^ ((r >> 1) & 1); };
+
+  pdl_wait();
+  pdl_launch_dependents();
+  uint32_t step = 0;  // blocks this warp has consumed, over all pieces: stage and phase
+  const int i0 = __ldg(a.cta_first + blockIdx.x), i1 = __ldg(a.cta_first + blockIdx.x + 1);
+  for (int ii = i0; ii < i1; ++ii) {
+    const Item it = a.items[ii];
+    const kvq_paged_seq sq = a.p.seqs[it.seq];
+    const int start = sq.kv_len - sq.q_len;
+    int n_mine = it.je - it.jb > warp ? (it.je - it.jb - warp + kWarps - 1) / kWarps : 0;
+    if (__any_sync(0xffffffffu, *abort)) n_mine = 0;  // a wait gave up: only the counting goes on
+    const uint32_t step0 = step;
+
+    // copies: lane i of the warp looks up the block of step base + i, 32 steps at a time
+    int64_t where = 0;
+    auto issue = [&](int k) {
+      if ((k & 31) == 0) {
+        const int kk = k + lane;
+        bool ok;
+        if (kk < n_mine) where = a.p.block(it.seq, it.head, it.block_at(it.jb + warp + kWarps * kk), ok);
+      }
+      const int64_t b = __shfl_sync(0xffffffffu, where, k & 31);
+      if (lane == 0) {
+        const uint32_t st = (step0 + k) % S;
+        const uint32_t dst = smem_u32(ring) + st * GEO::kStage;
+        mbar_arrive_expect_tx(&bars[st], GEO::kStage);
+        bulk_load(dst, a.k_pages + b * GEO::kRecK, GEO::kRecK, &bars[st]);
+        bulk_load(dst + GEO::kRecK, a.v_pages + b * GEO::kRecV, GEO::kRecV, &bars[st]);
+      }
+    };
+    for (int k = 0; k < S - 1 && k < n_mine; ++k) issue(k);
+
+    // q fragments: rows 8 nt + g, channels (32t + 8i + 2h + {0, 4}) and the next two
+    uint32_t qf[NT][8][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int n = 8 * nt + g;
+      const int row = it.row0 + min(n, it.n_rows - 1);
+      const int i = row / a.group;
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(sq.q_first + i) * a.q_stride +
+                                                        (it.head * a.group + row - i * a.group) * D + 32 * t);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint4 v = ld_global_nc_v4(src + w);
+        if (n >= it.n_rows) v = make_uint4(0, 0, 0, 0);
+        qf[nt][2 * w][0] = __byte_perm(v.x, v.z, 0x5410);
+        qf[nt][2 * w][1] = __byte_perm(v.x, v.z, 0x7632);
+        qf[nt][2 * w + 1][0] = __byte_perm(v.y, v.w, 0x5410);
+        qf[nt][2 * w + 1][1] = __byte_perm(v.y, v.w, 0x7632);
+      }
+    }
+    // what the rows 8 nt + 2t, + 2t + 1 see, and what all rows of the item see
+    Seen see[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = it.row0 + min(8 * nt + 2 * t + e, it.n_rows - 1);
+        see[nt][e] = seen_by(a, start + row / a.group, sq.kv_len);
+      }
+    const Seen first = seen_by(a, start + it.row0 / a.group, sq.kv_len);
+    const Seen final_ = seen_by(a, start + (it.row0 + it.n_rows - 1) / a.group, sq.kv_len);
+
+    float o[NT][8][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.0f;
+      m[nt][0] = m[nt][1] = -1.0e30f;
+      l[nt][0] = l[nt][1] = 0.0f;
+    }
+
+    bool ok = true;
+    for (int k = 0; k < n_mine; ++k) {
+      const uint32_t st = (step0 + k) % S;
+      if (k + S - 1 < n_mine) {
+        // stage of step k - 1: every lane has read it (the __syncwarp that ended that step)
+        issue(k + S - 1);
+      }
+      ok = mbar_wait(&bars[st], ((step0 + k) / S) & 1, abort, a.status, a.wait_cycles);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        // copies in flight land before the shared memory is given up
+        const int issued = min(n_mine, k + S);
+        for (int d = k; d < issued; ++d)
+          mbar_drain(&bars[(step0 + d) % S], ((step0 + d) / S) & 1, a.status, a.wait_cycles);
+        break;
+      }
+      const uint8_t* rk = ring + st * GEO::kStage;
+      const uint8_t* rv = rk + GEO::kRecK;
+      const int t0 = it.block_at(it.jb + warp + kWarps * k) * kBlock;
+
+      // ---- S^T
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+      uint32_t kw[2][KB == 4 ? 4 : 8], ks01[2], ks23[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int tok = 8 * r + token_of(g);
+        const uint4* src = reinterpret_cast<const uint4*>(rk + tok * Rec<L, KB>::CW) + t * (KB / 4);
+#pragma unroll
+        for (int w = 0; w < KB / 4; ++w) {
+          const uint4 v = src[w];
+          kw[r][4 * w] = v.x;
+          kw[r][4 * w + 1] = v.y;
+          kw[r][4 * w + 2] = v.z;
+          kw[r][4 * w + 3] = v.w;
+        }
+        const uint16_t* sc = reinterpret_cast<const uint16_t*>(rk + Rec<L, KB>::kCodes) + tok * G;
+        uint32_t x[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] = q < KG ? sc[KG == 1 ? kbase : min(kbase + q, G - 1)] : 0u;
+        if constexpr (KG == 1) {
+          ks01[r] = __byte_perm(x[0], 0, 0x1010);
+        } else {
+          ks01[r] = __byte_perm(x[0], x[1], 0x5410);
+          ks23[r] = __byte_perm(x[2], x[3], 0x5410);
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t f[2][4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t v;
+            if constexpr (KB == 4)
+              v = int4_pair(kw[r][w] >> (4 * j));
+            else
+              v = int8_pair(__byte_perm(kw[r][2 * w], kw[r][2 * w + 1], j | j << 4 | (4 + j) << 8 | (4 + j) << 12));
+            const uint32_t sp = KG == 1 ? ks01[r] : __byte_perm(ks01[r], ks23[r], ksel[KG == 1 ? 0 : 4 * w + j]);
+            f[r][j] = hmul2(v, sp);
+          }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma16816(s[nt], f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], qf[nt][2 * w + h][0],
+                     qf[nt][2 * w + h][1]);
+      }
+
+      // ---- softmax weights
+      const bool whole = t0 + kBlock <= first.hi && (t0 >= final_.lo || t0 + kBlock <= first.kept);
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] *= a.scale_log2;
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = t0 + 8 * (e >> 1) + token_of(g);
+            const Seen& v = see[nt][e & 1];
+            if (!(j < v.hi && (j >= v.lo || j < v.kept))) s[nt][e] = -INFINITY;
+          }
+        }
+        const float mx0 = fmaxf(s[nt][0], s[nt][2]), mx1 = fmaxf(s[nt][1], s[nt][3]);
+        if (__any_sync(0xffffffffu, mx0 > m[nt][0] + 8.0f || mx1 > m[nt][1] + 8.0f)) {
+          float n0 = mx0, n1 = mx1;
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) {
+            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
+            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+          }
+          n0 = fmaxf(n0, m[nt][0]);
+          n1 = fmaxf(n1, m[nt][1]);
+          const float a0 = ex2f(m[nt][0] - n0), a1 = ex2f(m[nt][1] - n1);
+          m[nt][0] = n0;
+          m[nt][1] = n1;
+          l[nt][0] *= a0;
+          l[nt][1] *= a1;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            o[nt][i][0] *= a0;
+            o[nt][i][1] *= a1;
+            o[nt][i][2] *= a0;
+            o[nt][i][3] *= a1;
+          }
+        }
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = ex2f(s[nt][e] - m[nt][e & 1]);
+        l[nt][0] += p[0] + p[2];
+        l[nt][1] += p[1] + p[3];
+        pf[nt][0] = transpose8x8(pack_bf16x2(p[0], p[1]));
+        pf[nt][1] = transpose8x8(pack_bf16x2(p[2], p[3]));
+      }
+
+      // ---- O^T: this lane's tokens are S rows 2t, 2t + 1, 8 + 2t, 9 + 2t
+      const int vt[4] = {token_of(2 * t), token_of(2 * t + 1), 8 + token_of(2 * t), 8 + token_of(2 * t + 1)};
+      uint32_t vw[4][VB == 4 ? 2 : 4], vs[2][VG];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if constexpr (VB == 4) {
+          const uint2 v = reinterpret_cast<const uint2*>(rv + vt[u] * Rec<L, VB>::CW)[g];
+          vw[u][0] = v.x;
+          vw[u][1] = v.y;
+        } else {
+          const uint4 v = reinterpret_cast<const uint4*>(rv + vt[u] * Rec<L, VB>::CW)[g];
+          vw[u][0] = v.x;
+          vw[u][1] = v.y;
+          vw[u][2] = v.z;
+          vw[u][3] = v.w;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < VG; ++q) {
+        uint32_t x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint16_t* sc = reinterpret_cast<const uint16_t*>(rv + Rec<L, VB>::kCodes) + vt[u] * G;
+          x[u] = sc[VG == 1 ? vbase : min(vbase + q, G - 1)];
+          // rows past the end hold anything: as zeros they add nothing
+          if (!whole && t0 + vt[u] >= sq.kv_len) x[u] = 0;
+        }
+        vs[0][q] = __byte_perm(x[0], x[1], 0x5410);
+        vs[1][q] = __byte_perm(x[2], x[3], 0x5410);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // channels 16g + 2i (rows g) and 16g + 2i + 1 (rows 8 + g)
+        uint32_t f[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t sp = vs[u][0];
+          if (VG > 1) sp = i >= ve1 ? vs[u][VG > 1 ? 1 : 0] : sp;
+          if (VG > 2) sp = i >= ve2 ? vs[u][VG > 2 ? 2 : 0] : sp;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t v;
+            if constexpr (VB == 4) {
+              const uint32_t x = __byte_perm(vw[2 * u][i >> 2], vw[2 * u + 1][i >> 2], (i & 2) ? 0x7632 : 0x5410);
+              v = int4_pair(x >> (8 * (i & 1) + 4 * e));
+            } else {
+              const int c = 2 * i + e, b = c & 3;
+              v = int8_pair(__byte_perm(vw[2 * u][c >> 2], vw[2 * u + 1][c >> 2], b | b << 4 | (4 + b) << 8 | (4 + b) << 12));
+            }
+            f[u][e] = hmul2(v, sp);
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][i], f[0][0], f[0][1], f[1][0], f[1][1], pf[nt][0], pf[nt][1]);
+      }
+      __syncwarp();
+    }
+    step = step0 + n_mine;
+
+    // ---- join the warps: each leaves (m, l, O) in its own ring, whose copies are all consumed
+    float* mine = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[nt][e];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+        const int n = 8 * nt + 2 * t + e;
+        if (g == 0) {
+          sm_ml[(warp * kRows + n) * 2] = m[nt][e];
+          sm_ml[(warp * kRows + n) * 2 + 1] = x;
+        }
+        float4* dst = reinterpret_cast<float4*>(mine + n * D + 16 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          dst[i] = make_float4(o[nt][2 * i][e], o[nt][2 * i][2 + e], o[nt][2 * i + 1][e], o[nt][2 * i + 1][2 + e]);
+      }
+    }
+    __syncthreads();
+    float* slot = it.parts > 1 ? a.ws + static_cast<int64_t>(it.slot + it.part) * slot_floats(kRows) : nullptr;
+    auto finish = [&](int n, int c, float acc, float mm, float total) {
+      const int row = it.row0 + n, i = row / a.group;
+      const int64_t tok = sq.q_first + i;
+      const int h = it.head * a.group + row - i * a.group;
+      a.out[tok * a.out_stride + h * D + c] = f32_to_bf16_bits(total == 0.0f ? 0.0f : acc / total);
+      if (a.lse && c == 0)
+        a.lse[tok * a.n_q_heads + h] = total == 0.0f ? -INFINITY : 0.69314718055994531f * (mm + log2f(total));
+    };
+    for (int n = 0; n < it.n_rows; ++n) {
+      float mw[kWarps], mm = -1.0e30f, total = 0.0f, acc = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        mw[w] = sm_ml[(w * kRows + n) * 2];
+        mm = fmaxf(mm, mw[w]);
+      }
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = ex2f(mw[w] - mm);
+        total += f * sm_ml[(w * kRows + n) * 2 + 1];
+        acc += f * reinterpret_cast<const float*>(smem + w * GEO::kRing)[n * D + tid];
+      }
+      if (slot) {
+        slot[n * D + tid] = acc;
+        if (tid == 0) {
+          slot[kRows * D + 2 * n] = mm;
+          slot[kRows * D + 2 * n + 1] = total;
+        }
+      } else {
+        finish(n, tid, acc, mm, total);
+      }
+    }
+    if (slot) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const unsigned old = atomicAdd(a.ctr + it.unit, 1u);
+        *last = old == static_cast<unsigned>(it.parts - 1);
+        if (*last) a.ctr[it.unit] = 0u;  // ready for the next launch
+      }
+      __syncthreads();
+      if (*last) {
+        __threadfence();
+        const float* base = a.ws + static_cast<int64_t>(it.slot) * slot_floats(kRows);
+        for (int n = 0; n < it.n_rows; ++n) {
+          float mm = -1.0e30f;
+          for (int p = 0; p < it.parts; ++p)
+            mm = fmaxf(mm, __ldcg(base + static_cast<int64_t>(p) * slot_floats(kRows) + kRows * D + 2 * n));
+          float total = 0.0f, acc = 0.0f;
+#pragma unroll 4
+          for (int p = 0; p < it.parts; ++p) {
+            const float* sp = base + static_cast<int64_t>(p) * slot_floats(kRows);
+            const float f = ex2f(__ldcg(sp + kRows * D + 2 * n) - mm);
+            total += f * __ldcg(sp + kRows * D + 2 * n + 1);
+            acc += f * __ldcg(sp + n * D + tid);
+          }
+          finish(n, tid, acc, mm, total);
+        }
+      }
+    }
+    // the ring was written by threads: order that before the next piece's copies into it
+    fence_proxy_async_smem();
+    __syncthreads();
+  }
+}
+
+int launch_rows(const AttnArgs& a, int layout, int k_bits, int v_bits, int row_tile, int n_ctas, cudaStream_t st) {
+  return with_layout(layout, [&](auto lt) {
+    using L = decltype(lt);
+    return with_bits(k_bits, v_bits, [&](auto bt) {
+      using B = decltype(bt);
+      auto go = [&](auto kernel, int smem, bool* configured) -> int {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (dev < 0 || dev >= 64 || !configured[dev]) {
+          cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+          KVQ_REQUIRE(e == cudaSuccess, KVQ_ERR_CUDA, "cudaFuncSetAttribute(paged rows): %s", cudaGetErrorString(e));
+          if (dev >= 0 && dev < 64) configured[dev] = true;
+        }
+        cudaError_t e = launch_pdl(kernel, static_cast<unsigned>(n_ctas), kRowThreads, smem, st, a);
+        KVQ_REQUIRE(e == cudaSuccess, KVQ_ERR_CUDA, "kvq_paged_attention: launch failed: %s", cudaGetErrorString(e));
+        return KVQ_OK;
+      };
+      static bool done1[64], done2[64];
+      if (row_tile == 8) return go(rows_kernel<L, B::k, B::v, 1>, RowGeo<L, B::k, B::v, 1>::kSmemBytes, done1);
+      return go(rows_kernel<L, B::k, B::v, 2>, RowGeo<L, B::k, B::v, 2>::kSmemBytes, done2);
+    });
+  });
+}
+
+}  // namespace paged
+}  // namespace kvq

@@ -47,7 +47,8 @@ SIGNATURES = {
     "kvq_device_status": (_i32, [_i32]),
     "kvq_paged_append": (_i32, [_p, _i64, _p, _i64, _p, _p, _p]),
     "kvq_paged_read": (_i32, [_p, _p, _i32, _p, _i64, _p, _i64, _p]),
-    "kvq_paged_attention": (_i32, [_p, _i64, _p, _p, _p, _i64, _p, _i32, _i32, _i64, _i64, _f32, _p]),
+    "kvq_paged_plan": (_i32, [_p, _p, _i32, _i32, _i32, _i32, _i64, _i64, _i32, _p, _i64, _p]),
+    "kvq_paged_attention": (_i32, [_p, _i64, _p, _p, _p, _i64, _p, _i32, _i32, _i64, _i64, _f32, _p, _p, _p, _p, _p]),
 }
 
 
@@ -61,6 +62,12 @@ class PagedBatchArgs(ctypes.Structure):
     """kvq_paged_batch"""
     _fields_ = [("table", _p), ("table_stride", _i64), ("seqs", _p), ("n_new", _i64), ("n_tokens", _i64),
                 ("n_new_blocks", _i64), ("n_blocks", _i64), ("n_seqs", _i32), ("reserved", _i32)]
+
+
+class PagedPlanInfo(ctypes.Structure):
+    """kvq_paged_plan_info"""
+    _fields_ = [("n_row_items", _i32), ("n_row_ctas", _i32), ("n_tile_items", _i32), ("row_tile", _i32),
+                ("n_units", _i32), ("n_slots", _i32), ("words", _i64), ("workspace_bytes", _i64)]
 
 
 ABI_VERSION = 3

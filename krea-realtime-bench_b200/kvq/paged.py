@@ -23,7 +23,7 @@ import torch
 import quant_kv_kernels as _kern
 
 from . import _lib
-from .ops import _ptr, _require_cuda, _stream
+from .ops import _ptr, _require_cuda
 
 BLOCK = 16  # tokens of one storage block
 PAGE_SIZES = (16, 32, 64, 128)
@@ -81,6 +81,7 @@ class PagedBatch:
         if ids.size and (ids.min() < 0 or ids.max() >= 2 ** 31):
             raise ValueError("block_table has a page id that is not a page of any pool")
         self.device, self.page_size, self.n_seqs = dev, int(page_size), n
+        self._plans = {}
         self.kv_lens, self.q_lens = kv, ql
         self.n_new, self.n_tokens = int(ql.sum()), int(kv.sum())
         self.n_pages_needed = int(ids.max()) + 1 if ids.size else 0
@@ -110,30 +111,78 @@ class PagedBatch:
         rows = np.where(used, table, 0)[:, :width].astype(np.int32)
         self._upload(seqs, rows)
 
+    def _plan(self, n_heads: int, n_q_heads: int, causal: bool, window: int, sink: int) -> "_Plan":
+        """The work list of attention with these heads and masks, made at its first use in
+        the step and shared by the step's layers."""
+        key = (n_heads, n_q_heads, causal, window, sink)
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._plans[key] = _Plan(self, *key)
+        return plan
+
     def _upload(self, seqs: np.ndarray, rows: np.ndarray) -> None:
-        flat = np.concatenate((seqs.ravel(), rows.ravel()))
-        with torch.cuda.device(self.device):
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("make the PagedBatch before the capture: its upload cannot be replayed")
-            self._dev = torch.empty(max(flat.size, 8), dtype=torch.int32, device=self.device)
-            if flat.size:
-                self._dev.copy_(torch.from_numpy(flat).pin_memory(), non_blocking=True)
-            self._ready = torch.cuda.Event()
-            self._ready.record()
-            self._made_on = torch.cuda.current_stream(self.device).cuda_stream
-        base = self._dev.data_ptr()
+        self._dev = _Uploaded(np.concatenate((seqs.ravel(), rows.ravel())), self.device)
+        base = self._dev.data.data_ptr()
         self._args = _lib.PagedBatchArgs(base + seqs.size * 4, rows.shape[1], base, self.n_new, self.n_tokens,
                                          self.n_new_blocks, self.n_blocks, self.n_seqs, 0)
 
-    def _on_stream(self):
-        """The C arguments, safe to use on the current stream: another stream than the one
-        that uploaded them waits for the upload, and the allocator is told of it."""
-        st = torch.cuda.current_stream(self.device)
-        # a capture begins with a synchronization, so the upload before it has completed
-        if st.cuda_stream != self._made_on and not torch.cuda.is_current_stream_capturing():
-            st.wait_event(self._ready)
-            self._dev.record_stream(st)
+    def _on_stream(self, stream):
+        self._dev.use(stream)
         return ctypes.byref(self._args)
+
+
+class _Uploaded:
+    """int32 data copied to the device on the stream that is current when it is made."""
+
+    def __init__(self, flat: np.ndarray, device: torch.device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("call this once before the capture: its upload cannot be replayed")
+        self.data = torch.empty(max(flat.size, 8), dtype=torch.int32, device=device)
+        if flat.size:
+            self.data[:flat.size].copy_(torch.from_numpy(flat).pin_memory(), non_blocking=True)
+        self._event = torch.cuda.Event()
+        self._stream = torch.cuda.current_stream(device)
+        self._event.record(self._stream)
+
+    def use(self, stream) -> None:
+        """Makes the data safe to read on `stream`: another stream than the one that
+        uploaded it waits for the upload, and the allocator is told of it. A capture
+        begins with a synchronization, so an upload before it has completed."""
+        if stream != self._stream and not torch.cuda.is_current_stream_capturing():
+            stream.wait_event(self._event)
+            self.data.record_stream(stream)
+
+
+class _Plan:
+    """kvq_paged_plan of a batch: the work list on the device, and per stream a workspace
+    and counters, so that launches on different streams may overlap."""
+
+    def __init__(self, batch: PagedBatch, n_heads: int, n_q_heads: int, causal: bool, window: int, sink: int):
+        kv, ql = batch.kv_lens.astype(np.int32), batch.q_lens.astype(np.int32)
+        self.info = _lib.PagedPlanInfo()
+        sms = torch.cuda.get_device_properties(batch.device).multi_processor_count
+        lib = _lib.load()
+        words = np.empty(0, dtype=np.int32)
+        for _ in range(2):  # its size, then the plan
+            rc = lib.kvq_paged_plan(kv.ctypes.data, ql.ctypes.data, len(kv), n_heads, n_q_heads, causal, window, sink, sms,
+                                    words.ctypes.data if words.size else None, words.size, ctypes.byref(self.info))
+            _lib.check(rc, "kvq_paged_plan")
+            if words.size == 0:
+                words = np.empty(self.info.words, dtype=np.int32)
+        self.device = batch.device
+        self.items = _Uploaded(words, batch.device)
+        self._work = {}
+
+    def args(self, stream):
+        self.items.use(stream)
+        work = self._work.get(stream.cuda_stream)
+        if work is None:
+            n, c = self.info.workspace_bytes, self.info.n_units
+            # counters count up to a unit's parts and are set back by the last one
+            work = (torch.empty(n, dtype=torch.uint8, device=self.device) if n else None,
+                    torch.zeros(c, dtype=torch.int32, device=self.device) if c else None)
+            self._work[stream.cuda_stream] = work
+        return ctypes.byref(self.info), _ptr(self.items.data), _ptr(work[0]), _ptr(work[1])
 
 
 class PagedKVCache:
@@ -214,8 +263,9 @@ class PagedKVCache:
             raise ValueError(batch._append_error)
         k, v = (_rows(t, (batch.n_new, self.n_heads, self.head_dim), self.device, n) for t, n in ((k, "k"), (v, "v")))
         with torch.cuda.device(self.device):
+            stream = torch.cuda.current_stream()
             rc = _lib.load().kvq_paged_append(_ptr(k), _row_stride(k), _ptr(v), _row_stride(v), self._args(),
-                                              batch._on_stream(), _stream(self.device))
+                                              batch._on_stream(stream), stream.cuda_stream)
         _lib.check(rc, "kvq_paged_append")
 
     def read(self, batch: PagedBatch, new_only: bool = False):
@@ -228,8 +278,9 @@ class PagedKVCache:
         k, v = (torch.empty((n, self.n_heads, self.head_dim), dtype=torch.bfloat16, device=self.device)
                 for _ in range(2))
         with torch.cuda.device(self.device):
-            rc = _lib.load().kvq_paged_read(self._args(), batch._on_stream(), 1 if new_only else 0, _ptr(k),
-                                            _row_stride(k), _ptr(v), _row_stride(v), _stream(self.device))
+            stream = torch.cuda.current_stream()
+            rc = _lib.load().kvq_paged_read(self._args(), batch._on_stream(stream), 1 if new_only else 0, _ptr(k),
+                                            _row_stride(k), _ptr(v), _row_stride(v), stream.cuda_stream)
         _lib.check(rc, "kvq_paged_read")
         return k, v
 
@@ -291,8 +342,10 @@ def attention(q: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, causal: b
         raise ValueError("out must have contiguous [heads, channels] blocks, 16-byte aligned rows")
     lse = torch.empty(shape[:2], dtype=torch.float32, device=cache.device) if return_lse else None
     with torch.cuda.device(cache.device):
-        rc = _lib.load().kvq_paged_attention(_ptr(q), _row_stride(q), cache._args(), batch._on_stream(), _ptr(out),
+        stream = torch.cuda.current_stream()
+        plan = batch._plan(cache.n_heads, heads, bool(causal), window, sink)
+        rc = _lib.load().kvq_paged_attention(_ptr(q), _row_stride(q), cache._args(), batch._on_stream(stream), _ptr(out),
                                              _row_stride(out), _ptr(lse), heads, 1 if causal else 0, window, sink,
-                                             scale, _stream(cache.device))
+                                             scale, *plan.args(stream), stream.cuda_stream)
     _lib.check(rc, "kvq_paged_attention")
     return (out, lse) if return_lse else out
