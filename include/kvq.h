@@ -378,9 +378,9 @@ typedef struct {
   int32_t n_row_items, n_row_ctas; /* items of the kernel for few rows, and its blocks */
   int32_t n_tile_items;            /* items of the kernel for many rows */
   int32_t row_tile;                /* rows per row tile of the kernel for few rows */
-  int32_t n_units, n_slots;        /* split units (counters), parts of them */
+  int32_t n_units, reserved;       /* split units (counters) */
   int64_t words;                   /* int32 words of the plan */
-  int64_t workspace_bytes;
+  int64_t workspace_bytes, tile_workspace_offset;
 } kvq_paged_plan_info;
 
 /*

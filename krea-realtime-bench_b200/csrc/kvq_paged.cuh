@@ -113,6 +113,12 @@ __device__ __forceinline__ Seen seen_by(const AttnArgs& a, int pos, int kv_len) 
   return s;
 }
 
+// Workspace of one part in the kernel for many rows: two Q tiles of float4 [33][128 rows],
+// 32 columns of O and one of (m, l).
+constexpr int kTileRows = 256;
+constexpr int64_t kTileSlotBytes = 2 * 33 * 128 * 16;
+
+int launch_tiles(const AttnArgs& a, int layout, int k_bits, int v_bits, int n_items, cudaStream_t st);
 int launch_rows(const AttnArgs& a, int layout, int k_bits, int v_bits, int row_tile, int n_ctas, cudaStream_t st);
 
 // Checks that hold for every entry point; fills the group layout.

@@ -58,6 +58,13 @@ extern "C" int kvq_paged_attention(const void* q, int64_t q_token_stride, const 
   rc = status_word(&a.status);
   if (rc) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (info->n_tile_items > 0) {
+    paged::AttnArgs t = a;
+    t.items += info->n_row_items;
+    t.ws = reinterpret_cast<float*>(static_cast<char*>(workspace) + info->tile_workspace_offset);
+    rc = paged::launch_tiles(t, layout, cache->k_bits, cache->v_bits, info->n_tile_items, st);
+    if (rc) return rc;
+  }
   if (info->n_row_ctas > 0) {
     rc = paged::launch_rows(a, layout, cache->k_bits, cache->v_bits, info->row_tile, info->n_row_ctas, st);
     if (rc) return rc;

@@ -31,7 +31,7 @@ static Unit make_unit(int seq, int kv_len, int q_len, int group, int row0, int n
 struct Plan {
   std::vector<Item> rows, tiles;
   std::vector<int32_t> cta_first;
-  int units = 0, slots = 0, row_tile = 8;
+  int units = 0, slots = 0, tile_slots = 0, row_tile = 8;
 };
 
 // Few rows: the work of all units is one line of blocks (an empty unit counts as
@@ -76,21 +76,54 @@ static void cut_rows(const std::vector<Unit>& units, int n_heads, int n_sms, Pla
     p->cta_first.push_back(static_cast<int32_t>(p->rows.size()));
 }
 
+// Many rows: one block of the device per item and SM, started in the order of the list.
+// Long units first, whole while much work is left; later ones are cut so that no piece is
+// longer than an equal share of the work that is left, and the last ones to run
+// end together. No piece is shorter than kMinTiles tiles of four storage blocks, no
+// unit has more than kMaxTileParts parts (their join is serial work of one block).
+constexpr int kMinTiles = 8, kMaxTileParts = 32;
+
+static void cut_tiles(std::vector<Unit>& units, int n_heads, int n_sms, Plan* p) {
+  std::stable_sort(units.begin(), units.end(), [](const Unit& a, const Unit& b) { return a.n > b.n; });
+  int64_t left = 0;
+  for (const Unit& u : units) left += static_cast<int64_t>((u.n + 3) / 4) * n_heads;
+  for (const Unit& u : units) {
+    const int64_t t = (u.n + 3) / 4;
+    for (int h = 0; h < n_heads; ++h, left -= t) {
+      const int64_t piece = std::max<int64_t>(kMinTiles, left / n_sms);
+      const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((t + piece - 1) / piece, kMaxTileParts)));
+      for (int i = 0; i < parts; ++i)
+        p->tiles.push_back(Item{u.seq, h, u.row0, u.n_rows, u.n_sink, u.first, static_cast<int32_t>(4 * (t * i / parts)),
+                                static_cast<int32_t>(std::min<int64_t>(u.n, 4 * (t * (i + 1) / parts))), i, parts,
+                                parts > 1 ? p->units : -1, parts > 1 ? p->tile_slots : -1});
+      if (parts > 1) {
+        ++p->units;
+        p->tile_slots += parts;
+      }
+    }
+  }
+}
+
+// Up to kFewRows rows of a sequence and KV head go to the kernel for few rows.
+constexpr int kFewRows = 16;
+
 static int make_plan(const int32_t* kv_lens, const int32_t* q_lens, int n_seqs, int n_heads, int group, int causal,
                      int64_t window, int64_t sink, int n_sms, Plan* p) {
-  int64_t most_rows = 0;
-  for (int s = 0; s < n_seqs; ++s)
-    most_rows = std::max<int64_t>(most_rows, static_cast<int64_t>(q_lens[s]) * group);
-  p->row_tile = most_rows <= 8 ? 8 : 16;
-  std::vector<Unit> units;
+  std::vector<Unit> few, many;
   for (int s = 0; s < n_seqs; ++s) {
     const int64_t rows = static_cast<int64_t>(q_lens[s]) * group;
-    for (int64_t r = 0; r < rows; r += p->row_tile)
-      units.push_back(make_unit(s, kv_lens[s], q_lens[s], group, static_cast<int>(r),
-                                static_cast<int>(std::min<int64_t>(p->row_tile, rows - r)), causal, window, sink));
+    const int tile = rows <= kFewRows ? kFewRows : kTileRows;
+    for (int64_t r = 0; r < rows; r += tile) {
+      const int n = static_cast<int>(std::min<int64_t>(tile, rows - r));
+      (rows <= kFewRows ? few : many)
+          .push_back(make_unit(s, kv_lens[s], q_lens[s], group, static_cast<int>(r), n, causal, window, sink));
+      if (rows <= kFewRows && rows > 8) p->row_tile = 16;
+    }
   }
-  KVQ_REQUIRE(static_cast<int64_t>(units.size()) * n_heads < (1 << 26), KVQ_ERR_ARG, "too many rows for one launch");
-  cut_rows(units, n_heads, n_sms, p);
+  KVQ_REQUIRE(static_cast<int64_t>(few.size() + many.size()) * n_heads < (1 << 24), KVQ_ERR_ARG,
+              "too many rows for one launch");
+  cut_rows(few, n_heads, n_sms, p);
+  cut_tiles(many, n_heads, n_sms, p);
   return KVQ_OK;
 }
 
@@ -123,9 +156,9 @@ extern "C" int kvq_paged_plan(const int32_t* kv_lens, const int32_t* q_lens, int
     info->n_tile_items = static_cast<int32_t>(p.tiles.size());
     info->row_tile = p.row_tile;
     info->n_units = p.units;
-    info->n_slots = p.slots;
     info->words = static_cast<int64_t>(p.rows.size() + p.tiles.size()) * 12 + static_cast<int64_t>(p.cta_first.size());
-    info->workspace_bytes = static_cast<int64_t>(p.slots) * paged::slot_floats(p.row_tile) * 4;
+    info->tile_workspace_offset = (static_cast<int64_t>(p.slots) * paged::slot_floats(p.row_tile) * 4 + 255) / 256 * 256;
+    info->workspace_bytes = info->tile_workspace_offset + p.tile_slots * paged::kTileSlotBytes;
     if (!out) return KVQ_OK;
     KVQ_REQUIRE(capacity >= info->words, KVQ_ERR_ARG, "the plan needs %lld words", (long long)info->words);
     auto put = [&out](const void* src, size_t words) {

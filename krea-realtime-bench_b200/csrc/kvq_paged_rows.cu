@@ -22,12 +22,9 @@
 // 4, lane % 4) holds channels 32t..32t+31 of K rows and channels 16g..16g+15 of V
 // rows, 8 or 16 contiguous bytes of shared memory.
 // The warps' (m, l, O) are joined in shared memory, parts of a unit in the workspace.
-#include <cuda_bf16.h>
-
 #include <cmath>
 
-#include "kvq_paged.cuh"
-#include "kvq_sm100.cuh"
+#include "kvq_paged_dev.cuh"
 
 namespace kvq {
 namespace paged {
@@ -52,11 +49,6 @@ struct RowGeo {
   static_assert(kRowCtasPerSm * (kSmemBytes + 1024) <= 228 * 1024, "resident blocks");
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -69,39 +61,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-// Nibbles at bits 0-3 and 16-19 (code = q + 8) -> bf16x2 (q, q): 128 + code - 136.
-__device__ __forceinline__ uint32_t int4_pair(uint32_t x) { return hsub2((x & 0x000F000Fu) | 0x43004300u, 0x43084308u); }
-// Bytes at bits 0-7 and 16-23 (code = q + 128) -> bf16x2 (q, q). The low seven bits give
-// 128 + code % 128, from which 256 is taken, or 128 where the top bit is set.
-__device__ __forceinline__ uint32_t int8_pair(uint32_t x) {
-  return hsub2((x & 0x007F007Fu) | 0x43004300u, (x & 0x00800080u) ^ 0x43804380u);
-}
-
-// Most channel groups that an aligned run of N channels meets.
-template <class L, int N>
-__host__ __device__ constexpr int most_groups() {
-  int most = 0;
-  for (int c = 0; c < D; c += N) {
-    int n = 0;
-    for (int g = 0; g < L::G; ++g) n += L::E[g] < c + N && L::E[g + 1] > c;
-    most = n > most ? n : most;
-  }
-  return most;
-}
-
 template <class L, int KB, int VB, int NT>
 __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) rows_kernel(const __grid_constant__ AttnArgs a) {
   using GEO = RowGeo<L, KB, VB, NT>;

@@ -1,0 +1,616 @@
+// Attention of many query rows per KV head over the paged quantized cache (sm_100a):
+// prompt chunks, denoising blocks. Tensor-bound: tcgen05.mma with TMEM accumulators.
+//
+// One CTA of 16 warps per item of the plan: up to 256 rows (two Q tiles of 128) of a
+// sequence and KV head, row = query * group + grouped head, over its list of 16-token
+// storage blocks; a KV tile is four consecutive entries of that list (64 tokens), so the
+// kept first tokens and a sliding window need no tokens between them.
+//   warps 0-3 / 4-7  softmax of Q tile 0 / 1: thread r owns row r (TMEM lane r); all
+//                    eight first gather the Q rows (cp.async into the MMA's layout)
+//   warps 8-9/10-11  converters of K / V: four lanes per row, 32 channels each, codes and
+//                    scales from the staged records to 128B-swizzled bf16 tiles
+//   warps 12 / 15    producers of K / V: a storage block is contiguous, one bulk copy
+//   warps 13 / 14    one thread each issuing the tcgen05.mma of Q tile 0 / 1:
+//                    S_x = Q_x K^T (M128 N64 K128), O_x += P_x V (M128 N128 K64, P in TMEM)
+// The pipeline is that of the contiguous-window attention kernel (S double-buffered,
+// S_x(j+2) issued behind PV_x(j), one commit per tile and Q tile, K and V as separate
+// streams): see there for what was measured. What differs: rows of different lengths
+// of sight. A tile that some row of the Q tile does not see whole takes a masked step
+// (a 64-bit mask per row; a masked logit is -inf); the running maximum starts at -1e30,
+// so a row without any visible token ends with l = 0 and is stored as 0.
+// K, V, P are rounded to bf16 for the MMA: codes * scale as kvq_paged_read returns
+// them, weights once; S, m, l, O are fp32.
+#include <cmath>
+
+#include "kvq_paged_dev.cuh"
+
+namespace kvq {
+namespace paged {
+using namespace sm100;
+namespace tiles {
+
+constexpr int BM = 128, BN = 64;
+constexpr int kThreads = 512;
+constexpr int kConvWarp0 = 8, kProdWarp = 12, kMmaWarp = 13, kProdWarpV = 15;
+constexpr uint32_t kTmemCols = 512, kColO = 0, kColS = 256;
+constexpr int kKVTile = BN * D * 2;  // 16 KB: two SWIZZLE_128B atoms (channels 0-63, 64-127)
+constexpr int kAtom = BN * 128;
+constexpr int kQTile = BM * D * 2;
+constexpr int kQAtom = BM * 128;
+
+// Shared memory: bf16 stages of K and V, staged records, the Q tiles. Four bf16
+// stages per tensor and three staged tiles where the codes are small; int8 codes leave
+// room for two, and with both tensors int8 for three bf16 stages of V.
+template <class L, int KB, int VB>
+struct Geo {
+  static constexpr int kRecK = Rec<L, KB>::kBytes, kRecV = Rec<L, VB>::kBytes;
+  static constexpr int kStageK = 4 * kRecK, kStageV = 4 * kRecV;
+  static constexpr int NK = 4, NV = VB == 8 ? 3 : 4;
+  static constexpr int LK = KB == 8 ? 2 : 3, LV = KB == 8 ? 2 : 3;
+  static constexpr int kOffK = 0;
+  static constexpr int kOffV = kOffK + NK * kKVTile;
+  static constexpr int kOffQ = kOffV + NV * kKVTile;
+  static constexpr int kOffCK = kOffQ + 2 * kQTile;
+  static constexpr int kOffCV = kOffCK + LK * kStageK;
+  static constexpr int kOffBar = (kOffCV + LV * kStageV + 15) / 16 * 16;
+  // barriers; index + stages of K for V
+  static constexpr int bLdFull = 0, bLdEmpty = bLdFull + LK + LV, bKvFull = bLdEmpty + LK + LV,
+                       bKvEmpty = bKvFull + NK + NV, bQReady = bKvEmpty + NK + NV, bSFull = bQReady + 2,
+                       bPFull = bSFull + 4, bOReady = bPFull + 4, bOFinal = bOReady + 2, bMmaDone = bOFinal + 2,
+                       kNumBars = bMmaDone + 2;
+  static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+  static constexpr int kSmemBytes = kOffMisc + 32 + 1024;  // + alignment slack
+  static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM must fit");
+  static_assert(kOffCK % 16 == 0 && kOffCV % 16 == 0, "bulk copies");
+};
+
+__device__ __forceinline__ uint32_t tile_off(int r, int c) {
+  return static_cast<uint32_t>((c >> 3) * kAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_shared_u16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Converters: four lanes per row, lane t channels 32t..32t+31.
+template <class L, int BITS>
+struct Converter {
+  static constexpr int KG = most_groups<L, 32>();
+  int base;
+  uint32_t sel[KG == 1 ? 1 : 16];
+  // Lanes 2 and 3 of a row write atom 1: taking their 16-byte chunks in the order 2, 3, 0,
+  // 1 keeps the eight lanes of a store phase on different banks.
+  __device__ __forceinline__ void init(int t) {
+    base = group_at<L>(32 * t);
+    if constexpr (KG > 1) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int w = (i >> 2) ^ (t & 2);
+        const uint32_t l = 2 * (group_at<L>(32 * t + 8 * w + 2 * (i & 3)) - base);
+        sel[i] = l | (l + 1) << 4 | l << 8 | (l + 1) << 12;
+      }
+    }
+  }
+  // One row: record block `rec`, row `rr` of it, to row r of the bf16 tile at dst.
+  __device__ __forceinline__ void row(uint32_t rec, int rr, uint32_t dst, int r, int t, bool live) const {
+    using R = Rec<L, BITS>;
+    uint32_t w[BITS];  // 4 or 8 words of codes
+    const uint32_t src = rec + rr * R::CW + t * (R::CW / 4);
+#pragma unroll
+    for (int i = 0; i < BITS / 4; ++i) {
+      const uint4 v = ld_shared_v4(src + 16 * i);
+      w[4 * i] = v.x;
+      w[4 * i + 1] = v.y;
+      w[4 * i + 2] = v.z;
+      w[4 * i + 3] = v.w;
+    }
+    const uint32_t sc = rec + R::kCodes + rr * L::G * 2;
+    uint32_t s01, s23 = 0;
+    if constexpr (KG == 1) {
+      s01 = __byte_perm(ld_shared_u16(sc + 2 * base), 0, 0x1010);
+    } else {
+      uint32_t x[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] = q < KG ? ld_shared_u16(sc + 2 * min(base + q, L::G - 1)) : 0u;
+      s01 = __byte_perm(x[0], x[1], 0x5410);
+      if constexpr (KG > 2) s23 = __byte_perm(x[2], x[3], 0x5410);
+    }
+    if (!live) s01 = s23 = 0;  // rows past the end hold anything: as zeros they add nothing
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int hi = t & 2;  // word i ^ hi
+      uint32_t o[4];
+      if constexpr (BITS == 4) {
+        const uint32_t x = hi ? w[i ^ 2] : w[i], y = x >> 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = int4_pair(__byte_perm(x, y, (4 + j) << 8 | j));
+      } else {
+        const uint32_t x = hi ? w[2 * (i ^ 2)] : w[2 * i], y = hi ? w[2 * (i ^ 2) + 1] : w[2 * i + 1];
+        o[0] = int8_pair(__byte_perm(x, 0, 0x4140));
+        o[1] = int8_pair(__byte_perm(x, 0, 0x4342));
+        o[2] = int8_pair(__byte_perm(y, 0, 0x4140));
+        o[3] = int8_pair(__byte_perm(y, 0, 0x4342));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = hmul2(o[j], KG == 1 ? s01 : __byte_perm(s01, s23, sel[KG == 1 ? 0 : 4 * i + j]));
+      st_shared_v4(dst + tile_off(r, 4 * t + (i ^ hi)), o[0], o[1], o[2], o[3]);
+    }
+  }
+};
+
+template <class L, int KB, int VB>
+__global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constant__ AttnArgs a) {
+  using GEO = Geo<L, KB, VB>;
+  constexpr int NK = GEO::NK, NV = GEO::NV, LK = GEO::LK, LV = GEO::LV;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + GEO::kOffBar);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + GEO::kOffMisc);
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + GEO::kOffMisc + 8);
+  volatile int* last = abort + 1;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const long long lim = a.wait_cycles;
+  pdl_wait();
+  pdl_launch_dependents();
+  const Item it = a.items[blockIdx.x];
+  const kvq_paged_seq sq = a.p.seqs[it.seq];
+  const int start = sq.kv_len - sq.q_len;
+  const int nq = it.n_rows > BM ? 2 : 1;
+  const int n_blk = it.je - it.jb;  // entries of the block list
+  const int nkv = (n_blk + 3) / 4;
+
+  if (tid == 0) {
+    for (int i = 0; i < LK + LV; ++i) {
+      mbar_init(&bars[GEO::bLdFull + i], 1);
+      mbar_init(&bars[GEO::bLdEmpty + i], 2);  // the tensor's two converter warps
+    }
+    for (int i = 0; i < NK + NV; ++i) {
+      mbar_init(&bars[GEO::bKvFull + i], 2);
+      mbar_init(&bars[GEO::bKvEmpty + i], nq);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&bars[GEO::bQReady + x], 8);  // the eight gathering warps
+      mbar_init(&bars[GEO::bSFull + 2 * x], 1);
+      mbar_init(&bars[GEO::bSFull + 2 * x + 1], 1);
+      mbar_init(&bars[GEO::bPFull + 2 * x], 4);
+      mbar_init(&bars[GEO::bPFull + 2 * x + 1], 4);
+      mbar_init(&bars[GEO::bOReady + x], 1);
+      mbar_init(&bars[GEO::bOFinal + x], 1);
+      mbar_init(&bars[GEO::bMmaDone + x], 1);
+    }
+    *abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // where row n of the item reads its query and writes its output
+  auto place = [&](int n, int64_t& tok, int& h) {
+    const int row = it.row0 + n, i = row / a.group;
+    tok = sq.q_first + i;
+    h = it.head * a.group + row - i * a.group;
+  };
+  // A warp's 32 output rows (rows n0.. of the item, rr0.. of the Q tile), staged in
+  // the Q buffer, to global memory: half a warp per row, 256 contiguous bytes.
+  auto store_rows = [&](uint32_t stage, int rr0, int n0) {
+#pragma unroll 4
+    for (int k = 0; k < 16; ++k) {
+      const int rr = rr0 + 2 * k + (lane >> 4), n = n0 + 2 * k + (lane >> 4), c = lane & 15;
+      if (n < it.n_rows) {
+        int64_t tok;
+        int h;
+        place(n, tok, h);
+        const uint4 v = ld_shared_v4(stage + (c >> 3) * kQAtom + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
+        st_global_v4(a.out + tok * a.out_stride + h * D + 8 * c, v);
+      }
+    }
+  };
+  auto stage_chunk = [&](uint32_t stage, int r, int ch, const float* v, float inv) {
+    st_shared_v4(stage + (ch >> 3) * kQAtom + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
+                 pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv),
+                 pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
+  };
+  auto store_lse = [&](int n, float m, float l) {
+    if (a.lse && n < it.n_rows) {
+      int64_t tok;
+      int h;
+      place(n, tok, h);
+      a.lse[tok * a.n_q_heads + h] = l == 0.0f ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
+    }
+  };
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ Q, by all eight softmax warps
+    for (int k = 0; k < 8 * nq; ++k) {
+      const int n = 16 * k + (tid >> 4), c = tid & 15, r = n & (BM - 1);
+      const uint32_t dst = sbase + GEO::kOffQ + (n >> 7) * kQTile + (c >> 3) * kQAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+      if (n < it.n_rows) {
+        int64_t tok;
+        int h;
+        place(n, tok, h);
+        cp_async16(dst, a.q + tok * a.q_stride + h * D + 8 * c);
+      } else {
+        st_shared_v4(dst, 0, 0, 0, 0);
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(&bars[GEO::bQReady]);
+      mbar_arrive(&bars[GEO::bQReady + 1]);
+    }
+  }
+  if (warp < 4 * nq) {
+    // ------------------------------------------------------------ softmax (Q tile x)
+    const int x = warp >> 2;
+    const int r = tid - x * BM;
+    const int n = x * BM + r;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tO = tmem + lane_off + kColO + 128 * x;
+    const uint32_t tS0 = tmem + lane_off + kColS + 128 * x;
+    const int n_last = min(x * BM + BM, it.n_rows) - 1;
+    const Seen see = seen_by(a, start + (it.row0 + min(n, it.n_rows - 1)) / a.group, sq.kv_len);
+    const Seen first = seen_by(a, start + (it.row0 + x * BM) / a.group, sq.kv_len);
+    const Seen fin = seen_by(a, start + (it.row0 + n_last) / a.group, sq.kv_len);
+    float m = -1.0e30f, l = 0.0f;
+    bool ok = true;
+    auto step = [&](const int j, auto masked) -> bool {
+      constexpr bool MASK = decltype(masked)::value;
+      const uint32_t tS = tS0 + 64 * (j & 1);
+      if (!mbar_wait_warp(&bars[GEO::bSFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim)) return false;
+      // S_x(j) complete: this Q tile no longer reads K stage j, and PV_x(j-2) (issued
+      // before it) is complete: nor V stage j-2
+      if ((warp & 3) == 0 && lane == 0) {
+        mbar_arrive(&bars[GEO::bKvEmpty + j % NK]);
+        if (j >= 2) mbar_arrive(&bars[GEO::bKvEmpty + NK + (j - 2) % NV]);
+      }
+      tc_fence_after();
+      uint32_t s0[32], s1[32];
+      tmem_ld32x2_wait(tS, tS + 32, s0, s1);
+      if constexpr (MASK) {
+        uint32_t mk[2] = {0, 0};  // bit c: column c is seen
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int e = it.jb + 4 * j + b;
+          if (e < it.je) {
+            const int tb = it.block_at(e) * kBlock;
+            auto below = [&](int lim_) { return (1u << max(0, min(kBlock, lim_ - tb))) - 1u; };
+            const uint32_t bits = below(see.hi) & (~below(see.lo) | below(see.kept)) & 0xFFFFu;
+            mk[b >> 1] |= bits << (16 * (b & 1));
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          if (!((mk[0] >> c) & 1u)) s0[c] = 0xFF800000u;  // -inf
+          if (!((mk[1] >> c) & 1u)) s1[c] = 0xFF800000u;
+        }
+      }
+      float pm[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pm[i] = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 32; ++c) pm[c & 7] = fmax3(pm[c & 7], __uint_as_float(s0[c]), __uint_as_float(s1[c]));
+      const float mt =
+          fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * a.scale_log2;
+      bool rescale = false;
+      float alpha = 1.0f;
+      if (j == 0) {
+        m = fmaxf(m, mt);
+      } else if (mt > m + 8.0f) {
+        rescale = true;
+        alpha = ex2f(m - mt);
+        m = mt;
+        l *= alpha;
+      }
+      const float nm = -m;
+      uint32_t pw[32];
+      const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(nm, nm);
+      float2 sum2 = make_float2(0.0f, 0.0f);
+      auto half = [&](const uint32_t (&sv)[32], int base) {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const float2 xx =
+              __ffma2_rn(make_float2(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), sc2, nm2);
+          const float p0 = ex2f(xx.x), p1 = ex2f(xx.y);
+          sum2 = __fadd2_rn(sum2, make_float2(p0, p1));
+          pw[base / 2 + c] = pack_bf16x2(p0, p1);
+        }
+      };
+      half(s0, 0);
+      tmem_st16(tS, pw);
+      half(s1, 32);
+      tmem_st16(tS + 16, pw + 16);
+      l += sum2.x + sum2.y;
+      if (__any_sync(0xffffffffu, rescale)) {
+        // O_x must hold every product up to PV_x(j-1) before it is rescaled: wait for
+        // S_x(j+1), issued behind PV_x(j-1), or at the last tile for the commit behind it
+        const bool tail = j + 1 == nkv;
+        if (!mbar_wait_warp(&bars[tail ? GEO::bOReady + x : GEO::bSFull + 2 * x + ((j + 1) & 1)],
+                            tail ? 0u : static_cast<uint32_t>(((j + 1) >> 1) & 1), abort, a.status, lim))
+          return false;
+        tc_fence_after();
+#pragma unroll 1
+        for (int k = 0; k < 8; ++k) {
+          uint32_t o[16];
+          tmem_ld16_wait(tO + 16 * k, o);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+          tmem_st16(tO + 16 * k, o);
+        }
+        tmem_wait_st();
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[GEO::bPFull + 2 * x + (j & 1)]);
+      return true;
+    };
+    for (int j = 0; j < nkv && ok; ++j) {
+      const int e0 = it.jb + 4 * j;
+      const int ta = it.block_at(e0) * kBlock, tz = it.block_at(e0 + 3) * kBlock + kBlock;
+      const bool whole = e0 + 4 <= it.je && tz <= first.hi && (ta >= fin.lo || tz <= first.kept);
+      ok = whole ? step(j, std::false_type{}) : step(j, std::true_type{});
+    }
+    const bool done = ok && nkv > 0 && mbar_wait_warp(&bars[GEO::bOFinal + x], 0, abort, a.status, lim);
+    if (it.parts > 1) {
+      // one part of a unit: unnormalised O row, m and l for the join. float4 column c of
+      // row r at [c][r]: a warp's 32 rows are contiguous
+      tc_fence_after();
+      float4* dst = reinterpret_cast<float4*>(a.ws) + (static_cast<int64_t>(it.slot + it.part) * 2 + x) * 33 * BM + r;
+#pragma unroll 1
+      for (int k = 0; k < 4; ++k) {
+        uint32_t o[32];
+        if (done) tmem_ld32_wait(tO + 32 * k, o);
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          dst[(8 * k + c) * BM] = done ? make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]),
+                                                     __uint_as_float(o[4 * c + 2]), __uint_as_float(o[4 * c + 3]))
+                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+      dst[32 * BM] = make_float4(m, l, 0.0f, 0.0f);
+      __threadfence();
+    } else if (done || (nkv == 0 && mbar_wait_warp(&bars[GEO::bQReady + x], 0, abort, a.status, lim))) {
+      // (no tiles: Q_x has landed before its buffer is reused below)
+      tc_fence_after();
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      store_lse(n, m, l);
+      const uint32_t stage = sbase + GEO::kOffQ + x * kQTile;  // Q_x is no longer read
+#pragma unroll 1
+      for (int k = 0; k < 4; ++k) {
+        uint32_t o[32];
+        if (done) {
+          tmem_ld32_wait(tO + 32 * k, o);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = 0;
+        }
+        float v[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(o[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) stage_chunk(stage, r, 4 * k + c, v + 8 * c, inv);
+      }
+      __syncwarp();
+      store_rows(stage, (warp & 3) * 32, x * BM + (warp & 3) * 32);
+    }
+  } else if (warp < 8) {
+    // a Q tile without rows: nothing to do
+  } else if (warp < kProdWarp) {
+    // ------------------------------------------------------------ converters
+    const int is_v = (warp - kConvWarp0) >> 1;
+    const int t = lane & 3, r0 = (warp & 1) * 32 + (lane >> 2);
+    auto convert = [&](auto conv, uint32_t codes, uint32_t tiles, int n_ld, int n_kv, uint64_t* ld_full, uint64_t* ld_empty,
+                       uint64_t* kv_full, uint64_t* kv_empty, int rec, int stage_bytes) {
+      conv.init(t);
+      for (int j = 0; j < nkv; ++j) {
+        const int ls = j % n_ld, ks = j % n_kv;
+        if (!mbar_wait_warp(&ld_full[ls], (j / n_ld) & 1, abort, a.status, lim)) break;
+        if (j >= n_kv && !mbar_wait_warp(&kv_empty[ks], ((j / n_kv) - 1) & 1, abort, a.status, lim)) break;
+        const uint32_t dst = tiles + ks * kKVTile;
+#pragma unroll 2
+        for (int p = 0; p < 4; ++p) {
+          const int r = r0 + 8 * p, e = it.jb + 4 * j + (r >> 4);
+          const bool live = e < it.je && it.block_at(e) * kBlock + (r & 15) < sq.kv_len;
+          conv.row(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, dst, r, t, live);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&ld_empty[ls]);
+          mbar_arrive(&kv_full[ks]);
+        }
+      }
+    };
+    if (!is_v)
+      convert(Converter<L, KB>{}, sbase + GEO::kOffCK, sbase + GEO::kOffK, LK, NK, bars + GEO::bLdFull, bars + GEO::bLdEmpty,
+              bars + GEO::bKvFull, bars + GEO::bKvEmpty, GEO::kRecK, GEO::kStageK);
+    else
+      convert(Converter<L, VB>{}, sbase + GEO::kOffCV, sbase + GEO::kOffV, LV, NV, bars + GEO::bLdFull + LK,
+              bars + GEO::bLdEmpty + LK, bars + GEO::bKvFull + NK, bars + GEO::bKvEmpty + NK, GEO::kRecV, GEO::kStageV);
+  } else if (warp == kProdWarp || warp == kProdWarpV) {
+    // ------------------------------------------------------------ producers
+    const bool pv = warp != kProdWarp;
+    const int n_ld = pv ? LV : LK;
+    const uint32_t rec = pv ? GEO::kRecV : GEO::kRecK;
+    const uint8_t* pages = pv ? a.v_pages : a.k_pages;
+    uint64_t* full = bars + GEO::bLdFull + (pv ? LK : 0);
+    uint64_t* empty = bars + GEO::bLdEmpty + (pv ? LK : 0);
+    const uint32_t base = sbase + (pv ? GEO::kOffCV : GEO::kOffCK);
+    int64_t where = 0;  // lane i: the pool block of list entry 32 k + i
+    int issued = 0;
+    for (int j = 0; j < nkv; ++j) {
+      const int ls = j % n_ld;
+      if ((j & 7) == 0) {
+        const int e = it.jb + 4 * j + lane;
+        bool ok;
+        if (e < it.je) where = a.p.block(it.seq, it.head, it.block_at(e), ok);
+      }
+      if (j >= n_ld && !mbar_wait_warp(&empty[ls], ((j / n_ld) - 1) & 1, abort, a.status, lim)) break;
+      const int nb = min(4, n_blk - 4 * j);
+      if (lane == 0) mbar_arrive_expect_tx(&full[ls], nb * rec);
+      __syncwarp();
+      const int64_t blk = __shfl_sync(0xffffffffu, where, 4 * (j & 7) + (lane & 3));
+      if (lane < nb) bulk_load(base + (4 * ls + lane) * rec, pages + blk * rec, rec, &full[ls]);
+      issued = j + 1;
+    }
+    // leave no copy into this CTA's shared memory in flight
+    if (lane == 0)
+      for (int j = max(0, issued - n_ld); j < issued; ++j) mbar_drain(&full[j % n_ld], (j / n_ld) & 1, a.status, lim);
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ MMA issuers
+    const int x = warp - kMmaWarp;
+    if (lane == 0 && x < nq) {
+      constexpr uint32_t idS = idesc_bf16(BM, BN, 0);
+      constexpr uint32_t idPV = idesc_bf16(BM, D, 1);
+      const uint32_t tS0 = tmem + kColS + 128 * x, tO = tmem + kColO + 128 * x;
+      const uint32_t qaddr = sbase + GEO::kOffQ + x * kQTile;
+      auto issue_s = [&](int j) {
+        const uint32_t kaddr = sbase + GEO::kOffK + (j % NK) * kKVTile;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          mma_bf16_ss(tS0 + 64 * (j & 1), smem_desc_sw128(qaddr + (kk >> 2) * kQAtom + (kk & 3) * 32, 16, 1024),
+                      smem_desc_sw128(kaddr + (kk >> 2) * kAtom + (kk & 3) * 32, 16, 1024), idS, kk > 0);
+        mma_commit(&bars[GEO::bSFull + 2 * x + (j & 1)]);
+      };
+      auto issue_pv = [&](int j) {
+        const uint32_t vaddr = sbase + GEO::kOffV + (j % NV) * kKVTile;
+        const uint32_t p = tS0 + 64 * (j & 1);
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk)
+          mma_bf16_ts(tO, p + 8 * kk, smem_desc_sw128(vaddr + kk * 2048, kAtom, 1024), idPV,
+                      (j > 0 || kk > 0) ? 1u : 0u);
+      };
+      auto wait_k = [&](int j) { return mbar_wait(&bars[GEO::bKvFull + j % NK], (j / NK) & 1, abort, a.status, lim); };
+      bool ok = nkv > 0 && mbar_wait(&bars[GEO::bQReady + x], 0, abort, a.status, lim) && wait_k(0);
+      if (ok) {
+        tc_fence_after();
+        issue_s(0);
+        if (nkv > 1 && (ok = wait_k(1))) {
+          tc_fence_after();
+          issue_s(1);
+        }
+      }
+      for (int j = 0; j < nkv && ok; ++j) {
+        if (!(ok = mbar_wait(&bars[GEO::bKvFull + NK + j % NV], (j / NV) & 1, abort, a.status, lim))) break;
+        if (j + 2 < nkv && !(ok = wait_k(j + 2))) break;
+        if (!(ok = mbar_wait(&bars[GEO::bPFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim))) break;
+        tc_fence_after();
+        issue_pv(j);
+        if (j + 2 < nkv) {
+          issue_s(j + 2);
+        } else if (j + 2 == nkv) {
+          mma_commit(&bars[GEO::bOReady + x]);
+        }
+      }
+      if (ok) mma_commit(&bars[GEO::bOFinal + x]);
+      // all MMAs issued by this thread have completed before TMEM is released
+      mma_commit(&bars[GEO::bMmaDone + x]);
+      mbar_drain(&bars[GEO::bMmaDone + x], 0, a.status, lim);
+    }
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+  if (it.parts > 1) {
+    // the part that ends last joins them, in part order
+    if (tid == 0) {
+      const unsigned old = atomicAdd(a.ctr + it.unit, 1u);
+      *last = old == static_cast<unsigned>(it.parts - 1);
+      if (*last) a.ctr[it.unit] = 0u;  // ready for the next launch
+    }
+    __syncthreads();
+    if (*last && warp < 4 * nq) {
+      __threadfence();
+      const int x = warp >> 2, r = tid - x * BM, n = tid;
+      const int64_t pstride = static_cast<int64_t>(2) * 33 * BM;
+      const float4* src = reinterpret_cast<const float4*>(a.ws) + (static_cast<int64_t>(it.slot) * 2 + x) * 33 * BM + r;
+      float mx = -1.0e30f, lsum = 0.0f;
+      for (int p = 0; p < it.parts; ++p) mx = fmaxf(mx, __ldcg(src + p * pstride + 32 * BM).x);
+      for (int p = 0; p < it.parts; ++p) {
+        const float4 ml = __ldcg(src + p * pstride + 32 * BM);
+        lsum = fmaf(ml.y, ex2f(ml.x - mx), lsum);
+      }
+      const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+      store_lse(n, mx, lsum);
+      const uint32_t stage = sbase + GEO::kOffQ + x * kQTile;
+#pragma unroll 1
+      for (int ch = 0; ch < 16; ++ch) {
+        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 2
+        for (int p = 0; p < it.parts; ++p) {
+          const float f = ex2f(__ldcg(src + p * pstride + 32 * BM).x - mx);
+          const float4 v0 = __ldcg(src + p * pstride + (2 * ch) * BM), v1 = __ldcg(src + p * pstride + (2 * ch + 1) * BM);
+          acc[0] = fmaf(v0.x, f, acc[0]);
+          acc[1] = fmaf(v0.y, f, acc[1]);
+          acc[2] = fmaf(v0.z, f, acc[2]);
+          acc[3] = fmaf(v0.w, f, acc[3]);
+          acc[4] = fmaf(v1.x, f, acc[4]);
+          acc[5] = fmaf(v1.y, f, acc[5]);
+          acc[6] = fmaf(v1.z, f, acc[6]);
+          acc[7] = fmaf(v1.w, f, acc[7]);
+        }
+        stage_chunk(stage, r, ch, acc, inv);
+      }
+      __syncwarp();
+      store_rows(stage, (warp & 3) * 32, x * BM + (warp & 3) * 32);
+    }
+  }
+}
+
+}  // namespace tiles
+
+int launch_tiles(const AttnArgs& a, int layout, int k_bits, int v_bits, int n_items, cudaStream_t st) {
+  return with_layout(layout, [&](auto lt) {
+    using L = decltype(lt);
+    return with_bits(k_bits, v_bits, [&](auto bt) -> int {
+      using B = decltype(bt);
+      auto kernel = tiles::tiles_kernel<L, B::k, B::v>;
+      constexpr int smem = tiles::Geo<L, B::k, B::v>::kSmemBytes;
+      static bool configured[64];
+      int dev = 0;
+      cudaGetDevice(&dev);
+      if (dev < 0 || dev >= 64 || !configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        KVQ_REQUIRE(e == cudaSuccess, KVQ_ERR_CUDA, "cudaFuncSetAttribute(paged tiles): %s", cudaGetErrorString(e));
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+      }
+      cudaError_t e = launch_pdl(kernel, static_cast<unsigned>(n_items), tiles::kThreads, smem, st, a);
+      KVQ_REQUIRE(e == cudaSuccess, KVQ_ERR_CUDA, "kvq_paged_attention: launch failed: %s", cudaGetErrorString(e));
+      return KVQ_OK;
+    });
+  });
+}
+
+}  // namespace paged
+}  // namespace kvq

@@ -67,7 +67,8 @@ class PagedBatchArgs(ctypes.Structure):
 class PagedPlanInfo(ctypes.Structure):
     """kvq_paged_plan_info"""
     _fields_ = [("n_row_items", _i32), ("n_row_ctas", _i32), ("n_tile_items", _i32), ("row_tile", _i32),
-                ("n_units", _i32), ("n_slots", _i32), ("words", _i64), ("workspace_bytes", _i64)]
+                ("n_units", _i32), ("reserved", _i32), ("words", _i64), ("workspace_bytes", _i64),
+                ("tile_workspace_offset", _i64)]
 
 
 ABI_VERSION = 3

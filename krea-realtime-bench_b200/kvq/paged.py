@@ -23,11 +23,25 @@ import torch
 import quant_kv_kernels as _kern
 
 from . import _lib
-from .ops import _ptr, _require_cuda
+from .ops import _require_cuda
 
 BLOCK = 16  # tokens of one storage block
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIM = 128
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream of a device, as an integer
+
+
+def _call(device: torch.device, fn, what: str, *args) -> None:
+    """One C call on `device`, with its current stream as the last argument."""
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device.index))
+    if rc:
+        _lib.check(rc, what)
 
 
 def _cuda_device(device) -> torch.device:
@@ -125,10 +139,12 @@ class PagedBatch:
         base = self._dev.data.data_ptr()
         self._args = _lib.PagedBatchArgs(base + seqs.size * 4, rows.shape[1], base, self.n_new, self.n_tokens,
                                          self.n_new_blocks, self.n_blocks, self.n_seqs, 0)
+        self._c = ctypes.byref(self._args)
 
-    def _on_stream(self, stream):
-        self._dev.use(stream)
-        return ctypes.byref(self._args)
+    def _ref(self):
+        """The C arguments, safe to read on the current stream."""
+        self._dev.use()
+        return self._c
 
 
 class _Uploaded:
@@ -141,16 +157,20 @@ class _Uploaded:
         if flat.size:
             self.data[:flat.size].copy_(torch.from_numpy(flat).pin_memory(), non_blocking=True)
         self._event = torch.cuda.Event()
-        self._stream = torch.cuda.current_stream(device)
-        self._event.record(self._stream)
+        self._stream = _raw_stream(device.index)
+        self._event.record(torch.cuda.current_stream(device))
 
-    def use(self, stream) -> None:
-        """Makes the data safe to read on `stream`: another stream than the one that
-        uploaded it waits for the upload, and the allocator is told of it. A capture
-        begins with a synchronization, so an upload before it has completed."""
-        if stream != self._stream and not torch.cuda.is_current_stream_capturing():
+    def use(self) -> int:
+        """Makes the data safe to read on the current stream, which it returns: another
+        stream than the one that uploaded it waits for the upload, and the allocator is
+        told of it. A capture begins with a synchronization, so an upload before it has
+        completed."""
+        raw = _raw_stream(self.data.device.index)
+        if raw != self._stream and not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(self.data.device)
             stream.wait_event(self._event)
             self.data.record_stream(stream)
+        return raw
 
 
 class _Plan:
@@ -173,16 +193,17 @@ class _Plan:
         self.items = _Uploaded(words, batch.device)
         self._work = {}
 
-    def args(self, stream):
-        self.items.use(stream)
-        work = self._work.get(stream.cuda_stream)
-        if work is None:
+    def args(self):
+        raw = self.items.use()
+        got = self._work.get(raw)
+        if got is None:
             n, c = self.info.workspace_bytes, self.info.n_units
             # counters count up to a unit's parts and are set back by the last one
-            work = (torch.empty(n, dtype=torch.uint8, device=self.device) if n else None,
-                    torch.zeros(c, dtype=torch.int32, device=self.device) if c else None)
-            self._work[stream.cuda_stream] = work
-        return ctypes.byref(self.info), _ptr(self.items.data), _ptr(work[0]), _ptr(work[1])
+            ws = torch.empty(max(n, 1), dtype=torch.uint8, device=self.device)
+            counters = torch.zeros(max(c, 1), dtype=torch.int32, device=self.device)
+            got = self._work[raw] = (ctypes.byref(self.info), self.items.data.data_ptr(), ws.data_ptr(),
+                                     counters.data_ptr(), ws, counters)
+        return got[:4]
 
 
 class PagedKVCache:
@@ -215,6 +236,9 @@ class PagedKVCache:
         self.k_pages, self.v_pages = (
             torch.zeros((n_pages, n_heads, page_size // BLOCK, BLOCK * self._row_bytes(b)), dtype=torch.uint8,
                         device=dev) for b in (k_bits, v_bits))
+        self._c = _lib.PagedCacheArgs(None, None, self.n_pages, self.page_size, self.n_heads, self.head_dim, self.k_bits,
+                                      self.v_bits, len(self.bands), self._map.ctypes.data)
+        self._c_ref = ctypes.byref(self._c)
 
     def _row_bytes(self, bits: int) -> int:
         return self._code_bytes(bits) + 2 * len(self.bands)
@@ -237,12 +261,10 @@ class PagedKVCache:
     def storage_bytes(self) -> int:
         return self.k_pages.numel() + self.v_pages.numel()
 
-    def _args(self):
-        for t in (self.k_pages, self.v_pages):
-            _require_cuda(t)
-        return ctypes.byref(_lib.PagedCacheArgs(
-            self.k_pages.data_ptr(), self.v_pages.data_ptr(), self.n_pages, self.page_size, self.n_heads,
-            self.head_dim, self.k_bits, self.v_bits, len(self.bands), self._map.ctypes.data))
+    def _ref(self):
+        c = self._c
+        c.k_pages, c.v_pages = self.k_pages.data_ptr(), self.v_pages.data_ptr()
+        return self._c_ref
 
     def _check(self, batch: PagedBatch) -> None:
         if not isinstance(batch, PagedBatch):
@@ -261,12 +283,10 @@ class PagedKVCache:
         self._check(batch)
         if batch._append_error:
             raise ValueError(batch._append_error)
-        k, v = (_rows(t, (batch.n_new, self.n_heads, self.head_dim), self.device, n) for t, n in ((k, "k"), (v, "v")))
-        with torch.cuda.device(self.device):
-            stream = torch.cuda.current_stream()
-            rc = _lib.load().kvq_paged_append(_ptr(k), _row_stride(k), _ptr(v), _row_stride(v), self._args(),
-                                              batch._on_stream(stream), stream.cuda_stream)
-        _lib.check(rc, "kvq_paged_append")
+        shape = (batch.n_new, self.n_heads, self.head_dim)
+        k, v = _rows(k, shape, self.device, "k"), _rows(v, shape, self.device, "v")
+        _call(self.device, _lib.load().kvq_paged_append, "kvq_paged_append", k.data_ptr(), _row_stride(k), v.data_ptr(),
+              _row_stride(v), self._ref(), batch._ref())
 
     def read(self, batch: PagedBatch, new_only: bool = False):
         """(k, v) bf16 [n, n_heads, 128]: the values held for the sequences' tokens, or
@@ -275,13 +295,11 @@ class PagedKVCache:
         if new_only and batch._append_error and (batch.q_lens > batch.kv_lens).any():
             raise ValueError("new_only needs q_lens <= kv_lens: every new token has a position")
         n = batch.n_new if new_only else batch.n_tokens
-        k, v = (torch.empty((n, self.n_heads, self.head_dim), dtype=torch.bfloat16, device=self.device)
-                for _ in range(2))
-        with torch.cuda.device(self.device):
-            stream = torch.cuda.current_stream()
-            rc = _lib.load().kvq_paged_read(self._args(), batch._on_stream(stream), 1 if new_only else 0, _ptr(k),
-                                            _row_stride(k), _ptr(v), _row_stride(v), stream.cuda_stream)
-        _lib.check(rc, "kvq_paged_read")
+        shape, row = (n, self.n_heads, self.head_dim), self.n_heads * self.head_dim
+        k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        _call(self.device, _lib.load().kvq_paged_read, "kvq_paged_read", self._ref(), batch._ref(), 1 if new_only else 0,
+              k.data_ptr(), row, v.data_ptr(), row)
         return k, v
 
     def __repr__(self):
@@ -291,16 +309,21 @@ class PagedKVCache:
 
 
 def _rows(t, shape, device, name: str) -> torch.Tensor:
-    if _require_cuda(t) != device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        if _require_cuda(t) != device:
+            raise ValueError(f"{name} is on {t.device}, the cache on {device}")
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]) or t.data_ptr() % 16
-                      or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1] * t.shape[2]))):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        s0, s1, s2 = t.stride()
+        row = shape[1] * shape[2]
+        if s2 == 1 and (s1 == shape[2] or shape[1] == 1) and s0 % 8 == 0 and (s0 >= row or shape[0] == 1):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -334,18 +357,15 @@ def attention(q: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, causal: b
     scale = 0.0 if softmax_scale is None else float(softmax_scale)
     if softmax_scale is not None and not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"softmax_scale must be a positive number, got {softmax_scale}")
-    shape = (batch.n_new, heads, cache.head_dim)
+    shape = torch.Size((batch.n_new, heads, cache.head_dim))
     q = _rows(q, shape, cache.device, "q")
     if out is None:
         out = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
     elif _rows(out, shape, cache.device, "out") is not out:
         raise ValueError("out must have contiguous [heads, channels] blocks, 16-byte aligned rows")
     lse = torch.empty(shape[:2], dtype=torch.float32, device=cache.device) if return_lse else None
-    with torch.cuda.device(cache.device):
-        stream = torch.cuda.current_stream()
-        plan = batch._plan(cache.n_heads, heads, bool(causal), window, sink)
-        rc = _lib.load().kvq_paged_attention(_ptr(q), _row_stride(q), cache._args(), batch._on_stream(stream), _ptr(out),
-                                             _row_stride(out), _ptr(lse), heads, 1 if causal else 0, window, sink,
-                                             scale, *plan.args(stream), stream.cuda_stream)
-    _lib.check(rc, "kvq_paged_attention")
+    plan = batch._plan(cache.n_heads, heads, bool(causal), window, sink)
+    _call(cache.device, _lib.load().kvq_paged_attention, "kvq_paged_attention", q.data_ptr(), _row_stride(q), cache._ref(),
+          batch._ref(), out.data_ptr(), _row_stride(out), lse.data_ptr() if return_lse else None, heads,
+          1 if causal else 0, window, sink, scale, *plan.args())
     return (out, lse) if return_lse else out
