@@ -385,12 +385,12 @@ typedef struct {
 
 /*
  * Writes the plan to out (HOST int32[capacity], to be copied to the device; NULL:
- * only *info is filled). kv_lens, q_lens: HOST int32[n_seqs]. n_sms: SMs of the
- * device that will run it. KVQ_ERR_ARG where capacity < info->words.
+ * only *info is filled). Of the cache only its format counts, not its pages. kv_lens,
+ * q_lens: HOST int32[n_seqs]. n_sms: SMs of the device that will run it. KVQ_ERR_ARG where capacity < info->words.
  */
-KVQ_API int kvq_paged_plan(const int32_t* kv_lens, const int32_t* q_lens, int n_seqs, int n_heads, int n_q_heads,
-                           int causal, int64_t window, int64_t sink, int n_sms, int32_t* out, int64_t capacity,
-                           kvq_paged_plan_info* info);
+KVQ_API int kvq_paged_plan(const kvq_paged_cache* cache, const int32_t* kv_lens, const int32_t* q_lens, int n_seqs,
+                           int n_q_heads, int causal, int64_t window, int64_t sink, int n_sms, int32_t* out,
+                           int64_t capacity, kvq_paged_plan_info* info);
 
 /*
  * Attention of the new tokens' queries over their sequences' cached tokens:

@@ -10,8 +10,8 @@
 namespace kvq {
 namespace paged {
 
-int check_cache(const kvq_paged_cache* c, const kvq_paged_batch* b, int* layout) {
-  KVQ_REQUIRE(c != nullptr && b != nullptr, KVQ_ERR_ARG, "NULL cache or batch");
+int check_format(const kvq_paged_cache* c, int* layout) {
+  KVQ_REQUIRE(c != nullptr, KVQ_ERR_ARG, "NULL cache");
   KVQ_REQUIRE(c->head_dim == D, KVQ_ERR_UNSUPPORTED, "the paged cache supports head_dim 128, got %d", c->head_dim);
   KVQ_REQUIRE((c->k_bits == 4 && c->v_bits == 4) || (c->k_bits == 8 && (c->v_bits == 4 || c->v_bits == 8)),
               KVQ_ERR_UNSUPPORTED, "the paged cache holds K/V in 4/4, 8/4 or 8/8 bits, got %d/%d", c->k_bits,
@@ -26,6 +26,13 @@ int check_cache(const kvq_paged_cache* c, const kvq_paged_batch* b, int* layout)
   KVQ_REQUIRE(id != kLayoutGeneric, KVQ_ERR_UNSUPPORTED,
               "the paged cache supports the bands, bands2, bands4, blind32 and blind64 group maps");
   *layout = id;
+  return KVQ_OK;
+}
+
+int check_cache(const kvq_paged_cache* c, const kvq_paged_batch* b, int* layout) {
+  const int rc = check_format(c, layout);
+  if (rc) return rc;
+  KVQ_REQUIRE(b != nullptr, KVQ_ERR_ARG, "NULL batch");
   KVQ_REQUIRE(c->k_pages && c->v_pages, KVQ_ERR_ARG, "NULL page pointer");
   KVQ_REQUIRE((reinterpret_cast<uintptr_t>(c->k_pages) & 15) == 0 && (reinterpret_cast<uintptr_t>(c->v_pages) & 15) == 0,
               KVQ_ERR_ALIGN, "pages must be 16-byte aligned");

@@ -65,18 +65,20 @@ __device__ __forceinline__ int find_seq(const Pages& p, int i) {
 // One piece of attention work: rows [row0, row0 + n_rows) of a sequence and KV head
 // over entries [jb, je) of the list of storage blocks the rows see: blocks [0, n_sink),
 // then first, first + 1, ... ; part `part` of `parts`, its partial result in workspace
-// slot `slot` + part, its unit counted in counter `unit`. (kvq_paged_plan)
+// slot `slot` + part, its unit counted in counter `unit`; start = position of the
+// sequence's first query, q_first = its index. (kvq_paged_plan)
 struct alignas(16) Item {
   int32_t seq, head, row0, n_rows, n_sink, first, jb, je, part, parts, unit, slot;
+  int32_t kv_len, start, q_first, reserved;
   __host__ __device__ __forceinline__ int block_at(int j) const { return j < n_sink ? j : first + (j - n_sink); }
 };
-static_assert(sizeof(Item) == 48, "the plan's layout");
+static_assert(sizeof(Item) == 64, "the plan's layout");
+constexpr int kItemWords = 16;
 
 // Workspace of one part: O [rows][128] unnormalised, then m, l per row (fp32).
 __host__ __device__ constexpr int slot_floats(int rows) { return rows * (D + 2); }
 // Most parts of a unit: joining them is serial work of one block.
 constexpr int kMaxParts = 128;
-constexpr int kRowCtasPerSm = 3;  // resident blocks of the kernel for few rows
 
 // What both attention kernels take.
 struct AttnArgs {
@@ -119,9 +121,12 @@ constexpr int kTileRows = 256;
 constexpr int64_t kTileSlotBytes = 2 * 33 * 128 * 16;
 
 int launch_tiles(const AttnArgs& a, int layout, int k_bits, int v_bits, int n_items, cudaStream_t st);
+// Resident blocks per SM of the kernel for few rows.
+int rows_ctas_per_sm(int layout, int k_bits, int v_bits, int row_tile);
 int launch_rows(const AttnArgs& a, int layout, int k_bits, int v_bits, int row_tile, int n_ctas, cudaStream_t st);
 
 // Checks that hold for every entry point; fills the group layout.
+int check_format(const kvq_paged_cache* c, int* layout);
 int check_cache(const kvq_paged_cache* c, const kvq_paged_batch* b, int* layout);
 Pages make_pages(const kvq_paged_cache* c, const kvq_paged_batch* b);
 

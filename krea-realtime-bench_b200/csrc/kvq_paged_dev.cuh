@@ -28,8 +28,23 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Nibbles at bits 0-3 and 16-19 (code = q + 8) -> bf16x2 (q, q): 128 + code - 136.
-__device__ __forceinline__ uint32_t int4_pair(uint32_t x) { return hsub2((x & 0x000F000Fu) | 0x43004300u, 0x43084308u); }
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  const __nv_bfloat162 r = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b),
+                                   *reinterpret_cast<__nv_bfloat162*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// int4 codes (code = q + 8) at bits 0-3 and 16-19, or 4-7 and 20-23, of a word -> bf16x2
+// (q / 4, q / 4), exact, one logic operation and one FMA each and no shift:
+//   low   ored into the mantissa of 128: 128 + code, times 1/4, minus 34;
+//   high  bits 4-7 of a bf16 are its lowest exponent bit and the top of its mantissa, and
+//         a bf16 with that exponent or none is linear in its bits: code * 2^-129, times
+//         2^127, minus 2.
+// With four times the scale the product is q * s, rounded once.
+__device__ __forceinline__ uint32_t int4_low(uint32_t x) {
+  return hfma2((x & 0x000F000Fu) | 0x43004300u, 0x3E803E80u, 0xC208C208u);
+}
+__device__ __forceinline__ uint32_t int4_high(uint32_t x) { return hfma2(x & 0x00F000F0u, 0x7F007F00u, 0xC000C000u); }
+constexpr uint32_t kFour = 0x40804080u;  // bf16x2 (4, 4)
 // Bytes at bits 0-7 and 16-23 (code = q + 128) -> bf16x2 (q, q). The low seven bits give
 // 128 + code % 128, from which 256 is taken, or 128 where the top bit is set.
 __device__ __forceinline__ uint32_t int8_pair(uint32_t x) {

@@ -1,6 +1,7 @@
 // Host-side plan of one attention step over a paged batch (kvq_paged_plan).
 #include <algorithm>
 #include <cstring>
+#include <functional>
 #include <new>
 #include <vector>
 
@@ -11,11 +12,12 @@ namespace paged {
 
 struct Unit {
   int32_t seq, row0, n_rows, n_sink, first, n;  // n: entries of the block list
+  int32_t kv_len, start, q_first;
 };
 
 // The storage blocks that rows [row0, row0 + n_rows) of a sequence see between them.
-static Unit make_unit(int seq, int kv_len, int q_len, int group, int row0, int n_rows, int causal, int64_t window,
-                      int64_t sink) {
+static Unit make_unit(int seq, int kv_len, int q_len, int64_t q_first, int group, int row0, int n_rows, int causal,
+                      int64_t window, int64_t sink) {
   const int64_t start = static_cast<int64_t>(kv_len) - q_len;
   const int64_t p0 = start + row0 / group, p1 = start + (row0 + n_rows - 1) / group;
   const int64_t hi = std::max<int64_t>(0, causal ? std::min<int64_t>(p1 + 1, kv_len) : kv_len);
@@ -24,8 +26,13 @@ static Unit make_unit(int seq, int kv_len, int q_len, int group, int row0, int n
   const int64_t b1 = (hi + kBlock - 1) / kBlock;
   const int64_t b0 = std::min(lo / kBlock, b1);
   const int64_t ns = std::min((kept + kBlock - 1) / kBlock, b0);
-  return Unit{seq, row0, n_rows, static_cast<int32_t>(ns), static_cast<int32_t>(b0),
-              static_cast<int32_t>(ns + b1 - b0)};
+  return Unit{seq, row0, n_rows, static_cast<int32_t>(ns), static_cast<int32_t>(b0), static_cast<int32_t>(ns + b1 - b0),
+              kv_len, static_cast<int32_t>(start), static_cast<int32_t>(q_first)};
+}
+
+static Item make_item(const Unit& u, int head, int64_t jb, int64_t je, int part, int parts, int unit, int slot) {
+  return Item{u.seq, head, u.row0, u.n_rows, u.n_sink, u.first, static_cast<int32_t>(jb), static_cast<int32_t>(je), part,
+              parts, parts > 1 ? unit : -1, parts > 1 ? slot : -1, u.kv_len, u.start, u.q_first, 0};
 }
 
 struct Plan {
@@ -41,16 +48,17 @@ struct Plan {
 // no unit gets more than kMaxParts parts.
 constexpr int kMinBlocks = 8;
 
-static void cut_rows(const std::vector<Unit>& units, int n_heads, int n_sms, Plan* p) {
+static void cut_rows(const std::vector<Unit>& units, int n_heads, int64_t n_resident, Plan* p) {
   int64_t total = 0, longest = 0;
   for (const Unit& u : units) {
     total += static_cast<int64_t>(std::max(u.n, 1)) * n_heads;
     longest = std::max<int64_t>(longest, u.n);
   }
   if (total == 0) return;
-  const int64_t most = static_cast<int64_t>(n_sms) * kRowCtasPerSm;
-  int64_t piece = std::max<int64_t>({(total + most - 1) / most, kMinBlocks, (longest + kMaxParts - 2) / (kMaxParts - 1)});
+  const int64_t piece = std::max<int64_t>(
+      {(total + n_resident - 1) / n_resident, kMinBlocks, (longest + kMaxParts - 2) / (kMaxParts - 1)});
   const int64_t n_ctas = (total + piece - 1) / piece;
+  p->rows.reserve(units.size() * n_heads + n_ctas);
   p->cta_first.push_back(0);
   int64_t at = 0;  // position on the line
   for (const Unit& u : units) {
@@ -62,9 +70,8 @@ static void cut_rows(const std::vector<Unit>& units, int n_heads, int n_sms, Pla
         while (static_cast<int64_t>(p->cta_first.size()) <= c)
           p->cta_first.push_back(static_cast<int32_t>(p->rows.size()));
         const int64_t b = std::max(c * piece, at) - at, e = std::min((c + 1) * piece, at + len) - at;
-        p->rows.push_back(Item{u.seq, h, u.row0, u.n_rows, u.n_sink, u.first, static_cast<int32_t>(std::min<int64_t>(b, u.n)),
-                               static_cast<int32_t>(std::min<int64_t>(e, u.n)), static_cast<int32_t>(c - c0), parts,
-                               parts > 1 ? p->units : -1, parts > 1 ? p->slots : -1});
+        p->rows.push_back(make_item(u, h, std::min<int64_t>(b, u.n), std::min<int64_t>(e, u.n), static_cast<int>(c - c0),
+                                    parts, p->units, p->slots));
       }
       if (parts > 1) {
         ++p->units;
@@ -76,26 +83,82 @@ static void cut_rows(const std::vector<Unit>& units, int n_heads, int n_sms, Pla
     p->cta_first.push_back(static_cast<int32_t>(p->rows.size()));
 }
 
-// Many rows: one block of the device per item and SM, started in the order of the list.
-// Long units first, whole while much work is left; later ones are cut so that no piece is
-// longer than an equal share of the work that is left, and the last ones to run
-// end together. No piece is shorter than kMinTiles tiles of four storage blocks, no
-// unit has more than kMaxTileParts parts (their join is serial work of one block).
-constexpr int kMinTiles = 8, kMaxTileParts = 32;
+// Many rows: one CTA per item and SM, started in the order of the list, long units first.
+// Which units are cut into parts, and into how many, is chosen by simulating that list
+// on the SMs for a few ways to cut it: none; all units, the units behind the last full
+// wave, or those and one wave more, into pieces of about 1/1 to 1/4 of an SM's share of
+// them. Costs in tiles of 64 tokens: kItemCost for an item (fill, epilogue), kPartCost
+// more for a part's partial sums and kJoinCost for each part that the last one joins.
+// Lists of more than kSimWaves waves are left whole: the last wave is a small share.
+constexpr double kItemCost = 4.0, kPartCost = 1.5, kJoinCost = 0.5;
+constexpr int kMinTiles = 4, kMaxTileParts = 32, kSimWaves = 8;
 
-static void cut_tiles(std::vector<Unit>& units, int n_heads, int n_sms, Plan* p) {
-  std::stable_sort(units.begin(), units.end(), [](const Unit& a, const Unit& b) { return a.n > b.n; });
-  int64_t left = 0;
-  for (const Unit& u : units) left += static_cast<int64_t>((u.n + 3) / 4) * n_heads;
+struct Cut {
+  size_t from;   // units (heads multiplied) from this one on are cut
+  double piece;  // into pieces of about this many tiles
+  int parts(size_t i, int64_t t) const {
+    if (i < from || piece <= 0) return 1;
+    const int64_t n = static_cast<int64_t>(static_cast<double>(t) / piece + 0.5);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({n, t / kMinTiles, kMaxTileParts})));
+  }
+};
+
+static double simulate(const std::vector<Unit>& units, int n_heads, int n_sms, const Cut& cut) {
+  std::vector<double> busy(static_cast<size_t>(n_sms), 0.0);  // heap of the SMs' finishing times
+  const std::greater<double> later;
+  double end = 0.0;
+  size_t i = 0;
   for (const Unit& u : units) {
     const int64_t t = (u.n + 3) / 4;
-    for (int h = 0; h < n_heads; ++h, left -= t) {
-      const int64_t piece = std::max<int64_t>(kMinTiles, left / n_sms);
-      const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((t + piece - 1) / piece, kMaxTileParts)));
-      for (int i = 0; i < parts; ++i)
-        p->tiles.push_back(Item{u.seq, h, u.row0, u.n_rows, u.n_sink, u.first, static_cast<int32_t>(4 * (t * i / parts)),
-                                static_cast<int32_t>(std::min<int64_t>(u.n, 4 * (t * (i + 1) / parts))), i, parts,
-                                parts > 1 ? p->units : -1, parts > 1 ? p->tile_slots : -1});
+    const double pace = u.n_rows > 128 ? 1.0 : 0.85;
+    for (int h = 0; h < n_heads; ++h, ++i) {
+      const int parts = cut.parts(i, t);
+      const double cost = pace * static_cast<double>(t) / parts + kItemCost + (parts > 1 ? kPartCost : 0.0);
+      for (int k = 0; k < parts; ++k) {
+        std::pop_heap(busy.begin(), busy.end(), later);
+        busy.back() += cost + (parts > 1 && k + 1 == parts ? kJoinCost * parts : 0.0);
+        end = std::max(end, busy.back());
+        std::push_heap(busy.begin(), busy.end(), later);
+      }
+    }
+  }
+  return end;
+}
+
+static void cut_tiles(std::vector<Unit>& units, int n_heads, int n_sms, Plan* p) {
+  if (units.empty()) return;
+  std::stable_sort(units.begin(), units.end(), [](const Unit& a, const Unit& b) { return a.n > b.n; });
+  const size_t n = units.size() * n_heads, wave = static_cast<size_t>(n_sms);
+  Cut best{n, 0.0};
+  if (n <= kSimWaves * wave) {
+    double least = simulate(units, n_heads, n_sms, best);
+    const size_t rest = n % wave;
+    const size_t tail[3] = {n, rest, rest + wave};
+    for (int m = 0; m < 3; ++m) {
+      if (tail[m] == 0 || tail[m] > n || (m > 0 && tail[m] == n)) continue;
+      double work = 0.0;
+      size_t i = 0;
+      for (const Unit& u : units)
+        for (int h = 0; h < n_heads; ++h, ++i)
+          if (i >= n - tail[m]) work += (u.n + 3) / 4;
+      for (int k = 1; k <= 4; ++k) {
+        const Cut c{n - tail[m], work / (static_cast<double>(wave) * k)};
+        const double end = simulate(units, n_heads, n_sms, c);
+        if (end < least * 0.98) {  // a cut has to be worth something
+          least = end;
+          best = c;
+        }
+      }
+    }
+  }
+  size_t i = 0;
+  for (const Unit& u : units) {
+    const int64_t t = (u.n + 3) / 4;
+    for (int h = 0; h < n_heads; ++h, ++i) {
+      const int parts = best.parts(i, t);
+      for (int k = 0; k < parts; ++k)
+        p->tiles.push_back(make_item(u, h, 4 * (t * k / parts), std::min<int64_t>(u.n, 4 * (t * (k + 1) / parts)), k, parts,
+                                     p->units, p->tile_slots));
       if (parts > 1) {
         ++p->units;
         p->tile_slots += parts;
@@ -107,23 +170,25 @@ static void cut_tiles(std::vector<Unit>& units, int n_heads, int n_sms, Plan* p)
 // Up to kFewRows rows of a sequence and KV head go to the kernel for few rows.
 constexpr int kFewRows = 16;
 
-static int make_plan(const int32_t* kv_lens, const int32_t* q_lens, int n_seqs, int n_heads, int group, int causal,
-                     int64_t window, int64_t sink, int n_sms, Plan* p) {
+static int make_plan(const kvq_paged_cache* c, int layout, const int32_t* kv_lens, const int32_t* q_lens, int n_seqs,
+                     int group, int causal, int64_t window, int64_t sink, int n_sms, Plan* p) {
   std::vector<Unit> few, many;
+  int64_t q_first = 0;
   for (int s = 0; s < n_seqs; ++s) {
     const int64_t rows = static_cast<int64_t>(q_lens[s]) * group;
     const int tile = rows <= kFewRows ? kFewRows : kTileRows;
     for (int64_t r = 0; r < rows; r += tile) {
       const int n = static_cast<int>(std::min<int64_t>(tile, rows - r));
       (rows <= kFewRows ? few : many)
-          .push_back(make_unit(s, kv_lens[s], q_lens[s], group, static_cast<int>(r), n, causal, window, sink));
+          .push_back(make_unit(s, kv_lens[s], q_lens[s], q_first, group, static_cast<int>(r), n, causal, window, sink));
       if (rows <= kFewRows && rows > 8) p->row_tile = 16;
     }
+    q_first += q_lens[s];
   }
-  KVQ_REQUIRE(static_cast<int64_t>(few.size() + many.size()) * n_heads < (1 << 24), KVQ_ERR_ARG,
-              "too many rows for one launch");
-  cut_rows(few, n_heads, n_sms, p);
-  cut_tiles(many, n_heads, n_sms, p);
+  KVQ_REQUIRE(static_cast<int64_t>(few.size() + many.size()) * c->n_heads < (1 << 24) && q_first < ((int64_t)1 << 31),
+              KVQ_ERR_ARG, "too many rows for one launch");
+  cut_rows(few, c->n_heads, static_cast<int64_t>(n_sms) * rows_ctas_per_sm(layout, c->k_bits, c->v_bits, p->row_tile), p);
+  cut_tiles(many, c->n_heads, n_sms, p);
   return KVQ_OK;
 }
 
@@ -132,13 +197,17 @@ static int make_plan(const int32_t* kv_lens, const int32_t* q_lens, int n_seqs, 
 
 using namespace kvq;
 
-extern "C" int kvq_paged_plan(const int32_t* kv_lens, const int32_t* q_lens, int n_seqs, int n_heads, int n_q_heads,
-                              int causal, int64_t window, int64_t sink, int n_sms, int32_t* out, int64_t capacity,
-                              kvq_paged_plan_info* info) {
+extern "C" int kvq_paged_plan(const kvq_paged_cache* cache, const int32_t* kv_lens, const int32_t* q_lens, int n_seqs,
+                              int n_q_heads, int causal, int64_t window, int64_t sink, int n_sms, int32_t* out,
+                              int64_t capacity, kvq_paged_plan_info* info) {
   clear_error();
+  int layout = 0;
+  int rc = paged::check_format(cache, &layout);
+  if (rc) return rc;
+  const int n_heads = cache->n_heads;
   KVQ_REQUIRE(info != nullptr, KVQ_ERR_ARG, "NULL info");
   KVQ_REQUIRE(n_seqs >= 0 && n_sms >= 1 && (n_seqs == 0 || (kv_lens && q_lens)), KVQ_ERR_ARG, "bad lengths");
-  KVQ_REQUIRE(n_heads >= 1 && n_heads <= 65535 && n_q_heads >= n_heads && n_q_heads <= 65535 && n_q_heads % n_heads == 0,
+  KVQ_REQUIRE(n_q_heads >= n_heads && n_q_heads <= 65535 && n_q_heads % n_heads == 0,
               KVQ_ERR_ARG, "%d query heads are not a multiple of %d KV heads", n_q_heads, n_heads);
   KVQ_REQUIRE(window >= 0 && sink >= 0, KVQ_ERR_ARG, "window and sink must be >= 0");
   const int group = n_q_heads / n_heads;
@@ -148,7 +217,7 @@ extern "C" int kvq_paged_plan(const int32_t* kv_lens, const int32_t* q_lens, int
   }
   try {
     paged::Plan p;
-    const int rc = paged::make_plan(kv_lens, q_lens, n_seqs, n_heads, group, causal ? 1 : 0, window, sink, n_sms, &p);
+    rc = paged::make_plan(cache, layout, kv_lens, q_lens, n_seqs, group, causal ? 1 : 0, window, sink, n_sms, &p);
     if (rc) return rc;
     *info = kvq_paged_plan_info{};
     info->n_row_items = static_cast<int32_t>(p.rows.size());
@@ -156,7 +225,7 @@ extern "C" int kvq_paged_plan(const int32_t* kv_lens, const int32_t* q_lens, int
     info->n_tile_items = static_cast<int32_t>(p.tiles.size());
     info->row_tile = p.row_tile;
     info->n_units = p.units;
-    info->words = static_cast<int64_t>(p.rows.size() + p.tiles.size()) * 12 + static_cast<int64_t>(p.cta_first.size());
+    info->words = static_cast<int64_t>(p.rows.size() + p.tiles.size()) * paged::kItemWords + static_cast<int64_t>(p.cta_first.size());
     info->tile_workspace_offset = (static_cast<int64_t>(p.slots) * paged::slot_floats(p.row_tile) * 4 + 255) / 256 * 256;
     info->workspace_bytes = info->tile_workspace_offset + p.tile_slots * paged::kTileSlotBytes;
     if (!out) return KVQ_OK;
@@ -165,8 +234,8 @@ extern "C" int kvq_paged_plan(const int32_t* kv_lens, const int32_t* q_lens, int
       if (words) std::memcpy(out, src, words * 4);
       out += words;
     };
-    put(p.rows.data(), p.rows.size() * 12);
-    put(p.tiles.data(), p.tiles.size() * 12);
+    put(p.rows.data(), p.rows.size() * paged::kItemWords);
+    put(p.tiles.data(), p.tiles.size() * paged::kItemWords);
     put(p.cta_first.data(), p.cta_first.size());
   } catch (const std::bad_alloc&) {
     set_error("kvq_paged_plan: out of host memory");

@@ -3,10 +3,10 @@
 // head is read once for all its rows.
 //
 // A CTA of four warps streams its pieces of the plan (kvq_paged_plan) one after the
-// other; warp w takes every fourth 16-token storage block of a piece. A block's K and
-// V records are contiguous, so a stage of the warp's ring is filled by two bulk copies
-// (no tensor map), kStages - 1 ahead; the warps never wait for each other inside a
-// piece. Per block (tokens j, rows n, channels c; mma.sync m16n8k16, bf16 in, fp32 out):
+// other; warp w takes every fourth pair of 16-token storage blocks of a piece. A block's K
+// and V records are contiguous, so a stage of the warp's ring is filled by four bulk
+// copies (no tensor map) while the other stage is worked on; the warps never wait for
+// each other inside a piece. Per block (tokens j, rows n, channels c; mma.sync m16n8k16, bf16 in, fp32 out):
 //   S^T[j, n] = sum_c K[j, c] q[n, c]      A = K from registers, B = q held in registers
 //   p = 2^(S^T scale - m_n)                m_n lags the true maximum by at most 8: it moves
 //                                          (and O, l are rescaled) only when some logit
@@ -36,17 +36,18 @@ constexpr int kRowThreads = 32 * kWarps;
 template <class L, int KB, int VB, int NT>
 struct RowGeo {
   static constexpr int kRecK = Rec<L, KB>::kBytes, kRecV = Rec<L, VB>::kBytes;
-  static constexpr int kStage = kRecK + kRecV;
-  static constexpr int kStages = kStage <= 3072 ? 5 : kStage <= 4096 ? 4 : 3;
+  static constexpr int kStage = 2 * (kRecK + kRecV);  // two storage blocks
+  static constexpr int kStages = 2;
   static constexpr int kRing = kStages * kStage;  // one warp's
-  static constexpr int kOffO = 0;  // the join reuses each warp's ring: 8 NT rows of 128 floats
   static constexpr int kOffML = kWarps * kRing;
   static constexpr int kOffBar = kOffML + kWarps * 8 * NT * 8;
   static constexpr int kOffMisc = kOffBar + kWarps * kStages * 8;
   static constexpr int kSmemBytes = kOffMisc + 16;
+  // resident blocks: shared memory, and registers (128 a thread for four, 168 for three)
+  static constexpr int kFit = (228 * 1024) / (kSmemBytes + 1024);
+  static constexpr int kCtas = kFit < (NT == 1 ? 4 : 3) ? kFit : (NT == 1 ? 4 : 3);
   static_assert(kRing >= 8 * NT * D * 4, "the join fits a warp's ring");
   static_assert(kRecK % 16 == 0 && kStage % 16 == 0, "bulk copies");
-  static_assert(kRowCtasPerSm * (kSmemBytes + 1024) <= 228 * 1024, "resident blocks");
 };
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -62,7 +63,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 template <class L, int KB, int VB, int NT>
-__global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) rows_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) rows_kernel(const __grid_constant__ AttnArgs a) {
   using GEO = RowGeo<L, KB, VB, NT>;
   constexpr int S = GEO::kStages, G = L::G;
   constexpr int KG = most_groups<L, 32>(), VG = most_groups<L, 16>();
@@ -112,27 +113,31 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) rows_kernel(const 
   const int i0 = __ldg(a.cta_first + blockIdx.x), i1 = __ldg(a.cta_first + blockIdx.x + 1);
   for (int ii = i0; ii < i1; ++ii) {
     const Item it = a.items[ii];
-    const kvq_paged_seq sq = a.p.seqs[it.seq];
-    const int start = sq.kv_len - sq.q_len;
-    int n_mine = it.je - it.jb > warp ? (it.je - it.jb - warp + kWarps - 1) / kWarps : 0;
+    // this warp's pairs of list entries: 2 (warp + kWarps k) and the next
+    const int n_blk = it.je - it.jb, n_pair = (n_blk + 1) / 2;
+    int n_mine = n_pair > warp ? (n_pair - warp + kWarps - 1) / kWarps : 0;
     if (__any_sync(0xffffffffu, *abort)) n_mine = 0;  // a wait gave up: only the counting goes on
     const uint32_t step0 = step;
+    auto entry = [&](int k) { return 2 * (warp + kWarps * k); };  // relative to jb
 
-    // copies: lane i of the warp looks up the block of step base + i, 32 steps at a time
+    // copies: lanes 2i, 2i + 1 look up the two blocks of step base + i, 16 steps at a time;
+    // lanes 0-3 copy the step's records: K, V of the first block, K, V of the second
     int64_t where = 0;
     auto issue = [&](int k) {
-      if ((k & 31) == 0) {
-        const int kk = k + lane;
+      if ((k & 15) == 0) {
+        const int e = entry(k + (lane >> 1)) + (lane & 1);
         bool ok;
-        if (kk < n_mine) where = a.p.block(it.seq, it.head, it.block_at(it.jb + warp + kWarps * kk), ok);
+        if (e < n_blk) where = a.p.block(it.seq, it.head, it.block_at(it.jb + e), ok);
       }
-      const int64_t b = __shfl_sync(0xffffffffu, where, k & 31);
-      if (lane == 0) {
-        const uint32_t st = (step0 + k) % S;
-        const uint32_t dst = smem_u32(ring) + st * GEO::kStage;
-        mbar_arrive_expect_tx(&bars[st], GEO::kStage);
-        bulk_load(dst, a.k_pages + b * GEO::kRecK, GEO::kRecK, &bars[st]);
-        bulk_load(dst + GEO::kRecK, a.v_pages + b * GEO::kRecV, GEO::kRecV, &bars[st]);
+      const int64_t b = __shfl_sync(0xffffffffu, where, 2 * (k & 15) + ((lane >> 1) & 1));
+      const uint32_t st = (step0 + k) % S;
+      const int nb = min(2, n_blk - entry(k));
+      if (lane == 0) mbar_arrive_expect_tx(&bars[st], nb * (GEO::kStage / 2));
+      __syncwarp();
+      if (lane < 2 * nb) {
+        const bool v = lane & 1;
+        bulk_load(smem_u32(ring) + st * GEO::kStage + (lane >> 1) * (GEO::kStage / 2) + (v ? GEO::kRecK : 0),
+                  v ? a.v_pages + b * GEO::kRecV : a.k_pages + b * GEO::kRecK, v ? GEO::kRecV : GEO::kRecK, &bars[st]);
       }
     };
     for (int k = 0; k < S - 1 && k < n_mine; ++k) issue(k);
@@ -144,7 +149,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) rows_kernel(const 
       const int n = 8 * nt + g;
       const int row = it.row0 + min(n, it.n_rows - 1);
       const int i = row / a.group;
-      const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(sq.q_first + i) * a.q_stride +
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(it.q_first + i) * a.q_stride +
                                                         (it.head * a.group + row - i * a.group) * D + 32 * t);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -163,10 +168,10 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) rows_kernel(const 
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = it.row0 + min(8 * nt + 2 * t + e, it.n_rows - 1);
-        see[nt][e] = seen_by(a, start + row / a.group, sq.kv_len);
+        see[nt][e] = seen_by(a, it.start + row / a.group, it.kv_len);
       }
-    const Seen first = seen_by(a, start + it.row0 / a.group, sq.kv_len);
-    const Seen final_ = seen_by(a, start + (it.row0 + it.n_rows - 1) / a.group, sq.kv_len);
+    const Seen first = seen_by(a, it.start + it.row0 / a.group, it.kv_len);
+    const Seen final_ = seen_by(a, it.start + (it.row0 + it.n_rows - 1) / a.group, it.kv_len);
 
     float o[NT][8][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -195,79 +200,92 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) rows_kernel(const 
           mbar_drain(&bars[(step0 + d) % S], ((step0 + d) / S) & 1, a.status, a.wait_cycles);
         break;
       }
-      const uint8_t* rk = ring + st * GEO::kStage;
-      const uint8_t* rv = rk + GEO::kRecK;
-      const int t0 = it.block_at(it.jb + warp + kWarps * k) * kBlock;
+      const uint8_t* rec0 = ring + st * GEO::kStage;
+      const int e0 = it.jb + entry(k);
+      const bool two = e0 + 1 < it.je;
+      const int ta = it.block_at(e0) * kBlock, tz = it.block_at(e0 + 1) * kBlock;  // first tokens of the blocks
+      const bool whole = two && tz + kBlock <= first.hi && (ta >= final_.lo || tz + kBlock <= first.kept);
 
       // ---- S^T
-      float s[NT][4];
+      float s[NT][2][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int bb = 0; bb < 2; ++bb) {
+        const uint8_t* rk = rec0 + bb * (GEO::kStage / 2);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
-      uint32_t kw[2][KB == 4 ? 4 : 8], ks01[2], ks23[2];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int tok = 8 * r + token_of(g);
-        const uint4* src = reinterpret_cast<const uint4*>(rk + tok * Rec<L, KB>::CW) + t * (KB / 4);
+          for (int e = 0; e < 4; ++e) s[nt][bb][e] = 0.0f;
+        uint32_t kw[2][KB == 4 ? 4 : 8], ks01[2], ks23[2];
 #pragma unroll
-        for (int w = 0; w < KB / 4; ++w) {
-          const uint4 v = src[w];
-          kw[r][4 * w] = v.x;
-          kw[r][4 * w + 1] = v.y;
-          kw[r][4 * w + 2] = v.z;
-          kw[r][4 * w + 3] = v.w;
-        }
-        const uint16_t* sc = reinterpret_cast<const uint16_t*>(rk + Rec<L, KB>::kCodes) + tok * G;
-        uint32_t x[4];
+        for (int r = 0; r < 2; ++r) {
+          const int tok = 8 * r + token_of(g);
+          const uint4* src = reinterpret_cast<const uint4*>(rk + tok * Rec<L, KB>::CW) + t * (KB / 4);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) x[q] = q < KG ? sc[KG == 1 ? kbase : min(kbase + q, G - 1)] : 0u;
-        if constexpr (KG == 1) {
-          ks01[r] = __byte_perm(x[0], 0, 0x1010);
-        } else {
-          ks01[r] = __byte_perm(x[0], x[1], 0x5410);
-          ks23[r] = __byte_perm(x[2], x[3], 0x5410);
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t f[2][4];
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t v;
-            if constexpr (KB == 4)
-              v = int4_pair(kw[r][w] >> (4 * j));
-            else
-              v = int8_pair(__byte_perm(kw[r][2 * w], kw[r][2 * w + 1], j | j << 4 | (4 + j) << 8 | (4 + j) << 12));
-            const uint32_t sp = KG == 1 ? ks01[r] : __byte_perm(ks01[r], ks23[r], ksel[KG == 1 ? 0 : 4 * w + j]);
-            f[r][j] = hmul2(v, sp);
+          for (int w = 0; w < KB / 4; ++w) {
+            const uint4 v = src[w];
+            kw[r][4 * w] = v.x;
+            kw[r][4 * w + 1] = v.y;
+            kw[r][4 * w + 2] = v.z;
+            kw[r][4 * w + 3] = v.w;
           }
+          const uint16_t* sc = reinterpret_cast<const uint16_t*>(rk + Rec<L, KB>::kCodes) + tok * G;
+          uint32_t x[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+          for (int q = 0; q < 4; ++q) x[q] = q < KG ? sc[KG == 1 ? kbase : min(kbase + q, G - 1)] : 0u;
+          ks01[r] = KG == 1 ? __byte_perm(x[0], 0, 0x1010) : __byte_perm(x[0], x[1], 0x5410);
+          if constexpr (KG > 2) ks23[r] = __byte_perm(x[2], x[3], 0x5410);
+          if constexpr (KB == 4) {  // for q / 4
+            ks01[r] = hmul2(ks01[r], kFour);
+            if constexpr (KG > 2) ks23[r] = hmul2(ks23[r], kFour);
+          }
+        }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816(s[nt], f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], qf[nt][2 * w + h][0],
-                     qf[nt][2 * w + h][1]);
+        for (int w = 0; w < 4; ++w) {
+          uint32_t f[2][4];
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t v;
+              if constexpr (KB == 4) {
+                const uint32_t x = j < 2 ? kw[r][w] : kw[r][w] >> 8;
+                v = (j & 1) ? int4_high(x) : int4_low(x);
+              } else {
+                v = int8_pair(__byte_perm(kw[r][2 * w], kw[r][2 * w + 1], j | j << 4 | (4 + j) << 8 | (4 + j) << 12));
+              }
+              uint32_t sp = ks01[r];
+              if constexpr (KG > 1) sp = __byte_perm(ks01[r], KG > 2 ? ks23[r] : 0u, ksel[4 * w + j]);
+              f[r][j] = hmul2(v, sp);
+            }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816(s[nt][bb], f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], qf[nt][2 * w + h][0],
+                       qf[nt][2 * w + h][1]);
+        }
       }
 
       // ---- softmax weights
-      const bool whole = t0 + kBlock <= first.hi && (t0 >= final_.lo || t0 + kBlock <= first.kept);
-      uint32_t pf[NT][2];
+      uint32_t pf[NT][2][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] *= a.scale_log2;
+        for (int bb = 0; bb < 2; ++bb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][bb][e] *= a.scale_log2;
         if (!whole) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = t0 + 8 * (e >> 1) + token_of(g);
-            const Seen& v = see[nt][e & 1];
-            if (!(j < v.hi && (j >= v.lo || j < v.kept))) s[nt][e] = -INFINITY;
-          }
+          for (int bb = 0; bb < 2; ++bb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = (bb ? tz : ta) + 8 * (e >> 1) + token_of(g);
+              const Seen& v = see[nt][e & 1];
+              if (!(j < v.hi && (j >= v.lo || j < v.kept)) || (bb && !two)) s[nt][bb][e] = -INFINITY;
+            }
         }
-        const float mx0 = fmaxf(s[nt][0], s[nt][2]), mx1 = fmaxf(s[nt][1], s[nt][3]);
+        const float mx0 = fmaxf(fmaxf(s[nt][0][0], s[nt][0][2]), fmaxf(s[nt][1][0], s[nt][1][2]));
+        const float mx1 = fmaxf(fmaxf(s[nt][0][1], s[nt][0][3]), fmaxf(s[nt][1][1], s[nt][1][3]));
         if (__any_sync(0xffffffffu, mx0 > m[nt][0] + 8.0f || mx1 > m[nt][1] + 8.0f)) {
           float n0 = mx0, n1 = mx1;
 #pragma unroll
@@ -290,68 +308,81 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) rows_kernel(const 
             o[nt][i][3] *= a1;
           }
         }
-        float p[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = ex2f(s[nt][e] - m[nt][e & 1]);
-        l[nt][0] += p[0] + p[2];
-        l[nt][1] += p[1] + p[3];
-        pf[nt][0] = transpose8x8(pack_bf16x2(p[0], p[1]));
-        pf[nt][1] = transpose8x8(pack_bf16x2(p[2], p[3]));
+        for (int bb = 0; bb < 2; ++bb) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[e] = ex2f(s[nt][bb][e] - m[nt][e & 1]);
+          l[nt][0] += p[0] + p[2];
+          l[nt][1] += p[1] + p[3];
+          pf[nt][bb][0] = transpose8x8(pack_bf16x2(p[0], p[1]));
+          pf[nt][bb][1] = transpose8x8(pack_bf16x2(p[2], p[3]));
+        }
       }
 
       // ---- O^T: this lane's tokens are S rows 2t, 2t + 1, 8 + 2t, 9 + 2t
       const int vt[4] = {token_of(2 * t), token_of(2 * t + 1), 8 + token_of(2 * t), 8 + token_of(2 * t + 1)};
-      uint32_t vw[4][VB == 4 ? 2 : 4], vs[2][VG];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if constexpr (VB == 4) {
-          const uint2 v = reinterpret_cast<const uint2*>(rv + vt[u] * Rec<L, VB>::CW)[g];
-          vw[u][0] = v.x;
-          vw[u][1] = v.y;
-        } else {
-          const uint4 v = reinterpret_cast<const uint4*>(rv + vt[u] * Rec<L, VB>::CW)[g];
-          vw[u][0] = v.x;
-          vw[u][1] = v.y;
-          vw[u][2] = v.z;
-          vw[u][3] = v.w;
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < VG; ++q) {
-        uint32_t x[4];
+      for (int bb = 0; bb < 2; ++bb) {
+        const uint8_t* rv = rec0 + bb * (GEO::kStage / 2) + GEO::kRecK;
+        uint32_t vw[4][VB == 4 ? 2 : 4], vs[2][VG];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const uint16_t* sc = reinterpret_cast<const uint16_t*>(rv + Rec<L, VB>::kCodes) + vt[u] * G;
-          x[u] = sc[VG == 1 ? vbase : min(vbase + q, G - 1)];
-          // rows past the end hold anything: as zeros they add nothing
-          if (!whole && t0 + vt[u] >= sq.kv_len) x[u] = 0;
-        }
-        vs[0][q] = __byte_perm(x[0], x[1], 0x5410);
-        vs[1][q] = __byte_perm(x[2], x[3], 0x5410);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {  // channels 16g + 2i (rows g) and 16g + 2i + 1 (rows 8 + g)
-        uint32_t f[2][2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t sp = vs[u][0];
-          if (VG > 1) sp = i >= ve1 ? vs[u][VG > 1 ? 1 : 0] : sp;
-          if (VG > 2) sp = i >= ve2 ? vs[u][VG > 2 ? 2 : 0] : sp;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint32_t v;
-            if constexpr (VB == 4) {
-              const uint32_t x = __byte_perm(vw[2 * u][i >> 2], vw[2 * u + 1][i >> 2], (i & 2) ? 0x7632 : 0x5410);
-              v = int4_pair(x >> (8 * (i & 1) + 4 * e));
-            } else {
-              const int c = 2 * i + e, b = c & 3;
-              v = int8_pair(__byte_perm(vw[2 * u][c >> 2], vw[2 * u + 1][c >> 2], b | b << 4 | (4 + b) << 8 | (4 + b) << 12));
-            }
-            f[u][e] = hmul2(v, sp);
+          if constexpr (VB == 4) {
+            const uint2 v = reinterpret_cast<const uint2*>(rv + vt[u] * Rec<L, VB>::CW)[g];
+            vw[u][0] = v.x;
+            vw[u][1] = v.y;
+          } else {
+            const uint4 v = reinterpret_cast<const uint4*>(rv + vt[u] * Rec<L, VB>::CW)[g];
+            vw[u][0] = v.x;
+            vw[u][1] = v.y;
+            vw[u][2] = v.z;
+            vw[u][3] = v.w;
           }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][i], f[0][0], f[0][1], f[1][0], f[1][1], pf[nt][0], pf[nt][1]);
+        for (int q = 0; q < VG; ++q) {
+          uint32_t x[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const uint16_t* sc = reinterpret_cast<const uint16_t*>(rv + Rec<L, VB>::kCodes) + vt[u] * G;
+            x[u] = sc[VG == 1 ? vbase : min(vbase + q, G - 1)];
+            // rows past the end hold anything: as zeros they add nothing
+            if (!whole && ((bb ? tz : ta) + vt[u] >= it.kv_len || (bb && !two))) x[u] = 0;
+          }
+          vs[0][q] = __byte_perm(x[0], x[1], 0x5410);
+          vs[1][q] = __byte_perm(x[2], x[3], 0x5410);
+          if constexpr (VB == 4) {  // for q / 4
+            vs[0][q] = hmul2(vs[0][q], kFour);
+            vs[1][q] = hmul2(vs[1][q], kFour);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // channels 16g + 2i (rows g) and 16g + 2i + 1 (rows 8 + g)
+          uint32_t f[2][2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t sp = vs[u][0];
+            if (VG > 1) sp = i >= ve1 ? vs[u][VG > 1 ? 1 : 0] : sp;
+            if (VG > 2) sp = i >= ve2 ? vs[u][VG > 2 ? 2 : 0] : sp;
+            if constexpr (VB == 4) {
+              const int b = i & 3;  // the byte with both channels, of either token
+              const uint32_t x = __byte_perm(vw[2 * u][i >> 2], vw[2 * u + 1][i >> 2], b | b << 4 | (4 + b) << 8 | (4 + b) << 12);
+              f[u][0] = hmul2(int4_low(x), sp);
+              f[u][1] = hmul2(int4_high(x), sp);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int c = 2 * i + e, b = c & 3;
+                f[u][e] = hmul2(int8_pair(__byte_perm(vw[2 * u][c >> 2], vw[2 * u + 1][c >> 2],
+                                                      b | b << 4 | (4 + b) << 8 | (4 + b) << 12)), sp);
+              }
+            }
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma16816(o[nt][i], f[0][0], f[0][1], f[1][0], f[1][1], pf[nt][bb][0], pf[nt][bb][1]);
+        }
       }
       __syncwarp();
     }
@@ -381,7 +412,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) rows_kernel(const 
     float* slot = it.parts > 1 ? a.ws + static_cast<int64_t>(it.slot + it.part) * slot_floats(kRows) : nullptr;
     auto finish = [&](int n, int c, float acc, float mm, float total) {
       const int row = it.row0 + n, i = row / a.group;
-      const int64_t tok = sq.q_first + i;
+      const int64_t tok = it.q_first + i;
       const int h = it.head * a.group + row - i * a.group;
       a.out[tok * a.out_stride + h * D + c] = f32_to_bf16_bits(total == 0.0f ? 0.0f : acc / total);
       if (a.lse && c == 0)
@@ -442,6 +473,16 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) rows_kernel(const 
     fence_proxy_async_smem();
     __syncthreads();
   }
+}
+
+int rows_ctas_per_sm(int layout, int k_bits, int v_bits, int row_tile) {
+  return with_layout(layout, [&](auto lt) {
+    using L = decltype(lt);
+    return with_bits(k_bits, v_bits, [&](auto bt) -> int {
+      using B = decltype(bt);
+      return row_tile == 8 ? RowGeo<L, B::k, B::v, 1>::kCtas : RowGeo<L, B::k, B::v, 2>::kCtas;
+    });
+  });
 }
 
 int launch_rows(const AttnArgs& a, int layout, int k_bits, int v_bits, int row_tile, int n_ctas, cudaStream_t st) {

@@ -132,6 +132,10 @@ struct Converter {
       s01 = __byte_perm(x[0], x[1], 0x5410);
       if constexpr (KG > 2) s23 = __byte_perm(x[2], x[3], 0x5410);
     }
+    if constexpr (BITS == 4) {
+      s01 = hmul2(s01, kFour);
+      s23 = hmul2(s23, kFour);
+    }
     if (!live) s01 = s23 = 0;  // rows past the end hold anything: as zeros they add nothing
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -140,7 +144,7 @@ struct Converter {
       if constexpr (BITS == 4) {
         const uint32_t x = hi ? w[i ^ 2] : w[i], y = x >> 4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = int4_pair(__byte_perm(x, y, (4 + j) << 8 | j));
+        for (int j = 0; j < 4; ++j) o[j] = int4_low(__byte_perm(x, y, (4 + j) << 8 | j));
       } else {
         const uint32_t x = hi ? w[2 * (i ^ 2)] : w[2 * i], y = hi ? w[2 * (i ^ 2) + 1] : w[2 * i + 1];
         o[0] = int8_pair(__byte_perm(x, 0, 0x4140));
@@ -171,8 +175,6 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   pdl_wait();
   pdl_launch_dependents();
   const Item it = a.items[blockIdx.x];
-  const kvq_paged_seq sq = a.p.seqs[it.seq];
-  const int start = sq.kv_len - sq.q_len;
   const int nq = it.n_rows > BM ? 2 : 1;
   const int n_blk = it.je - it.jb;  // entries of the block list
   const int nkv = (n_blk + 3) / 4;
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   // where row n of the item reads its query and writes its output
   auto place = [&](int n, int64_t& tok, int& h) {
     const int row = it.row0 + n, i = row / a.group;
-    tok = sq.q_first + i;
+    tok = it.q_first + i;
     h = it.head * a.group + row - i * a.group;
   };
   // A warp's 32 output rows (rows n0.. of the item, rr0.. of the Q tile), staged in
@@ -274,9 +276,9 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     const uint32_t tO = tmem + lane_off + kColO + 128 * x;
     const uint32_t tS0 = tmem + lane_off + kColS + 128 * x;
     const int n_last = min(x * BM + BM, it.n_rows) - 1;
-    const Seen see = seen_by(a, start + (it.row0 + min(n, it.n_rows - 1)) / a.group, sq.kv_len);
-    const Seen first = seen_by(a, start + (it.row0 + x * BM) / a.group, sq.kv_len);
-    const Seen fin = seen_by(a, start + (it.row0 + n_last) / a.group, sq.kv_len);
+    const Seen see = seen_by(a, it.start + (it.row0 + min(n, it.n_rows - 1)) / a.group, it.kv_len);
+    const Seen first = seen_by(a, it.start + (it.row0 + x * BM) / a.group, it.kv_len);
+    const Seen fin = seen_by(a, it.start + (it.row0 + n_last) / a.group, it.kv_len);
     float m = -1.0e30f, l = 0.0f;
     bool ok = true;
     auto step = [&](const int j, auto masked) -> bool {
@@ -435,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
 #pragma unroll 2
         for (int p = 0; p < 4; ++p) {
           const int r = r0 + 8 * p, e = it.jb + 4 * j + (r >> 4);
-          const bool live = e < it.je && it.block_at(e) * kBlock + (r & 15) < sq.kv_len;
+          const bool live = e < it.je && it.block_at(e) * kBlock + (r & 15) < it.kv_len;
           conv.row(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, dst, r, t, live);
         }
         fence_proxy_async_smem();

@@ -47,7 +47,7 @@ SIGNATURES = {
     "kvq_device_status": (_i32, [_i32]),
     "kvq_paged_append": (_i32, [_p, _i64, _p, _i64, _p, _p, _p]),
     "kvq_paged_read": (_i32, [_p, _p, _i32, _p, _i64, _p, _i64, _p]),
-    "kvq_paged_plan": (_i32, [_p, _p, _i32, _i32, _i32, _i32, _i64, _i64, _i32, _p, _i64, _p]),
+    "kvq_paged_plan": (_i32, [_p, _p, _p, _i32, _i32, _i32, _i64, _i64, _i32, _p, _i64, _p]),
     "kvq_paged_attention": (_i32, [_p, _i64, _p, _p, _p, _i64, _p, _i32, _i32, _i64, _i64, _f32, _p, _p, _p, _p, _p]),
 }
 

@@ -125,13 +125,13 @@ class PagedBatch:
         rows = np.where(used, table, 0)[:, :width].astype(np.int32)
         self._upload(seqs, rows)
 
-    def _plan(self, n_heads: int, n_q_heads: int, causal: bool, window: int, sink: int) -> "_Plan":
-        """The work list of attention with these heads and masks, made at its first use in
-        the step and shared by the step's layers."""
-        key = (n_heads, n_q_heads, causal, window, sink)
+    def _plan(self, cache: "PagedKVCache", n_q_heads: int, causal: bool, window: int, sink: int) -> "_Plan":
+        """The work list of attention with this cache format, heads and masks, made at its
+        first use in the step and shared by the step's layers."""
+        key = (cache._format, n_q_heads, causal, window, sink)
         plan = self._plans.get(key)
         if plan is None:
-            plan = self._plans[key] = _Plan(self, *key)
+            plan = self._plans[key] = _Plan(self, cache, n_q_heads, causal, window, sink)
         return plan
 
     def _upload(self, seqs: np.ndarray, rows: np.ndarray) -> None:
@@ -177,20 +177,21 @@ class _Plan:
     """kvq_paged_plan of a batch: the work list on the device, and per stream a workspace
     and counters, so that launches on different streams may overlap."""
 
-    def __init__(self, batch: PagedBatch, n_heads: int, n_q_heads: int, causal: bool, window: int, sink: int):
+    def __init__(self, batch: PagedBatch, cache: "PagedKVCache", n_q_heads: int, causal: bool, window: int, sink: int):
         kv, ql = batch.kv_lens.astype(np.int32), batch.q_lens.astype(np.int32)
         self.info = _lib.PagedPlanInfo()
         sms = torch.cuda.get_device_properties(batch.device).multi_processor_count
         lib = _lib.load()
-        words = np.empty(0, dtype=np.int32)
-        for _ in range(2):  # its size, then the plan
-            rc = lib.kvq_paged_plan(kv.ctypes.data, ql.ctypes.data, len(kv), n_heads, n_q_heads, causal, window, sink, sms,
-                                    words.ctypes.data if words.size else None, words.size, ctypes.byref(self.info))
-            _lib.check(rc, "kvq_paged_plan")
-            if words.size == 0:
-                words = np.empty(self.info.words, dtype=np.int32)
+        words = np.empty(1 << 15, dtype=np.int32)
+        for _ in range(2):  # again with more room where the plan is longer
+            rc = lib.kvq_paged_plan(cache._ref(), kv.ctypes.data, ql.ctypes.data, len(kv), n_q_heads, causal, window, sink,
+                                    sms, words.ctypes.data, words.size, ctypes.byref(self.info))
+            if self.info.words <= words.size:
+                break
+            words = np.empty(self.info.words, dtype=np.int32)
+        _lib.check(rc, "kvq_paged_plan")
         self.device = batch.device
-        self.items = _Uploaded(words, batch.device)
+        self.items = _Uploaded(words[:self.info.words], batch.device)
         self._work = {}
 
     def args(self):
@@ -239,6 +240,7 @@ class PagedKVCache:
         self._c = _lib.PagedCacheArgs(None, None, self.n_pages, self.page_size, self.n_heads, self.head_dim, self.k_bits,
                                       self.v_bits, len(self.bands), self._map.ctypes.data)
         self._c_ref = ctypes.byref(self._c)
+        self._format = (self.n_heads, self.k_bits, self.v_bits, group_mode)
 
     def _row_bytes(self, bits: int) -> int:
         return self._code_bytes(bits) + 2 * len(self.bands)
@@ -364,7 +366,7 @@ def attention(q: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, causal: b
     elif _rows(out, shape, cache.device, "out") is not out:
         raise ValueError("out must have contiguous [heads, channels] blocks, 16-byte aligned rows")
     lse = torch.empty(shape[:2], dtype=torch.float32, device=cache.device) if return_lse else None
-    plan = batch._plan(cache.n_heads, heads, bool(causal), window, sink)
+    plan = batch._plan(cache, heads, bool(causal), window, sink)
     _call(cache.device, _lib.load().kvq_paged_attention, "kvq_paged_attention", q.data_ptr(), _row_stride(q), cache._ref(),
           batch._ref(), out.data_ptr(), _row_stride(out), lse.data_ptr() if return_lse else None, heads,
           1 if causal else 0, window, sink, scale, *plan.args())
