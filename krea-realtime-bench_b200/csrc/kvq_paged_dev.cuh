@@ -15,6 +15,21 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
                : "memory");
 }
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_shared_u16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
+}
 __device__ __forceinline__ float ex2f(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -40,15 +55,23 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
 //         a bf16 with that exponent or none is linear in its bits: code * 2^-129, times
 //         2^127, minus 2.
 // With four times the scale the product is q * s, rounded once.
+// (x & m) | o as one instruction: from the C expression the compiler made two.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t o) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(m), "r"(o));
+  return y;
+}
 __device__ __forceinline__ uint32_t int4_low(uint32_t x) {
-  return hfma2((x & 0x000F000Fu) | 0x43004300u, 0x3E803E80u, 0xC208C208u);
+  return hfma2(and_or(x, 0x000F000Fu, 0x43004300u), 0x3E803E80u, 0xC208C208u);
 }
 __device__ __forceinline__ uint32_t int4_high(uint32_t x) { return hfma2(x & 0x00F000F0u, 0x7F007F00u, 0xC000C000u); }
 constexpr uint32_t kFour = 0x40804080u;  // bf16x2 (4, 4)
 // Bytes at bits 0-7 and 16-23 (code = q + 128) -> bf16x2 (q, q). The low seven bits give
 // 128 + code % 128, from which 256 is taken, or 128 where the top bit is set.
 __device__ __forceinline__ uint32_t int8_pair(uint32_t x) {
-  return hsub2((x & 0x007F007Fu) | 0x43004300u, (x & 0x00800080u) ^ 0x43804380u);
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(d) : "r"(x), "r"(0x00800080u), "r"(0x43804380u));  // (x & m) ^ o
+  return hsub2(and_or(x, 0x007F007Fu, 0x43004300u), d);
 }
 
 // Most channel groups that an aligned run of N channels meets.

@@ -65,19 +65,20 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 template <class L, int KB, int VB, int NT>
 __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) rows_kernel(const __grid_constant__ AttnArgs a) {
   using GEO = RowGeo<L, KB, VB, NT>;
-  constexpr int S = GEO::kStages, G = L::G;
+  constexpr int G = L::G;
+  static_assert(GEO::kStages == 2, "stage and phase below");
   constexpr int KG = most_groups<L, 32>(), VG = most_groups<L, 16>();
   static_assert(KG <= 4 && VG <= 3, "group selection");
   constexpr int kRows = 8 * NT;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + GEO::kOffBar) + warp * S;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + GEO::kOffBar) + warp * GEO::kStages;
   volatile int* abort = reinterpret_cast<volatile int*>(smem + GEO::kOffMisc);
   volatile int* last = abort + 1;
   uint8_t* ring = smem + warp * GEO::kRing;
   float* sm_ml = reinterpret_cast<float*>(smem + GEO::kOffML);  // [warp][row][2]
   if (lane == 0) {
-    for (int i = 0; i < S; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < GEO::kStages; ++i) mbar_init(&bars[i], 1);
     fence_mbar_init();
   }
   if (tid == 0) *abort = 0;
@@ -107,6 +108,18 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
   // physical token of S row r: a permutation that spreads both K and V reads over the banks
   auto token_of = [](int r) { return r ^ ((r >> 1) & 1); };
 
+  // what lanes 0-3 copy at each step
+  const uint32_t copy_bytes = (lane & 1) ? GEO::kRecV : GEO::kRecK;
+  const uint8_t* copy_src = (lane & 1) ? a.v_pages : a.k_pages;
+  const uint32_t copy_dst = smem_u32(ring) + ((lane >> 1) & 1) * (GEO::kStage / 2) + ((lane & 1) ? GEO::kRecK : 0);
+  // this lane's K row and V rows inside a stage, codes and scales
+  const uint32_t k_codes = smem_u32(ring) + token_of(g) * Rec<L, KB>::CW + t * (KB * 4);
+  const uint32_t k_scales = smem_u32(ring) + Rec<L, KB>::kCodes + token_of(g) * G * 2;
+  const int vt0 = token_of(2 * t), vt1 = token_of(2 * t + 1);  // and 8 more
+  const uint32_t v_ring = smem_u32(ring) + GEO::kRecK;
+  const uint32_t v_codes0 = v_ring + vt0 * Rec<L, VB>::CW + g * (2 * VB), v_codes1 = v_codes0 + (vt1 - vt0) * Rec<L, VB>::CW;
+  const uint32_t v_scales0 = v_ring + Rec<L, VB>::kCodes + vt0 * G * 2, v_scales1 = v_scales0 + (vt1 - vt0) * G * 2;
+
   pdl_wait();
   pdl_launch_dependents();
   uint32_t step = 0;  // blocks this warp has consumed, over all pieces: stage and phase
@@ -122,25 +135,22 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
 
     // copies: lanes 2i, 2i + 1 look up the two blocks of step base + i, 16 steps at a time;
     // lanes 0-3 copy the step's records: K, V of the first block, K, V of the second
-    int64_t where = 0;
+    uint32_t where = 0;
     auto issue = [&](int k) {
       if ((k & 15) == 0) {
         const int e = entry(k + (lane >> 1)) + (lane & 1);
         bool ok;
-        if (e < n_blk) where = a.p.block(it.seq, it.head, it.block_at(it.jb + e), ok);
+        if (e < n_blk) where = static_cast<uint32_t>(a.p.block(it.seq, it.head, it.block_at(it.jb + e), ok));
       }
-      const int64_t b = __shfl_sync(0xffffffffu, where, 2 * (k & 15) + ((lane >> 1) & 1));
-      const uint32_t st = (step0 + k) % S;
-      const int nb = min(2, n_blk - entry(k));
-      if (lane == 0) mbar_arrive_expect_tx(&bars[st], nb * (GEO::kStage / 2));
+      const uint32_t b = __shfl_sync(0xffffffffu, where, 2 * (k & 15) + ((lane >> 1) & 1));
+      const uint32_t st = (step0 + k) & 1;
+      const bool two = entry(k) + 1 < n_blk;
+      if (lane == 0) mbar_arrive_expect_tx(&bars[st], two ? GEO::kStage : GEO::kStage / 2);
       __syncwarp();
-      if (lane < 2 * nb) {
-        const bool v = lane & 1;
-        bulk_load(smem_u32(ring) + st * GEO::kStage + (lane >> 1) * (GEO::kStage / 2) + (v ? GEO::kRecK : 0),
-                  v ? a.v_pages + b * GEO::kRecV : a.k_pages + b * GEO::kRecK, v ? GEO::kRecV : GEO::kRecK, &bars[st]);
-      }
+      if (lane < (two ? 4 : 2))
+        bulk_load(copy_dst + st * GEO::kStage, copy_src + static_cast<uint64_t>(b) * copy_bytes, copy_bytes, &bars[st]);
     };
-    for (int k = 0; k < S - 1 && k < n_mine; ++k) issue(k);
+    if (n_mine > 0) issue(0);
 
     // q fragments: rows 8 nt + g, channels (32t + 8i + 2h + {0, 4}) and the next two
     uint32_t qf[NT][8][2];
@@ -184,23 +194,21 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
       l[nt][0] = l[nt][1] = 0.0f;
     }
 
-    bool ok = true;
     for (int k = 0; k < n_mine; ++k) {
-      const uint32_t st = (step0 + k) % S;
-      if (k + S - 1 < n_mine) {
-        // stage of step k - 1: every lane has read it (the __syncwarp that ended that step)
-        issue(k + S - 1);
+      const uint32_t st = (step0 + k) & 1;
+      // the other stage: every lane has read it (the __syncwarp that ended the last step)
+      if (k + 1 < n_mine) issue(k + 1);
+      const uint32_t phase = ((step0 + k) >> 1) & 1;
+      if (!__all_sync(0xffffffffu, mbar_try_wait(smem_u32(&bars[st]), phase))) {
+        const bool ok = mbar_wait(&bars[st], phase, abort, a.status, a.wait_cycles);
+        if (!__all_sync(0xffffffffu, ok)) {
+          // copies in flight land before the shared memory is given up
+          mbar_drain(&bars[st], phase, a.status, a.wait_cycles);
+          if (k + 1 < n_mine) mbar_drain(&bars[st ^ 1], ((step0 + k + 1) >> 1) & 1, a.status, a.wait_cycles);
+          break;
+        }
       }
-      ok = mbar_wait(&bars[st], ((step0 + k) / S) & 1, abort, a.status, a.wait_cycles);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        // copies in flight land before the shared memory is given up
-        const int issued = min(n_mine, k + S);
-        for (int d = k; d < issued; ++d)
-          mbar_drain(&bars[(step0 + d) % S], ((step0 + d) / S) & 1, a.status, a.wait_cycles);
-        break;
-      }
-      const uint8_t* rec0 = ring + st * GEO::kStage;
+      const uint32_t at = st * GEO::kStage;
       const int e0 = it.jb + entry(k);
       const bool two = e0 + 1 < it.je;
       const int ta = it.block_at(e0) * kBlock, tz = it.block_at(e0 + 1) * kBlock;  // first tokens of the blocks
@@ -210,7 +218,6 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
       float s[NT][2][4];
 #pragma unroll
       for (int bb = 0; bb < 2; ++bb) {
-        const uint8_t* rk = rec0 + bb * (GEO::kStage / 2);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -218,20 +225,19 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
         uint32_t kw[2][KB == 4 ? 4 : 8], ks01[2], ks23[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int tok = 8 * r + token_of(g);
-          const uint4* src = reinterpret_cast<const uint4*>(rk + tok * Rec<L, KB>::CW) + t * (KB / 4);
+          const uint32_t src = k_codes + at + bb * (GEO::kStage / 2) + 8 * r * Rec<L, KB>::CW;
 #pragma unroll
           for (int w = 0; w < KB / 4; ++w) {
-            const uint4 v = src[w];
+            const uint4 v = ld_shared_v4(src + 16 * w);
             kw[r][4 * w] = v.x;
             kw[r][4 * w + 1] = v.y;
             kw[r][4 * w + 2] = v.z;
             kw[r][4 * w + 3] = v.w;
           }
-          const uint16_t* sc = reinterpret_cast<const uint16_t*>(rk + Rec<L, KB>::kCodes) + tok * G;
+          const uint32_t sc = k_scales + at + bb * (GEO::kStage / 2) + 8 * r * G * 2;
           uint32_t x[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) x[q] = q < KG ? sc[KG == 1 ? kbase : min(kbase + q, G - 1)] : 0u;
+          for (int q = 0; q < 4; ++q) x[q] = q < KG ? ld_shared_u16(sc + 2 * (KG == 1 ? kbase : min(kbase + q, G - 1))) : 0u;
           ks01[r] = KG == 1 ? __byte_perm(x[0], 0, 0x1010) : __byte_perm(x[0], x[1], 0x5410);
           if constexpr (KG > 2) ks23[r] = __byte_perm(x[2], x[3], 0x5410);
           if constexpr (KB == 4) {  // for q / 4
@@ -270,10 +276,6 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
       uint32_t pf[NT][2][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int bb = 0; bb < 2; ++bb)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][bb][e] *= a.scale_log2;
         if (!whole) {
 #pragma unroll
           for (int bb = 0; bb < 2; ++bb)
@@ -284,8 +286,8 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
               if (!(j < v.hi && (j >= v.lo || j < v.kept)) || (bb && !two)) s[nt][bb][e] = -INFINITY;
             }
         }
-        const float mx0 = fmaxf(fmaxf(s[nt][0][0], s[nt][0][2]), fmaxf(s[nt][1][0], s[nt][1][2]));
-        const float mx1 = fmaxf(fmaxf(s[nt][0][1], s[nt][0][3]), fmaxf(s[nt][1][1], s[nt][1][3]));
+        const float mx0 = fmaxf(fmaxf(s[nt][0][0], s[nt][0][2]), fmaxf(s[nt][1][0], s[nt][1][2])) * a.scale_log2;
+        const float mx1 = fmaxf(fmaxf(s[nt][0][1], s[nt][0][3]), fmaxf(s[nt][1][1], s[nt][1][3])) * a.scale_log2;
         if (__any_sync(0xffffffffu, mx0 > m[nt][0] + 8.0f || mx1 > m[nt][1] + 8.0f)) {
           float n0 = mx0, n1 = mx1;
 #pragma unroll
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
         for (int bb = 0; bb < 2; ++bb) {
           float p[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = ex2f(s[nt][bb][e] - m[nt][e & 1]);
+          for (int e = 0; e < 4; ++e) p[e] = ex2f(fmaf(s[nt][bb][e], a.scale_log2, -m[nt][e & 1]));
           l[nt][0] += p[0] + p[2];
           l[nt][1] += p[1] + p[3];
           pf[nt][bb][0] = transpose8x8(pack_bf16x2(p[0], p[1]));
@@ -321,19 +323,19 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
       }
 
       // ---- O^T: this lane's tokens are S rows 2t, 2t + 1, 8 + 2t, 9 + 2t
-      const int vt[4] = {token_of(2 * t), token_of(2 * t + 1), 8 + token_of(2 * t), 8 + token_of(2 * t + 1)};
 #pragma unroll
       for (int bb = 0; bb < 2; ++bb) {
-        const uint8_t* rv = rec0 + bb * (GEO::kStage / 2) + GEO::kRecK;
+        const uint32_t off = at + bb * (GEO::kStage / 2);
         uint32_t vw[4][VB == 4 ? 2 : 4], vs[2][VG];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
+          const uint32_t src = ((u & 1) ? v_codes1 : v_codes0) + off + (u >> 1) * 8 * Rec<L, VB>::CW;
           if constexpr (VB == 4) {
-            const uint2 v = reinterpret_cast<const uint2*>(rv + vt[u] * Rec<L, VB>::CW)[g];
+            const uint2 v = ld_shared_v2(src);
             vw[u][0] = v.x;
             vw[u][1] = v.y;
           } else {
-            const uint4 v = reinterpret_cast<const uint4*>(rv + vt[u] * Rec<L, VB>::CW)[g];
+            const uint4 v = ld_shared_v4(src);
             vw[u][0] = v.x;
             vw[u][1] = v.y;
             vw[u][2] = v.z;
@@ -345,10 +347,10 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           uint32_t x[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const uint16_t* sc = reinterpret_cast<const uint16_t*>(rv + Rec<L, VB>::kCodes) + vt[u] * G;
-            x[u] = sc[VG == 1 ? vbase : min(vbase + q, G - 1)];
+            const uint32_t sc = ((u & 1) ? v_scales1 : v_scales0) + off + (u >> 1) * 8 * G * 2;
+            x[u] = ld_shared_u16(sc + 2 * (VG == 1 ? vbase : min(vbase + q, G - 1)));
             // rows past the end hold anything: as zeros they add nothing
-            if (!whole && ((bb ? tz : ta) + vt[u] >= it.kv_len || (bb && !two))) x[u] = 0;
+            if (!whole && ((bb ? tz : ta) + ((u & 1) ? vt1 : vt0) + (u >> 1) * 8 >= it.kv_len || (bb && !two))) x[u] = 0;
           }
           vs[0][q] = __byte_perm(x[0], x[1], 0x5410);
           vs[1][q] = __byte_perm(x[2], x[3], 0x5410);
@@ -451,21 +453,68 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
       }
       __syncthreads();
       if (*last) {
+        // Every part's (m, l) first, then its weight 2^(m_p - m), then the rows: a warp takes
+        // every fourth part, eight rows at a time, so that many loads are in flight.
         __threadfence();
         const float* base = a.ws + static_cast<int64_t>(it.slot) * slot_floats(kRows);
-        for (int n = 0; n < it.n_rows; ++n) {
-          float mm = -1.0e30f;
-          for (int p = 0; p < it.parts; ++p)
-            mm = fmaxf(mm, __ldcg(base + static_cast<int64_t>(p) * slot_floats(kRows) + kRows * D + 2 * n));
-          float total = 0.0f, acc = 0.0f;
-#pragma unroll 4
-          for (int p = 0; p < it.parts; ++p) {
-            const float* sp = base + static_cast<int64_t>(p) * slot_floats(kRows);
-            const float f = ex2f(__ldcg(sp + kRows * D + 2 * n) - mm);
-            total += f * __ldcg(sp + kRows * D + 2 * n + 1);
-            acc += f * __ldcg(sp + n * D + tid);
+        float* sm_f = reinterpret_cast<float*>(smem);                     // [part][row] m, then the weight
+        float* sm_l = sm_f + it.parts * kRows;                            // [part][row]
+        float* sm_o = reinterpret_cast<float*>(smem) + 2 * kMaxParts * kRows;  // [warp][8][D]
+        static_assert((2 * kMaxParts * kRows + kWarps * 8 * D) * 4 <= kWarps * GEO::kRing, "the join fits the rings");
+        for (int i = tid; i < it.parts * kRows; i += kRowThreads) {
+          const int q = i / kRows, n = i - q * kRows;
+          if (n < it.n_rows) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(base + static_cast<int64_t>(q) * slot_floats(kRows) +
+                                                                     kRows * D) + n);
+            sm_f[i] = ml.x;
+            sm_l[i] = ml.y;
           }
-          finish(n, tid, acc, mm, total);
+        }
+        __syncthreads();
+        for (int n = warp; n < it.n_rows; n += kWarps) {
+          float mm = -1.0e30f, total = 0.0f;
+          for (int q = lane; q < it.parts; q += 32) mm = fmaxf(mm, sm_f[q * kRows + n]);
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+          for (int q = lane; q < it.parts; q += 32) {
+            const float f = ex2f(sm_f[q * kRows + n] - mm);
+            sm_f[q * kRows + n] = f;
+            total += f * sm_l[q * kRows + n];
+          }
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+          if (lane == 0) {
+            sm_ml[2 * n] = mm;
+            sm_ml[2 * n + 1] = total;
+          }
+        }
+        __syncthreads();
+        for (int n0 = 0; n0 < it.n_rows; n0 += 8) {
+          float4 acc[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) acc[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+          for (int q = warp; q < it.parts; q += kWarps) {
+            const float4* src = reinterpret_cast<const float4*>(base + static_cast<int64_t>(q) * slot_floats(kRows) + n0 * D);
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+              if (n0 + r < it.n_rows) {
+                const float f = sm_f[q * kRows + n0 + r];
+                const float4 v = __ldcg(src + r * (D / 4) + lane);
+                acc[r] = make_float4(fmaf(f, v.x, acc[r].x), fmaf(f, v.y, acc[r].y), fmaf(f, v.z, acc[r].z),
+                                     fmaf(f, v.w, acc[r].w));
+              }
+          }
+#pragma unroll
+          for (int r = 0; r < 8; ++r) reinterpret_cast<float4*>(sm_o + (warp * 8 + r) * D)[lane] = acc[r];
+          __syncthreads();
+          for (int r = 0; r < 8 && n0 + r < it.n_rows; ++r) {
+            float x = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) x += sm_o[(w * 8 + r) * D + tid];
+            finish(n0 + r, tid, x, sm_ml[2 * (n0 + r)], sm_ml[2 * (n0 + r) + 1]);
+          }
+          __syncthreads();
         }
       }
     }
