@@ -51,7 +51,9 @@ extern "C" int kvq_paged_attention(const void* q, int64_t q_token_stride, const 
   a.sink = sink;
   a.scale_log2 = (softmax_scale > 0.0f ? softmax_scale : 1.0f / sqrtf(128.0f)) * 1.4426950408889634f;
   a.items = reinterpret_cast<const paged::Item*>(plan);
-  a.cta_first = plan + static_cast<int64_t>(info->n_row_items + info->n_tile_items) * paged::kItemWords;
+  a.cta_first = info->n_row_items == info->n_row_ctas
+                    ? nullptr
+                    : plan + static_cast<int64_t>(info->n_row_items + info->n_tile_items) * paged::kItemWords;
   a.ws = static_cast<float*>(workspace);
   a.ctr = counters;
   a.wait_cycles = sm100::kWaitCycles;

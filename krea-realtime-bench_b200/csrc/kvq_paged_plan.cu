@@ -38,15 +38,16 @@ static Item make_item(const Unit& u, int head, int64_t jb, int64_t je, int part,
 struct Plan {
   std::vector<Item> rows, tiles;
   std::vector<int32_t> cta_first;
-  int units = 0, slots = 0, tile_slots = 0, row_tile = 8;
+  int units = 0, slots = 0, tile_slots = 0, row_tile = 8, row_ctas = 0;
 };
 
-// Few rows: the work of all units is one line of blocks (an empty unit counts as
-// one), cut into equal pieces, one per resident block of the device, so every block
-// streams the same number of bytes whatever the lengths are; a piece is made of the
-// whole or partial units it meets. No piece is shorter than kMinBlocks blocks, and
-// no unit gets more than kMaxParts parts.
-constexpr int kMinBlocks = 8;
+// Few rows. With more work than the resident blocks can share in pieces of kMinBlocks
+// storage blocks, the units are one line of blocks (an empty unit counts as one), cut
+// into equal pieces, one per resident block: every block streams the same number of
+// bytes whatever the lengths are; a piece is made of the whole or partial units it meets.
+// With less, each unit is cut by itself into equal parts, so that a block has one item and
+// waits for its data once. No unit gets more than kMaxParts parts.
+constexpr int kMinBlocks = 16;
 
 static void cut_rows(const std::vector<Unit>& units, int n_heads, int64_t n_resident, Plan* p) {
   int64_t total = 0, longest = 0;
@@ -59,6 +60,21 @@ static void cut_rows(const std::vector<Unit>& units, int n_heads, int64_t n_resi
       {(total + n_resident - 1) / n_resident, kMinBlocks, (longest + kMaxParts - 2) / (kMaxParts - 1)});
   const int64_t n_ctas = (total + piece - 1) / piece;
   p->rows.reserve(units.size() * n_heads + n_ctas);
+  if (total < n_resident * kMinBlocks) {
+    for (const Unit& u : units)
+      for (int h = 0; h < n_heads; ++h) {
+        const int64_t parts = std::max<int64_t>(1, (u.n + piece - 1) / piece);
+        for (int64_t k = 0; k < parts; ++k)
+          p->rows.push_back(make_item(u, h, u.n * k / parts, u.n * (k + 1) / parts, static_cast<int>(k),
+                                      static_cast<int>(parts), p->units, p->slots));
+        if (parts > 1) {
+          ++p->units;
+          p->slots += static_cast<int>(parts);
+        }
+      }
+    p->row_ctas = static_cast<int>(p->rows.size());
+    return;
+  }
   p->cta_first.push_back(0);
   int64_t at = 0;  // position on the line
   for (const Unit& u : units) {
@@ -81,6 +97,7 @@ static void cut_rows(const std::vector<Unit>& units, int n_heads, int64_t n_resi
   }
   while (static_cast<int64_t>(p->cta_first.size()) <= n_ctas)
     p->cta_first.push_back(static_cast<int32_t>(p->rows.size()));
+  p->row_ctas = static_cast<int>(n_ctas);
 }
 
 // Many rows: one CTA per item and SM, started in the order of the list, long units first.
@@ -221,7 +238,7 @@ extern "C" int kvq_paged_plan(const kvq_paged_cache* cache, const int32_t* kv_le
     if (rc) return rc;
     *info = kvq_paged_plan_info{};
     info->n_row_items = static_cast<int32_t>(p.rows.size());
-    info->n_row_ctas = p.cta_first.empty() ? 0 : static_cast<int32_t>(p.cta_first.size()) - 1;
+    info->n_row_ctas = p.row_ctas;
     info->n_tile_items = static_cast<int32_t>(p.tiles.size());
     info->row_tile = p.row_tile;
     info->n_units = p.units;

@@ -123,7 +123,9 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
   pdl_wait();
   pdl_launch_dependents();
   uint32_t step = 0;  // blocks this warp has consumed, over all pieces: stage and phase
-  const int i0 = __ldg(a.cta_first + blockIdx.x), i1 = __ldg(a.cta_first + blockIdx.x + 1);
+  // one item per block: no list of first items
+  const int i0 = a.cta_first ? __ldg(a.cta_first + blockIdx.x) : static_cast<int>(blockIdx.x);
+  const int i1 = a.cta_first ? __ldg(a.cta_first + blockIdx.x + 1) : i0 + 1;
   for (int ii = i0; ii < i1; ++ii) {
     const Item it = a.items[ii];
     // this warp's pairs of list entries: 2 (warp + kWarps k) and the next
@@ -150,10 +152,9 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
       if (lane < (two ? 4 : 2))
         bulk_load(copy_dst + st * GEO::kStage, copy_src + static_cast<uint64_t>(b) * copy_bytes, copy_bytes, &bars[st]);
     };
-    if (n_mine > 0) issue(0);
-
-    // q fragments: rows 8 nt + g, channels (32t + 8i + 2h + {0, 4}) and the next two
-    uint32_t qf[NT][8][2];
+    // q fragments: rows 8 nt + g, channels (32t + 8i + 2h + {0, 4}) and the next two; the
+    // loads are under way while the first copies are looked up
+    uint4 qv[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int n = 8 * nt + g;
@@ -162,15 +163,21 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
       const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(it.q_first + i) * a.q_stride +
                                                         (it.head * a.group + row - i * a.group) * D + 32 * t);
 #pragma unroll
+      for (int w = 0; w < 4; ++w) qv[nt][w] = ld_global_nc_v4(src + w);
+    }
+    if (n_mine > 0) issue(0);
+    uint32_t qf[NT][8][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
       for (int w = 0; w < 4; ++w) {
-        uint4 v = ld_global_nc_v4(src + w);
-        if (n >= it.n_rows) v = make_uint4(0, 0, 0, 0);
+        const uint4 v = 8 * nt + g < it.n_rows ? qv[nt][w] : make_uint4(0, 0, 0, 0);
         qf[nt][2 * w][0] = __byte_perm(v.x, v.z, 0x5410);
         qf[nt][2 * w][1] = __byte_perm(v.x, v.z, 0x7632);
         qf[nt][2 * w + 1][0] = __byte_perm(v.y, v.w, 0x5410);
         qf[nt][2 * w + 1][1] = __byte_perm(v.y, v.w, 0x7632);
       }
-    }
+
     // what the rows 8 nt + 2t, + 2t + 1 see, and what all rows of the item see
     Seen see[NT][2];
 #pragma unroll
@@ -412,35 +419,39 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
     }
     __syncthreads();
     float* slot = it.parts > 1 ? a.ws + static_cast<int64_t>(it.slot + it.part) * slot_floats(kRows) : nullptr;
-    auto finish = [&](int n, int c, float acc, float mm, float total) {
+    // Rows are dealt to the warps, lane i has channels 4i..4i+3.
+    auto finish = [&](int n, float4 acc, float mm, float total) {
       const int row = it.row0 + n, i = row / a.group;
       const int64_t tok = it.q_first + i;
       const int h = it.head * a.group + row - i * a.group;
-      a.out[tok * a.out_stride + h * D + c] = f32_to_bf16_bits(total == 0.0f ? 0.0f : acc / total);
-      if (a.lse && c == 0)
+      const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+      *reinterpret_cast<uint2*>(a.out + tok * a.out_stride + h * D + 4 * lane) =
+          make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+      if (a.lse && lane == 0)
         a.lse[tok * a.n_q_heads + h] = total == 0.0f ? -INFINITY : 0.69314718055994531f * (mm + log2f(total));
     };
-    for (int n = 0; n < it.n_rows; ++n) {
-      float mw[kWarps], mm = -1.0e30f, total = 0.0f, acc = 0.0f;
+    auto add = [](float4& acc, float f, const float4& v) {
+      acc = make_float4(fmaf(f, v.x, acc.x), fmaf(f, v.y, acc.y), fmaf(f, v.z, acc.z), fmaf(f, v.w, acc.w));
+    };
+    for (int n = warp; n < it.n_rows; n += kWarps) {
+      float mw[kWarps], mm = -1.0e30f, total = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         mw[w] = sm_ml[(w * kRows + n) * 2];
         mm = fmaxf(mm, mw[w]);
       }
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float f = ex2f(mw[w] - mm);
         total += f * sm_ml[(w * kRows + n) * 2 + 1];
-        acc += f * reinterpret_cast<const float*>(smem + w * GEO::kRing)[n * D + tid];
+        add(acc, f, reinterpret_cast<const float4*>(smem + w * GEO::kRing + n * D * 4)[lane]);
       }
       if (slot) {
-        slot[n * D + tid] = acc;
-        if (tid == 0) {
-          slot[kRows * D + 2 * n] = mm;
-          slot[kRows * D + 2 * n + 1] = total;
-        }
+        reinterpret_cast<float4*>(slot + n * D)[lane] = acc;
+        if (lane == 0) reinterpret_cast<float2*>(slot + kRows * D)[n] = make_float2(mm, total);
       } else {
-        finish(n, tid, acc, mm, total);
+        finish(n, acc, mm, total);
       }
     }
     if (slot) {
@@ -453,68 +464,40 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
       }
       __syncthreads();
       if (*last) {
-        // Every part's (m, l) first, then its weight 2^(m_p - m), then the rows: a warp takes
-        // every fourth part, eight rows at a time, so that many loads are in flight.
+        // All parts are in the workspace: join them in part order, kAtOnce parts of a row in
+        // flight per warp, with the online rescaling between those groups.
         __threadfence();
+        constexpr int kAtOnce = 16;
         const float* base = a.ws + static_cast<int64_t>(it.slot) * slot_floats(kRows);
-        float* sm_f = reinterpret_cast<float*>(smem);                     // [part][row] m, then the weight
-        float* sm_l = sm_f + it.parts * kRows;                            // [part][row]
-        float* sm_o = reinterpret_cast<float*>(smem) + 2 * kMaxParts * kRows;  // [warp][8][D]
-        static_assert((2 * kMaxParts * kRows + kWarps * 8 * D) * 4 <= kWarps * GEO::kRing, "the join fits the rings");
-        for (int i = tid; i < it.parts * kRows; i += kRowThreads) {
-          const int q = i / kRows, n = i - q * kRows;
-          if (n < it.n_rows) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(base + static_cast<int64_t>(q) * slot_floats(kRows) +
-                                                                     kRows * D) + n);
-            sm_f[i] = ml.x;
-            sm_l[i] = ml.y;
-          }
-        }
-        __syncthreads();
         for (int n = warp; n < it.n_rows; n += kWarps) {
           float mm = -1.0e30f, total = 0.0f;
-          for (int q = lane; q < it.parts; q += 32) mm = fmaxf(mm, sm_f[q * kRows + n]);
+          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int p0 = 0; p0 < it.parts; p0 += kAtOnce) {
+            const float* sp = base + static_cast<int64_t>(p0) * slot_floats(kRows);
+            const int np = it.parts - p0;
+            float2 ml = make_float2(-1.0e30f, 0.0f);
+            if (lane < min(np, kAtOnce))
+              ml = __ldcg(reinterpret_cast<const float2*>(sp + lane * slot_floats(kRows) + kRows * D) + n);
+            float4 v[kAtOnce];
 #pragma unroll
-          for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-          for (int q = lane; q < it.parts; q += 32) {
-            const float f = ex2f(sm_f[q * kRows + n] - mm);
-            sm_f[q * kRows + n] = f;
-            total += f * sm_l[q * kRows + n];
+            for (int q = 0; q < kAtOnce; ++q)
+              v[q] = q < np ? __ldcg(reinterpret_cast<const float4*>(sp + q * slot_floats(kRows) + n * D) + lane)
+                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float top = fmaxf(ml.x, mm);
+#pragma unroll
+            for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            top = __shfl_sync(0xffffffffu, top, 0);  // lanes 0-15 hold the parts
+            const float f0 = ex2f(mm - top), f = ex2f(ml.x - top);
+            float sum = f * ml.y;
+#pragma unroll
+            for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            total = total * f0 + __shfl_sync(0xffffffffu, sum, 0);
+            acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
+#pragma unroll
+            for (int q = 0; q < kAtOnce; ++q) add(acc, __shfl_sync(0xffffffffu, f, q), v[q]);
+            mm = top;
           }
-#pragma unroll
-          for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-          if (lane == 0) {
-            sm_ml[2 * n] = mm;
-            sm_ml[2 * n + 1] = total;
-          }
-        }
-        __syncthreads();
-        for (int n0 = 0; n0 < it.n_rows; n0 += 8) {
-          float4 acc[8];
-#pragma unroll
-          for (int r = 0; r < 8; ++r) acc[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 2
-          for (int q = warp; q < it.parts; q += kWarps) {
-            const float4* src = reinterpret_cast<const float4*>(base + static_cast<int64_t>(q) * slot_floats(kRows) + n0 * D);
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-              if (n0 + r < it.n_rows) {
-                const float f = sm_f[q * kRows + n0 + r];
-                const float4 v = __ldcg(src + r * (D / 4) + lane);
-                acc[r] = make_float4(fmaf(f, v.x, acc[r].x), fmaf(f, v.y, acc[r].y), fmaf(f, v.z, acc[r].z),
-                                     fmaf(f, v.w, acc[r].w));
-              }
-          }
-#pragma unroll
-          for (int r = 0; r < 8; ++r) reinterpret_cast<float4*>(sm_o + (warp * 8 + r) * D)[lane] = acc[r];
-          __syncthreads();
-          for (int r = 0; r < 8 && n0 + r < it.n_rows; ++r) {
-            float x = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) x += sm_o[(w * 8 + r) * D + tid];
-            finish(n0 + r, tid, x, sm_ml[2 * (n0 + r)], sm_ml[2 * (n0 + r) + 1]);
-          }
-          __syncthreads();
+          finish(n, acc, mm, total);
         }
       }
     }
