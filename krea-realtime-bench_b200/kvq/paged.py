@@ -30,16 +30,19 @@ PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIM = 128
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream of a device, as an integer
+# the current stream of a device as an integer, and the current device: what the public
+# calls return, without making a Stream object at every launch
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
-def _call(device: torch.device, fn, what: str, *args) -> None:
-    """One C call on `device`, with its current stream as the last argument."""
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, _raw_stream(device.index))
+def _launch(index: int, raw: int, fn, what: str, *args) -> None:
+    """One C call on device `index` and its stream `raw`."""
+    if _current_device() == index:
+        rc = fn(*args, raw)
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(device.index))
+        with torch.cuda.device(index):
+            rc = fn(*args, raw)
     if rc:
         _lib.check(rc, what)
 
@@ -139,12 +142,14 @@ class PagedBatch:
         base = self._dev.data.data_ptr()
         self._args = _lib.PagedBatchArgs(base + seqs.size * 4, rows.shape[1], base, self.n_new, self.n_tokens,
                                          self.n_new_blocks, self.n_blocks, self.n_seqs, 0)
-        self._c = ctypes.byref(self._args)
+        self._ref = ctypes.byref(self._args)
 
-    def _ref(self):
-        """The C arguments, safe to read on the current stream."""
-        self._dev.use()
-        return self._c
+    def _use(self) -> int:
+        """The current stream, on which the uploaded arguments are now safe to read."""
+        raw = _raw_stream(self.device.index)
+        if raw != self._dev.stream:
+            self._dev.use()
+        return raw
 
 
 class _Uploaded:
@@ -157,20 +162,17 @@ class _Uploaded:
         if flat.size:
             self.data[:flat.size].copy_(torch.from_numpy(flat).pin_memory(), non_blocking=True)
         self._event = torch.cuda.Event()
-        self._stream = _raw_stream(device.index)
+        self.stream = _raw_stream(device.index)
         self._event.record(torch.cuda.current_stream(device))
 
-    def use(self) -> int:
-        """Makes the data safe to read on the current stream, which it returns: another
-        stream than the one that uploaded it waits for the upload, and the allocator is
-        told of it. A capture begins with a synchronization, so an upload before it has
-        completed."""
-        raw = _raw_stream(self.data.device.index)
-        if raw != self._stream and not torch.cuda.is_current_stream_capturing():
+    def use(self) -> None:
+        """Makes the data safe to read on the current stream, another one than that which
+        uploaded it: waits for the upload, and tells the allocator. A capture begins
+        with a synchronization, so an upload before it has completed."""
+        if not torch.cuda.is_current_stream_capturing():
             stream = torch.cuda.current_stream(self.data.device)
             stream.wait_event(self._event)
             self.data.record_stream(stream)
-        return raw
 
 
 class _Plan:
@@ -184,7 +186,7 @@ class _Plan:
         lib = _lib.load()
         words = np.empty(1 << 15, dtype=np.int32)
         for _ in range(2):  # again with more room where the plan is longer
-            rc = lib.kvq_paged_plan(cache._ref(), kv.ctypes.data, ql.ctypes.data, len(kv), n_q_heads, causal, window, sink,
+            rc = lib.kvq_paged_plan(cache._ref, kv.ctypes.data, ql.ctypes.data, len(kv), n_q_heads, causal, window, sink,
                                     sms, words.ctypes.data, words.size, ctypes.byref(self.info))
             if self.info.words <= words.size:
                 break
@@ -192,19 +194,22 @@ class _Plan:
         _lib.check(rc, "kvq_paged_plan")
         self.device = batch.device
         self.items = _Uploaded(words[:self.info.words], batch.device)
-        self._work = {}
+        self._work, self._keep = {}, []
 
-    def args(self):
-        raw = self.items.use()
+    def args(self, raw: int):
+        """(info, plan, workspace, counters) for a launch on the current stream, raw."""
         got = self._work.get(raw)
         if got is None:
             n, c = self.info.workspace_bytes, self.info.n_units
             # counters count up to a unit's parts and are set back by the last one
             ws = torch.empty(max(n, 1), dtype=torch.uint8, device=self.device)
             counters = torch.zeros(max(c, 1), dtype=torch.int32, device=self.device)
+            self._keep.append((ws, counters))
             got = self._work[raw] = (ctypes.byref(self.info), self.items.data.data_ptr(), ws.data_ptr(),
-                                     counters.data_ptr(), ws, counters)
-        return got[:4]
+                                     counters.data_ptr())
+        if raw != self.items.stream:
+            self.items.use()
+        return got
 
 
 class PagedKVCache:
@@ -234,12 +239,13 @@ class PagedKVCache:
         self.bands = _band_edges(head_dim, group_mode)
         self._map = np.ascontiguousarray(_kern.host_chan_band(_kern.build_chan_band(self.bands, head_dim, "cpu")),
                                          dtype=np.int32)
-        self.k_pages, self.v_pages = (
+        self._k_pages, self._v_pages = (
             torch.zeros((n_pages, n_heads, page_size // BLOCK, BLOCK * self._row_bytes(b)), dtype=torch.uint8,
                         device=dev) for b in (k_bits, v_bits))
-        self._c = _lib.PagedCacheArgs(None, None, self.n_pages, self.page_size, self.n_heads, self.head_dim, self.k_bits,
-                                      self.v_bits, len(self.bands), self._map.ctypes.data)
-        self._c_ref = ctypes.byref(self._c)
+        self._c = _lib.PagedCacheArgs(self._k_pages.data_ptr(), self._v_pages.data_ptr(), self.n_pages, self.page_size,
+                                      self.n_heads, self.head_dim, self.k_bits, self.v_bits, len(self.bands),
+                                      self._map.ctypes.data)
+        self._ref = ctypes.byref(self._c)
         self._format = (self.n_heads, self.k_bits, self.v_bits, group_mode)
 
     def _row_bytes(self, bits: int) -> int:
@@ -254,6 +260,9 @@ class PagedKVCache:
     def _scales(self, pages, bits):
         return pages[..., BLOCK * self._code_bytes(bits):].view(torch.bfloat16).unflatten(-1, (BLOCK, len(self.bands)))
 
+    # written in place by append and by whoever loads saved pages; never rebound
+    k_pages = property(lambda self: self._k_pages)
+    v_pages = property(lambda self: self._v_pages)
     # [n_pages, n_heads, page_size / 16, 16, code bytes or groups]
     k_codes = property(lambda self: self._codes(self.k_pages, self.k_bits))
     v_codes = property(lambda self: self._codes(self.v_pages, self.v_bits))
@@ -261,12 +270,7 @@ class PagedKVCache:
     v_scales = property(lambda self: self._scales(self.v_pages, self.v_bits))
 
     def storage_bytes(self) -> int:
-        return self.k_pages.numel() + self.v_pages.numel()
-
-    def _ref(self):
-        c = self._c
-        c.k_pages, c.v_pages = self.k_pages.data_ptr(), self.v_pages.data_ptr()
-        return self._c_ref
+        return self._k_pages.numel() + self._v_pages.numel()
 
     def _check(self, batch: PagedBatch) -> None:
         if not isinstance(batch, PagedBatch):
@@ -286,9 +290,10 @@ class PagedKVCache:
         if batch._append_error:
             raise ValueError(batch._append_error)
         shape = (batch.n_new, self.n_heads, self.head_dim)
-        k, v = _rows(k, shape, self.device, "k"), _rows(v, shape, self.device, "v")
-        _call(self.device, _lib.load().kvq_paged_append, "kvq_paged_append", k.data_ptr(), _row_stride(k), v.data_ptr(),
-              _row_stride(v), self._ref(), batch._ref())
+        k, ks = _rows(k, shape, self.device, "k")
+        v, vs = _rows(v, shape, self.device, "v")
+        _launch(self.device.index, batch._use(), _lib.load().kvq_paged_append, "kvq_paged_append", k.data_ptr(), ks,
+                v.data_ptr(), vs, self._ref, batch._ref)
 
     def read(self, batch: PagedBatch, new_only: bool = False):
         """(k, v) bf16 [n, n_heads, 128]: the values held for the sequences' tokens, or
@@ -299,9 +304,9 @@ class PagedKVCache:
         n = batch.n_new if new_only else batch.n_tokens
         shape, row = (n, self.n_heads, self.head_dim), self.n_heads * self.head_dim
         k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-        v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-        _call(self.device, _lib.load().kvq_paged_read, "kvq_paged_read", self._ref(), batch._ref(), 1 if new_only else 0,
-              k.data_ptr(), row, v.data_ptr(), row)
+        v = torch.empty_like(k)
+        _launch(self.device.index, batch._use(), _lib.load().kvq_paged_read, "kvq_paged_read", self._ref, batch._ref,
+                1 if new_only else 0, k.data_ptr(), row, v.data_ptr(), row)
         return k, v
 
     def __repr__(self):
@@ -310,26 +315,23 @@ class PagedKVCache:
                 f"{self.storage_bytes() / 2**30:.2f} GiB resident>")
 
 
-def _rows(t, shape, device, name: str) -> torch.Tensor:
+def _rows(t, shape, device, name: str):
+    """(t, or a contiguous copy where its rows are not 16-byte aligned blocks; token stride)."""
     if not isinstance(t, torch.Tensor) or t.device != device:
         if _require_cuda(t) != device:
             raise ValueError(f"{name} is on {t.device}, the cache on {device}")
-    if t.dtype != torch.bfloat16:
+    if t.dtype is not torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    row = shape[1] * shape[2]
     if t.data_ptr() % 16 == 0:
         if t.is_contiguous():
-            return t
+            return t, row
         s0, s1, s2 = t.stride()
-        row = shape[1] * shape[2]
-        if s2 == 1 and (s1 == shape[2] or shape[1] == 1) and s0 % 8 == 0 and (s0 >= row or shape[0] == 1):
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+        if s2 == 1 and (s1 == shape[2] or shape[1] == 1) and (shape[0] == 1 or (s0 % 8 == 0 and s0 >= row)):
+            return t, (row if shape[0] == 1 else s0)
+    return t.clone(memory_format=torch.contiguous_format), row
 
 
 def attention(q: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, causal: bool = True, window: int = 0,
@@ -359,15 +361,18 @@ def attention(q: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, causal: b
     scale = 0.0 if softmax_scale is None else float(softmax_scale)
     if softmax_scale is not None and not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"softmax_scale must be a positive number, got {softmax_scale}")
-    shape = torch.Size((batch.n_new, heads, cache.head_dim))
-    q = _rows(q, shape, cache.device, "q")
+    shape, device = (batch.n_new, heads, cache.head_dim), cache.device
+    q, qs = _rows(q, shape, device, "q")
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
-    elif _rows(out, shape, cache.device, "out") is not out:
-        raise ValueError("out must have contiguous [heads, channels] blocks, 16-byte aligned rows")
-    lse = torch.empty(shape[:2], dtype=torch.float32, device=cache.device) if return_lse else None
+        out, os_ = torch.empty(shape, dtype=torch.bfloat16, device=device), heads * cache.head_dim
+    else:
+        rows, os_ = _rows(out, shape, device, "out")
+        if rows is not out:
+            raise ValueError("out must have contiguous [heads, channels] blocks, 16-byte aligned rows")
+    lse = torch.empty(shape[:2], dtype=torch.float32, device=device) if return_lse else None
     plan = batch._plan(cache, heads, bool(causal), window, sink)
-    _call(cache.device, _lib.load().kvq_paged_attention, "kvq_paged_attention", q.data_ptr(), _row_stride(q), cache._ref(),
-          batch._ref(), out.data_ptr(), _row_stride(out), lse.data_ptr() if return_lse else None, heads,
-          1 if causal else 0, window, sink, scale, *plan.args())
+    raw = batch._use()
+    _launch(device.index, raw, _lib.load().kvq_paged_attention, "kvq_paged_attention", q.data_ptr(), qs, cache._ref,
+            batch._ref, out.data_ptr(), os_, lse.data_ptr() if return_lse else None, heads, 1 if causal else 0, window, sink,
+            scale, *plan.args(raw))
     return (out, lse) if return_lse else out
