@@ -4,7 +4,9 @@
 // Append. Per (token, head) row x and channel group g: s_g = max_g |x| / qmax (1
 // where that is 0), code = rne(x / s_g) + offset, stored scale bf16(s_g): the
 // arithmetic of kvq_quantize, bit for bit, with rows going to pages.
-#include "kvq_paged.cuh"
+#include <algorithm>
+
+#include "kvq_paged_dev.cuh"
 #include "kvq_quant.cuh"
 
 namespace kvq {
@@ -67,88 +69,142 @@ struct AppendArgs {
   uint8_t* pages[2];
 };
 
+constexpr int kHeadsPerCta = 8;                      // heads of one tile
+constexpr int kTileRowsA = kBlock * kHeadsPerCta;    // rows of one tile, a thread each
+
+// 16-byte chunk c of row r in the staged input and in the staged codes: the XOR spreads
+// the threads' equal chunks of consecutive rows over the banks.
+__device__ __forceinline__ int in_slot(int r, int c) { return r * 16 + (c ^ (r & 7)); }
+template <int BITS>
+__device__ __forceinline__ int code_slot(int r, int c) {
+  return BITS == 4 ? r * 4 + (c ^ ((r >> 1) & 3)) : r * 8 + (c ^ (r & 7));
+}
+
 // Rare path: the groups flagged in slow_mask (amax below 2^-100, above 3e38 or not
 // finite) with the IEEE divide; NaN counts as 0, magnitudes above 3e38 as 3e38.
 template <class L, int BITS>
-__device__ __noinline__ void fix_slow(const uint16_t* x, uint32_t slow_mask, uint8_t* codes, uint16_t* scales) {
+__device__ __noinline__ void fix_slow(const uint4* tin, int r, uint32_t slow_mask, uint4* sm_codes, uint16_t* scales) {
   using C = QuantConsts<BITS>;
   constexpr float q = static_cast<float>(C::kQmax), top = 3.0e38f;
   int edges[L::G + 1];
   fill_edges<L>(edges, std::make_integer_sequence<int, L::G + 1>{});
+  auto value = [&](int c) {
+    const float v = bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(tin + in_slot(r, c >> 3))[c & 7]);
+    return v == v ? v : 0.0f;
+  };
   for (int g = 0; slow_mask; ++g, slow_mask >>= 1) {
     if (!(slow_mask & 1u)) continue;
     float amax = 0.0f;
-    for (int c = edges[g]; c < edges[g + 1]; ++c) {
-      const float v = fabsf(bf16_bits_to_f32(x[c]));
-      amax = fmaxf(amax, v == v ? fminf(v, top) : 0.0f);
-    }
+    for (int c = edges[g]; c < edges[g + 1]; ++c) amax = fmaxf(amax, fminf(fabsf(value(c)), top));
     float s = __fdiv_rn(amax, q);
     s = s > 0.0f ? s : 1.0f;
     scales[g] = f32_to_bf16_bits(s);
     for (int c = edges[g]; c < edges[g + 1]; ++c) {
-      float v = bf16_bits_to_f32(x[c]);
-      v = v == v ? v : 0.0f;
-      const uint32_t code = code_exact(v, s, q, C::kMagic) & 0xFFu;
-      if constexpr (BITS == 4) {
-        uint8_t& o = codes[c >> 1];
+      const uint32_t code = code_exact(value(c), s, q, C::kMagic) & 0xFFu;
+      const int b = BITS == 4 ? c >> 1 : c;
+      uint8_t& o = reinterpret_cast<uint8_t*>(sm_codes + code_slot<BITS>(r, b >> 4))[b & 15];
+      if constexpr (BITS == 4)
         o = (c & 1) ? static_cast<uint8_t>((o & 0x0F) | (code << 4)) : static_cast<uint8_t>((o & 0xF0) | code);
-      } else {
-        codes[c] = static_cast<uint8_t>(code);
-      }
+      else
+        o = static_cast<uint8_t>(code);
     }
   }
 }
 
-// One thread per row: 16 tokens of a storage block x 8 heads per CTA.
+// Bound by memory at many tokens, by latency at few. One CTA per tile of 16 tokens
+// (one storage block) x 8 heads of K or V: the rows arrive by cp.async (a token's heads
+// are contiguous: 2 KB runs), thread r quantizes row r = 16 head + token, and each head's
+// record, contiguous in its page, is written with 16-byte stores; a block that the step
+// fills partly is written row by row. Several CTAs per SM overlap the three phases.
 template <class L, int BITS>
-__device__ __forceinline__ void append_row(const AppendArgs& a, int which, int s, int blk, int row, int h, int tok) {
+__device__ __forceinline__ void append_tile(const AppendArgs& a, int which, int s, int blk, int row0, int n_tok, int tok0,
+                                            uint8_t* smem) {
   using R = Rec<L, BITS>;
-  const uint16_t* x = a.x[which] + tok * a.stride[which] + h * D;
-  uint32_t w[64];
-#pragma unroll
-  for (int c = 0; c < 16; ++c) {
-    const uint4 v = ld_global_nc_v4(x + 8 * c);
-    w[4 * c] = v.x;
-    w[4 * c + 1] = v.y;
-    w[4 * c + 2] = v.z;
-    w[4 * c + 3] = v.w;
+  constexpr int CCH = R::CW / 16;  // code chunks per row
+  uint4* tin = reinterpret_cast<uint4*>(smem);
+  uint4* sm_codes = tin + kTileRowsA * 16;
+  uint16_t* sm_sc = reinterpret_cast<uint16_t*>(sm_codes + kTileRowsA * CCH);
+  const int tid = threadIdx.x;
+  const int h0 = blockIdx.y * kHeadsPerCta, nh = min(kHeadsPerCta, a.p.n_heads - h0);
+  // tokens row0 .. row0 + n_tok of the block; copies in the order of memory
+  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(tin));
+  for (int i = tid; i < n_tok * nh * 16; i += kTileRowsA) {
+    const int c = i & 15, j = i >> 4, t = j / nh, h = j - t * nh, r = h * kBlock + row0 + t;
+    const uint16_t* src = a.x[which] + static_cast<int64_t>(tok0 + t) * a.stride[which] + (h0 + h) * D + 8 * c;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + in_slot(r, c) * 16), "l"(src) : "memory");
   }
-  uint32_t ow[BITS == 4 ? 16 : 32];
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  const int t = tid & (kBlock - 1), h = tid >> 4;
+  if (h < nh && t >= row0 && t < row0 + n_tok) {
+    uint32_t w[64];
 #pragma unroll
-  for (int i = 0; i < (BITS == 4 ? 16 : 32); ++i) ow[i] = 0;
-  uint16_t sc[L::G];
-  uint32_t slow = 0;
-  quant_row<L, BITS>(w, ow, sc, slow, std::make_integer_sequence<int, L::G>{});
+    for (int c = 0; c < 16; ++c) {
+      const uint4 v = tin[in_slot(tid, c)];
+      w[4 * c] = v.x;
+      w[4 * c + 1] = v.y;
+      w[4 * c + 2] = v.z;
+      w[4 * c + 3] = v.w;
+    }
+    uint32_t ow[BITS == 4 ? 16 : 32];
+#pragma unroll
+    for (int i = 0; i < (BITS == 4 ? 16 : 32); ++i) ow[i] = 0;
+    uint16_t sc[L::G];
+    uint32_t slow = 0;
+    quant_row<L, BITS>(w, ow, sc, slow, std::make_integer_sequence<int, L::G>{});
+#pragma unroll
+    for (int c = 0; c < CCH; ++c)
+      sm_codes[code_slot<BITS>(tid, c)] = make_uint4(ow[4 * c], ow[4 * c + 1], ow[4 * c + 2], ow[4 * c + 3]);
+#pragma unroll
+    for (int g = 0; g < L::G; ++g) sm_sc[tid * L::G + g] = sc[g];
+    if (slow) fix_slow<L, BITS>(tin, tid, slow, sm_codes, sm_sc + tid * L::G);
+  }
+  __syncthreads();
   bool ok;
-  uint8_t* rec = a.pages[which] + a.p.block(s, h, blk, ok) * R::kBytes;
+  const int64_t rec = a.p.block(s, h0, blk, ok);  // the next head's record is (1 << page_shift) records on
   if (!ok) return;
-  uint8_t* codes = rec + row * R::CW;
-  uint16_t* scales = reinterpret_cast<uint16_t*>(rec + R::kCodes) + row * L::G;
-#pragma unroll
-  for (int i = 0; i < R::CW / 16; ++i)
-    st_global_v4(codes + 16 * i, make_uint4(ow[4 * i], ow[4 * i + 1], ow[4 * i + 2], ow[4 * i + 3]));
-#pragma unroll
-  for (int g = 0; g < L::G; ++g) scales[g] = sc[g];
-  if (slow) fix_slow<L, BITS>(x, slow, codes, scales);
+  uint8_t* out = a.pages[which] + rec * R::kBytes;
+  const int64_t head_bytes = static_cast<int64_t>(R::kBytes) << a.p.page_shift;
+  for (int i = tid; i < n_tok * nh * CCH; i += kTileRowsA) {
+    const int hh = i / (n_tok * CCH), k = i - hh * (n_tok * CCH), r = row0 + k / CCH, c = k % CCH;
+    st_global_v4(out + hh * head_bytes + r * R::CW + 16 * c, sm_codes[code_slot<BITS>(hh * kBlock + r, c)]);
+  }
+  if (n_tok == kBlock) {
+    constexpr int SCH = 2 * L::G;  // 16-byte chunks of a block's scales
+    for (int i = tid; i < nh * SCH; i += kTileRowsA) {
+      const int hh = i / SCH, c = i - hh * SCH;
+      st_global_v4(out + hh * head_bytes + R::kCodes + 16 * c, reinterpret_cast<const uint4*>(sm_sc + hh * kBlock * L::G)[c]);
+    }
+  } else {
+    for (int i = tid; i < n_tok * nh * L::G; i += kTileRowsA) {
+      const int hh = i / (n_tok * L::G), k = i - hh * (n_tok * L::G);
+      reinterpret_cast<uint16_t*>(out + hh * head_bytes + R::kCodes)[row0 * L::G + k] =
+          sm_sc[(hh * kBlock + row0) * L::G + k];
+    }
+  }
+}
+
+template <class L, int BITS>
+constexpr int append_smem() {
+  return kTileRowsA * (256 + Rec<L, BITS>::CW + 2 * L::G);
 }
 
 template <class L, int KB, int VB>
-__global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kTileRowsA, 3) append_kernel(const __grid_constant__ AppendArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
   pdl_wait();
   pdl_launch_dependents();
-  const int h = blockIdx.y * 8 + (threadIdx.x >> 4);
   const int s = find_seq<true>(a.p, blockIdx.x);
   const kvq_paged_seq q = a.p.seqs[s];
   const int start = q.kv_len - q.q_len;
-  const int blk = start / kBlock + (static_cast<int>(blockIdx.x) - q.q_block);
-  const int row = threadIdx.x & (kBlock - 1);
-  const int pos = blk * kBlock + row;
-  if (h >= a.p.n_heads || pos < start || pos >= q.kv_len) return;
-  const int tok = q.q_first + pos - start;
+  const int blk = max(start, 0) / kBlock + (static_cast<int>(blockIdx.x) - q.q_block);
+  const int row0 = max(start - blk * kBlock, 0), n_tok = min(kBlock, q.kv_len - blk * kBlock) - row0;
+  if (n_tok <= 0) return;
+  const int tok0 = q.q_first + blk * kBlock + row0 - start;
   if (blockIdx.z == 0)
-    append_row<L, KB>(a, 0, s, blk, row, h, tok);
+    append_tile<L, KB>(a, 0, s, blk, row0, n_tok, tok0, smem);
   else
-    append_row<L, VB>(a, 1, s, blk, row, h, tok);
+    append_tile<L, VB>(a, 1, s, blk, row0, n_tok, tok0, smem);
 }
 
 // ---------------------------------------------------------------- read
@@ -159,34 +215,63 @@ struct ReadArgs {
   int64_t stride[2];
 };
 
-// 16 lanes per row, 8 channels each.
+// Bound by memory: one CTA per storage block, K and V of all heads, 16 lanes per row and
+// eight channels per lane, so a warp reads contiguous codes and writes 256-byte rows.
+// kHeadsAtOnce heads are loaded before the first is converted. An aligned run of eight
+// channels meets at most two groups.
+constexpr int kHeadsAtOnce = 4;
+
 template <class L, int BITS>
-__device__ __forceinline__ void read_row(const ReadArgs& a, int which, const uint8_t* rec, int row, int h, int tok) {
+__device__ __forceinline__ void read_block(const ReadArgs& a, int which, int64_t rec, int row, bool live, int64_t tok) {
   using R = Rec<L, BITS>;
   const int lane = threadIdx.x & 15;
-  const uint16_t* scales = reinterpret_cast<const uint16_t*>(rec + R::kCodes) + row * L::G;
-  uint32_t o[4];
-  uint2 w;
-  if constexpr (BITS == 4) {
-    w.x = __ldg(reinterpret_cast<const uint32_t*>(rec + row * R::CW) + lane);
-  } else {
-    w = __ldg(reinterpret_cast<const uint2*>(rec + row * R::CW) + lane);
-  }
+  const int ga = group_at<L>(8 * lane), gb = group_at<L>(8 * lane + 7);
+  int split = 4;  // first channel pair of the second group
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float s = bf16_bits_to_f32(__ldg(scales + group_at<L>(8 * lane + 2 * i)));
-    float lo, hi;
-    if constexpr (BITS == 4) {
-      lo = static_cast<float>(static_cast<int>((w.x >> (8 * i)) & 15u) - 8);
-      hi = static_cast<float>(static_cast<int>((w.x >> (8 * i + 4)) & 15u) - 8);
-    } else {
-      const uint32_t v = (i < 2 ? w.x : w.y) >> (16 * (i & 1));
-      lo = static_cast<float>(static_cast<int>(v & 255u) - 128);
-      hi = static_cast<float>(static_cast<int>((v >> 8) & 255u) - 128);
+  for (int i = 3; i > 0; --i)
+    if (group_at<L>(8 * lane + 2 * i) != ga) split = i;
+  const uint8_t* src = a.pages[which] + rec * R::kBytes + row * R::CW + lane * (BITS);
+  const uint8_t* sc = a.pages[which] + rec * R::kBytes + R::kCodes + row * L::G * 2;
+  const int64_t head_bytes = static_cast<int64_t>(R::kBytes) << a.p.page_shift;
+  uint16_t* dst = a.out[which] + tok * a.stride[which] + 8 * lane;
+  for (int h0 = 0; h0 < a.p.n_heads; h0 += kHeadsAtOnce) {
+    uint2 w[kHeadsAtOnce];
+    uint32_t sa[kHeadsAtOnce], sb[kHeadsAtOnce];
+#pragma unroll
+    for (int i = 0; i < kHeadsAtOnce; ++i) {
+      if (h0 + i < a.p.n_heads && live) {
+        const uint8_t* q = src + (h0 + i) * head_bytes;
+        if constexpr (BITS == 4)
+          w[i].x = __ldg(reinterpret_cast<const uint32_t*>(q));
+        else
+          w[i] = __ldg(reinterpret_cast<const uint2*>(q));
+        const uint16_t* s = reinterpret_cast<const uint16_t*>(sc + (h0 + i) * head_bytes);
+        sa[i] = __ldg(s + ga);
+        sb[i] = __ldg(s + gb);
+      }
     }
-    o[i] = pack_bf16x2(lo * s, hi * s);
+#pragma unroll
+    for (int i = 0; i < kHeadsAtOnce; ++i) {
+      if (h0 + i < a.p.n_heads && live) {
+        uint32_t o[4];
+        uint32_t pa = sa[i] * 0x10001u, pb = sb[i] * 0x10001u;
+        if constexpr (BITS == 4) {
+          pa = hmul2(pa, kFour);
+          pb = hmul2(pb, kFour);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t v;
+          if constexpr (BITS == 4)
+            v = int4_low(__byte_perm(w[i].x, w[i].x >> 4, (4 + j) << 8 | j));
+          else
+            v = int8_pair(__byte_perm(j < 2 ? w[i].x : w[i].y, 0, (j & 1) ? 0x4342 : 0x4140));
+          o[j] = hmul2(v, j >= split ? pb : pa);
+        }
+        st_global_v4(dst + (h0 + i) * D, make_uint4(o[0], o[1], o[2], o[3]));
+      }
+    }
   }
-  st_global_v4(a.out[which] + tok * a.stride[which] + h * D + 8 * lane, make_uint4(o[0], o[1], o[2], o[3]));
 }
 
 template <class L, int KB, int VB, bool NEW>
@@ -196,18 +281,18 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadA
   const int s = find_seq<NEW>(a.p, blockIdx.x);
   const kvq_paged_seq q = a.p.seqs[s];
   const int start = NEW ? q.kv_len - q.q_len : 0;
-  const int blk = start / kBlock + (static_cast<int>(blockIdx.x) - (NEW ? q.q_block : q.kv_block));
+  const int blk = max(start, 0) / kBlock + (static_cast<int>(blockIdx.x) - (NEW ? q.q_block : q.kv_block));
   const int row = threadIdx.x >> 4;
   const int pos = blk * kBlock + row;
-  if (pos < start || pos >= q.kv_len) return;
-  const int tok = (NEW ? q.q_first : q.kv_first) + pos - start;
-  const int h = blockIdx.y;
+  const bool live = pos >= start && pos < q.kv_len;
+  if (blk * kBlock >= q.kv_len) return;
+  const int64_t tok = static_cast<int64_t>(NEW ? q.q_first : q.kv_first) + pos - start;
   bool ok;
-  const int64_t b = a.p.block(s, h, blk, ok);
-  if (blockIdx.z == 0)
-    read_row<L, KB>(a, 0, a.pages[0] + b * Rec<L, KB>::kBytes, row, h, tok);
+  const int64_t rec = a.p.block(s, 0, blk, ok);
+  if (blockIdx.y == 0)
+    read_block<L, KB>(a, 0, rec, row, live, tok);
   else
-    read_row<L, VB>(a, 1, a.pages[1] + b * Rec<L, VB>::kBytes, row, h, tok);
+    read_block<L, VB>(a, 1, rec, row, live, tok);
 }
 
 static int check_rows(const void* k, int64_t ks, const void* v, int64_t vs, int n_heads, const char* what) {
@@ -244,13 +329,24 @@ extern "C" int kvq_paged_append(const void* k, int64_t k_token_stride, const voi
   a.stride[1] = v_token_stride;
   a.pages[0] = static_cast<uint8_t*>(cache->k_pages);
   a.pages[1] = static_cast<uint8_t*>(cache->v_pages);
-  const dim3 grid(static_cast<unsigned>(batch->n_new_blocks), (cache->n_heads + 7) / 8, 2);
+  const dim3 grid(static_cast<unsigned>(batch->n_new_blocks), (cache->n_heads + paged::kHeadsPerCta - 1) / paged::kHeadsPerCta, 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return paged::with_layout(layout, [&](auto l) {
     using L = decltype(l);
     return paged::with_bits(cache->k_bits, cache->v_bits, [&](auto b) {
       using B = decltype(b);
-      paged::append_kernel<L, B::k, B::v><<<grid, 128, 0, st>>>(a);
+      constexpr int smem = std::max(paged::append_smem<L, B::k>(), paged::append_smem<L, B::v>());
+      static_assert(smem <= 227 * 1024, "shared memory");
+      static bool configured[64];
+      int dev = 0;
+      cudaGetDevice(&dev);
+      if (dev < 0 || dev >= 64 || !configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(paged::append_kernel<L, B::k, B::v>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        KVQ_REQUIRE(e == cudaSuccess, KVQ_ERR_CUDA, "cudaFuncSetAttribute(paged append): %s", cudaGetErrorString(e));
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+      }
+      cudaError_t e = launch_pdl(paged::append_kernel<L, B::k, B::v>, grid, paged::kTileRowsA, smem, st, a);
+      KVQ_REQUIRE(e == cudaSuccess, KVQ_ERR_CUDA, "kvq_paged_append: launch failed: %s", cudaGetErrorString(e));
       return check_launch("kvq_paged_append");
     });
   });
@@ -275,16 +371,15 @@ extern "C" int kvq_paged_read(const kvq_paged_cache* cache, const kvq_paged_batc
   a.out[1] = static_cast<uint16_t*>(v_out);
   a.stride[0] = k_out_token_stride;
   a.stride[1] = v_out_token_stride;
-  const dim3 grid(static_cast<unsigned>(new_only ? batch->n_new_blocks : batch->n_blocks), cache->n_heads, 2);
+  const dim3 grid(static_cast<unsigned>(new_only ? batch->n_new_blocks : batch->n_blocks), 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return paged::with_layout(layout, [&](auto l) {
     using L = decltype(l);
     return paged::with_bits(cache->k_bits, cache->v_bits, [&](auto b) {
       using B = decltype(b);
-      if (new_only)
-        paged::read_kernel<L, B::k, B::v, true><<<grid, 256, 0, st>>>(a);
-      else
-        paged::read_kernel<L, B::k, B::v, false><<<grid, 256, 0, st>>>(a);
+      cudaError_t e = new_only ? launch_pdl(paged::read_kernel<L, B::k, B::v, true>, grid, 256, 0, st, a)
+                               : launch_pdl(paged::read_kernel<L, B::k, B::v, false>, grid, 256, 0, st, a);
+      KVQ_REQUIRE(e == cudaSuccess, KVQ_ERR_CUDA, "kvq_paged_read: launch failed: %s", cudaGetErrorString(e));
       return check_launch("kvq_paged_read");
     });
   });
