@@ -270,11 +270,13 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     const Seen first = seen_by(a, it.start + (it.row0 + x * BM) / a.group, it.kv_len);
     const Seen fin = seen_by(a, it.start + (it.row0 + n_last) / a.group, it.kv_len);
     float m = -1.0e30f, l = 0.0f;
-    bool ok = true;
+    bool ok = true, s_ready = false;  // s_ready: S of the coming tile was already found complete
     auto step = [&](const int j, auto masked) -> bool {
       constexpr bool MASK = decltype(masked)::value;
       const uint32_t tS = tS0 + 64 * (j & 1);
-      if (!mbar_wait_warp(&bars[GEO::bSFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim)) return false;
+      if (!__all_sync(0xffffffffu, s_ready) &&
+          !mbar_wait_warp(&bars[GEO::bSFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim))
+        return false;
       // S_x(j) complete: this Q tile no longer reads K stage j, and PV_x(j-2) (issued
       // before it) is complete: nor V stage j-2
       if ((warp & 3) == 0 && lane == 0) {
@@ -356,6 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         }
         tmem_wait_st();
       }
+      s_ready = j + 1 < nkv && mbar_try_wait(smem_u32(&bars[GEO::bSFull + 2 * x + ((j + 1) & 1)]), ((j + 1) >> 1) & 1);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -481,24 +484,29 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       constexpr uint32_t idS = idesc_bf16(BM, BN, 0);
       constexpr uint32_t idPV = idesc_bf16(BM, D, 1);
       const uint32_t tS0 = tmem + kColS + 128 * x, tO = tmem + kColO + 128 * x;
-      const uint32_t qaddr = sbase + GEO::kOffQ + x * kQTile;
+      // descriptors address shared memory in units of 16 bytes
+      const uint64_t dq = smem_desc_sw128(sbase + GEO::kOffQ + x * kQTile, 16, 1024);
+      const uint64_t dk = smem_desc_sw128(sbase + GEO::kOffK, 16, 1024);
+      const uint64_t dv = smem_desc_sw128(sbase + GEO::kOffV, kAtom, 1024);
       auto issue_s = [&](int j) {
-        const uint32_t kaddr = sbase + GEO::kOffK + (j % NK) * kKVTile;
+        const uint64_t k = dk + static_cast<uint64_t>((j % NK) * (kKVTile >> 4));
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          mma_bf16_ss(tS0 + 64 * (j & 1), smem_desc_sw128(qaddr + (kk >> 2) * kQAtom + (kk & 3) * 32, 16, 1024),
-                      smem_desc_sw128(kaddr + (kk >> 2) * kAtom + (kk & 3) * 32, 16, 1024), idS, kk > 0);
+          mma_bf16_ss(tS0 + 64 * (j & 1), dq + (((kk >> 2) * kQAtom + (kk & 3) * 32) >> 4),
+                      k + (((kk >> 2) * kAtom + (kk & 3) * 32) >> 4), idS, kk > 0);
         mma_commit(&bars[GEO::bSFull + 2 * x + (j & 1)]);
       };
       auto issue_pv = [&](int j) {
-        const uint32_t vaddr = sbase + GEO::kOffV + (j % NV) * kKVTile;
+        const uint64_t v = dv + static_cast<uint64_t>((j % NV) * (kKVTile >> 4));
         const uint32_t p = tS0 + 64 * (j & 1);
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          mma_bf16_ts(tO, p + 8 * kk, smem_desc_sw128(vaddr + kk * 2048, kAtom, 1024), idPV,
-                      (j > 0 || kk > 0) ? 1u : 0u);
+          mma_bf16_ts(tO, p + 8 * kk, v + ((kk * 2048) >> 4), idPV, (j > 0 || kk > 0) ? 1u : 0u);
       };
       auto wait_k = [&](int j) { return mbar_wait(&bars[GEO::bKvFull + j % NK], (j / NK) & 1, abort, a.status, lim); };
+      auto wait_v = [&](int j) {
+        return mbar_wait(&bars[GEO::bKvFull + NK + j % NV], (j / NV) & 1, abort, a.status, lim);
+      };
       bool ok = nkv > 0 && mbar_wait(&bars[GEO::bQReady + x], 0, abort, a.status, lim) && wait_k(0);
       if (ok) {
         tc_fence_after();
@@ -508,12 +516,18 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
           issue_s(1);
         }
       }
+      // A test of a barrier takes this thread over 100 cycles even where its phase has
+      // completed, and a tile's issue is what it has time for: V(j) and K(j+2) are tested
+      // while the MMAs of tile j - 1 are still being issued, and waited for only if that failed.
+      bool v_ready = false, k_ready = false;
       for (int j = 0; j < nkv && ok; ++j) {
-        if (!(ok = mbar_wait(&bars[GEO::bKvFull + NK + j % NV], (j / NV) & 1, abort, a.status, lim))) break;
-        if (j + 2 < nkv && !(ok = wait_k(j + 2))) break;
+        if (!v_ready && !(ok = wait_v(j))) break;
+        if (j + 2 < nkv && !k_ready && !(ok = wait_k(j + 2))) break;
         if (!(ok = mbar_wait(&bars[GEO::bPFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim))) break;
         tc_fence_after();
         issue_pv(j);
+        v_ready = j + 1 < nkv && mbar_try_wait(smem_u32(&bars[GEO::bKvFull + NK + (j + 1) % NV]), ((j + 1) / NV) & 1);
+        k_ready = j + 3 < nkv && mbar_try_wait(smem_u32(&bars[GEO::bKvFull + (j + 3) % NK]), ((j + 3) / NK) & 1);
         if (j + 2 < nkv) {
           issue_s(j + 2);
         } else if (j + 2 == nkv) {
