@@ -441,12 +441,18 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         }
       }
     };
-    if (!is_v)
-      convert(Converter<L, KB>{}, sbase + GEO::kOffCK, sbase + GEO::kOffK, LK, NK, bars + GEO::bLdFull, bars + GEO::bLdEmpty,
-              bars + GEO::bKvFull, bars + GEO::bKvEmpty, GEO::kRecK, GEO::kStageK);
+    const uint32_t codes = sbase + (is_v ? GEO::kOffCV : GEO::kOffCK), dst = sbase + (is_v ? GEO::kOffV : GEO::kOffK);
+    uint64_t* const ld_full = bars + GEO::bLdFull + (is_v ? LK : 0);
+    uint64_t* const ld_empty = bars + GEO::bLdEmpty + (is_v ? LK : 0);
+    uint64_t* const kv_full = bars + GEO::bKvFull + (is_v ? NK : 0);
+    uint64_t* const kv_empty = bars + GEO::bKvEmpty + (is_v ? NK : 0);
+    // one copy of the loop where K and V have the same format: the instruction caches
+    // hold four different loops per sub-partition as it is
+    if (KB == VB || !is_v)
+      convert(Converter<L, KB>{}, codes, dst, is_v ? LV : LK, is_v ? NV : NK, ld_full, ld_empty, kv_full, kv_empty, GEO::kRecK,
+              GEO::kStageK);
     else
-      convert(Converter<L, VB>{}, sbase + GEO::kOffCV, sbase + GEO::kOffV, LV, NV, bars + GEO::bLdFull + LK,
-              bars + GEO::bLdEmpty + LK, bars + GEO::bKvFull + NK, bars + GEO::bKvEmpty + NK, GEO::kRecV, GEO::kStageV);
+      convert(Converter<L, VB>{}, codes, dst, LV, NV, ld_full, ld_empty, kv_full, kv_empty, GEO::kRecV, GEO::kStageV);
   } else if (warp == kProdWarp || warp == kProdWarpV) {
     // ------------------------------------------------------------ producers
     const bool pv = warp != kProdWarp;
