@@ -10,6 +10,37 @@
 namespace kvq {
 namespace paged {
 
+// Waits for the phase of `parity`, as sm100::mbar_wait, but polls first: a thread that
+// try_wait suspends comes back 1000 to 2500 cycles after the phase completed, which in a
+// pipeline of 2000-cycle steps is a step; test_wait answers in about 100. A wait that
+// is still unfinished after kPolls polls goes on as the bounded, suspending one.
+constexpr int kPolls = 512;
+__device__ __forceinline__ bool mbar_test(const uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(sm100::smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool poll_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* status, long long limit) {
+#pragma unroll 1
+  for (int i = 0; i < kPolls; ++i)
+    if (mbar_test(bar, parity)) return true;
+  return sm100::mbar_wait(bar, parity, abort, status, limit);
+}
+// The same by a converged warp.
+__device__ __forceinline__ bool poll_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int* status,
+                                               long long limit) {
+#pragma unroll 1
+  for (int i = 0; i < kPolls; ++i)
+    if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+  return sm100::mbar_wait_warp(bar, parity, abort, status, limit);
+}
+
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))

@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       constexpr bool MASK = decltype(masked)::value;
       const uint32_t tS = tS0 + 64 * (j & 1);
       if (!__all_sync(0xffffffffu, s_ready) &&
-          !mbar_wait_warp(&bars[GEO::bSFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim))
+          !poll_wait_warp(&bars[GEO::bSFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim))
         return false;
       // S_x(j) complete: this Q tile no longer reads K stage j, and PV_x(j-2) (issued
       // before it) is complete: nor V stage j-2
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         // O_x must hold every product up to PV_x(j-1) before it is rescaled: wait for
         // S_x(j+1), issued behind PV_x(j-1), or at the last tile for the commit behind it
         const bool tail = j + 1 == nkv;
-        if (!mbar_wait_warp(&bars[tail ? GEO::bOReady + x : GEO::bSFull + 2 * x + ((j + 1) & 1)],
+        if (!poll_wait_warp(&bars[tail ? GEO::bOReady + x : GEO::bSFull + 2 * x + ((j + 1) & 1)],
                             tail ? 0u : static_cast<uint32_t>(((j + 1) >> 1) & 1), abort, a.status, lim))
           return false;
         tc_fence_after();
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         }
         tmem_wait_st();
       }
-      s_ready = j + 1 < nkv && mbar_try_wait(smem_u32(&bars[GEO::bSFull + 2 * x + ((j + 1) & 1)]), ((j + 1) >> 1) & 1);
+      s_ready = j + 1 < nkv && mbar_test(&bars[GEO::bSFull + 2 * x + ((j + 1) & 1)], ((j + 1) >> 1) & 1);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       const bool whole = e0 + 4 <= it.je && tz <= first.hi && (ta >= fin.lo || tz <= first.kept);
       ok = whole ? step(j, std::false_type{}) : step(j, std::true_type{});
     }
-    const bool done = ok && nkv > 0 && mbar_wait_warp(&bars[GEO::bOFinal + x], 0, abort, a.status, lim);
+    const bool done = ok && nkv > 0 && poll_wait_warp(&bars[GEO::bOFinal + x], 0, abort, a.status, lim);
     if (it.parts > 1) {
       // one part of a unit: unnormalised O row, m and l for the join. float4 column c of
       // row r at [c][r]: a warp's 32 rows are contiguous
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       }
       dst[32 * BM] = make_float4(m, l, 0.0f, 0.0f);
       __threadfence();
-    } else if (done || (nkv == 0 && mbar_wait_warp(&bars[GEO::bQReady + x], 0, abort, a.status, lim))) {
+    } else if (done || (nkv == 0 && poll_wait_warp(&bars[GEO::bQReady + x], 0, abort, a.status, lim))) {
       // (no tiles: Q_x has landed before its buffer is reused below)
       tc_fence_after();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -422,10 +422,14 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     auto convert = [&](auto conv, uint32_t codes, uint32_t tiles, int n_ld, int n_kv, uint64_t* ld_full, uint64_t* ld_empty,
                        uint64_t* kv_full, uint64_t* kv_empty, int rec, int stage_bytes) {
       conv.init(t);
+      bool ready = false;
       for (int j = 0; j < nkv; ++j) {
         const int ls = j % n_ld, ks = j % n_kv;
-        if (!mbar_wait_warp(&ld_full[ls], (j / n_ld) & 1, abort, a.status, lim)) break;
-        if (j >= n_kv && !mbar_wait_warp(&kv_empty[ks], ((j / n_kv) - 1) & 1, abort, a.status, lim)) break;
+        // usually already found ready at the end of the last tile
+        if (!__all_sync(0xffffffffu, ready)) {
+          if (!poll_wait_warp(&ld_full[ls], (j / n_ld) & 1, abort, a.status, lim)) break;
+          if (j >= n_kv && !poll_wait_warp(&kv_empty[ks], ((j / n_kv) - 1) & 1, abort, a.status, lim)) break;
+        }
         const uint32_t dst = tiles + ks * kKVTile;
 #pragma unroll 2
         for (int p = 0; p < 4; ++p) {
@@ -433,6 +437,9 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
           const bool live = e < it.je && it.block_at(e) * kBlock + (r & 15) < it.kv_len;
           conv.row(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, dst, r, t, live);
         }
+        const int jn = j + 1;
+        ready = mbar_test(&ld_full[jn % n_ld], (jn / n_ld) & 1);
+        ready = (jn < n_kv || mbar_test(&kv_empty[jn % n_kv], ((jn / n_kv) - 1) & 1)) && ready && jn < nkv;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -471,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         bool ok;
         if (e < it.je) where = a.p.block(it.seq, it.head, it.block_at(e), ok);
       }
-      if (j >= n_ld && !mbar_wait_warp(&empty[ls], ((j / n_ld) - 1) & 1, abort, a.status, lim)) break;
+      if (j >= n_ld && !poll_wait_warp(&empty[ls], ((j / n_ld) - 1) & 1, abort, a.status, lim)) break;
       const int nb = min(4, n_blk - 4 * j);
       if (lane == 0) mbar_arrive_expect_tx(&full[ls], nb * rec);
       __syncwarp();
@@ -509,11 +516,11 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         for (int kk = 0; kk < BN / 16; ++kk)
           mma_bf16_ts(tO, p + 8 * kk, v + ((kk * 2048) >> 4), idPV, (j > 0 || kk > 0) ? 1u : 0u);
       };
-      auto wait_k = [&](int j) { return mbar_wait(&bars[GEO::bKvFull + j % NK], (j / NK) & 1, abort, a.status, lim); };
+      auto wait_k = [&](int j) { return poll_wait(&bars[GEO::bKvFull + j % NK], (j / NK) & 1, abort, a.status, lim); };
       auto wait_v = [&](int j) {
-        return mbar_wait(&bars[GEO::bKvFull + NK + j % NV], (j / NV) & 1, abort, a.status, lim);
+        return poll_wait(&bars[GEO::bKvFull + NK + j % NV], (j / NV) & 1, abort, a.status, lim);
       };
-      bool ok = nkv > 0 && mbar_wait(&bars[GEO::bQReady + x], 0, abort, a.status, lim) && wait_k(0);
+      bool ok = nkv > 0 && poll_wait(&bars[GEO::bQReady + x], 0, abort, a.status, lim) && wait_k(0);
       if (ok) {
         tc_fence_after();
         issue_s(0);
@@ -529,11 +536,11 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       for (int j = 0; j < nkv && ok; ++j) {
         if (!v_ready && !(ok = wait_v(j))) break;
         if (j + 2 < nkv && !k_ready && !(ok = wait_k(j + 2))) break;
-        if (!(ok = mbar_wait(&bars[GEO::bPFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim))) break;
+        if (!(ok = poll_wait(&bars[GEO::bPFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim))) break;
         tc_fence_after();
         issue_pv(j);
-        v_ready = j + 1 < nkv && mbar_try_wait(smem_u32(&bars[GEO::bKvFull + NK + (j + 1) % NV]), ((j + 1) / NV) & 1);
-        k_ready = j + 3 < nkv && mbar_try_wait(smem_u32(&bars[GEO::bKvFull + (j + 3) % NK]), ((j + 3) / NK) & 1);
+        v_ready = j + 1 < nkv && mbar_test(&bars[GEO::bKvFull + NK + (j + 1) % NV], ((j + 1) / NV) & 1);
+        k_ready = j + 3 < nkv && mbar_test(&bars[GEO::bKvFull + (j + 3) % NK], ((j + 3) / NK) & 1);
         if (j + 2 < nkv) {
           issue_s(j + 2);
         } else if (j + 2 == nkv) {
