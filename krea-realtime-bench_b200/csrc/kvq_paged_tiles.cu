@@ -47,6 +47,8 @@ struct Geo {
   static constexpr int kStageK = 4 * kRecK, kStageV = 4 * kRecV;
   static constexpr int NK = 4, NV = VB == 8 ? 3 : 4;
   static constexpr int LK = KB == 8 ? 2 : 3, LV = KB == 8 ? 2 : 3;
+  static constexpr int kReady = 4;
+  static_assert(NK == 4 && NV <= 4, "no tile may be converted before the barrier of the one kReady before it completes");
   static constexpr int kOffK = 0;
   static constexpr int kOffV = kOffK + NK * kKVTile;
   static constexpr int kOffQ = kOffV + NV * kKVTile;
@@ -54,8 +56,8 @@ struct Geo {
   static constexpr int kOffCV = kOffCK + LK * kStageK;
   static constexpr int kOffBar = (kOffCV + LV * kStageV + 15) / 16 * 16;
   // barriers; index + stages of K for V
-  static constexpr int bLdFull = 0, bLdEmpty = bLdFull + LK + LV, bKvFull = bLdEmpty + LK + LV,
-                       bKvEmpty = bKvFull + NK + NV, bQReady = bKvEmpty + NK + NV, bSFull = bQReady + 2,
+  static constexpr int bLdFull = 0, bLdEmpty = bLdFull + LK + LV, bK01 = bLdEmpty + LK + LV, bReady = bK01 + 2,
+                       bKvEmpty = bReady + kReady, bQReady = bKvEmpty + NK + NV, bSFull = bQReady + 2,
                        bPFull = bSFull + 4, bOReady = bPFull + 4, bOFinal = bOReady + 2, bMmaDone = bOFinal + 2,
                        kNumBars = bMmaDone + 2;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
@@ -168,17 +170,17 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   const int nq = it.n_rows > BM ? 2 : 1;
   const int n_blk = it.je - it.jb;  // entries of the block list
   const int nkv = (n_blk + 3) / 4;
+  const int n_conv = nq == 2 ? 2 : 4;  // converter warps of a tensor: without a second Q tile its softmax warps help
 
   if (tid == 0) {
     for (int i = 0; i < LK + LV; ++i) {
       mbar_init(&bars[GEO::bLdFull + i], 1);
-      mbar_init(&bars[GEO::bLdEmpty + i], 2);  // the tensor's two converter warps
+      mbar_init(&bars[GEO::bLdEmpty + i], n_conv);
     }
-    for (int i = 0; i < NK + NV; ++i) {
-      mbar_init(&bars[GEO::bKvFull + i], 2);
-      mbar_init(&bars[GEO::bKvEmpty + i], nq);
-    }
+    for (int i = 0; i < NK + NV; ++i) mbar_init(&bars[GEO::bKvEmpty + i], nq);
+    for (int i = 0; i < GEO::kReady; ++i) mbar_init(&bars[GEO::bReady + i], 2 * n_conv);
     for (int x = 0; x < 2; ++x) {
+      mbar_init(&bars[GEO::bK01 + x], n_conv);
       mbar_init(&bars[GEO::bQReady + x], 8);  // the eight gathering warps
       mbar_init(&bars[GEO::bSFull + 2 * x], 1);
       mbar_init(&bars[GEO::bSFull + 2 * x + 1], 1);
@@ -413,29 +415,36 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       __syncwarp();
       store_rows(stage, (warp & 3) * 32, x * BM + (warp & 3) * 32);
     }
-  } else if (warp < 8) {
-    // a Q tile without rows: nothing to do
   } else if (warp < kProdWarp) {
     // ------------------------------------------------------------ converters
-    const int is_v = (warp - kConvWarp0) >> 1;
-    const int t = lane & 3, r0 = (warp & 1) * 32 + (lane >> 2);
+    // V(j) and K(j+2), the two tiles that the MMAs issued at step j read, count on one
+    // barrier, so an MMA thread waits once: K(j) arrives on barrier j - 2, K(0) and
+    // K(1) on their own. Two steps past its last tile the K side arrives for the tiles that
+    // there are not. A barrier is not reused early: K(j+6) and V(j+4) are converted
+    // only after S(j+2) has completed, which was issued behind a wait for barrier j.
+    const int is_v = (warp >> 1) & 1;
+    const int rows = 64 / n_conv;  // of this warp
+    const int t = lane & 3, r0 = ((warp & 1) + (warp < kConvWarp0 ? 2 : 0)) * rows + (lane >> 2);
     auto convert = [&](auto conv, uint32_t codes, uint32_t tiles, int n_ld, int n_kv, uint64_t* ld_full, uint64_t* ld_empty,
-                       uint64_t* kv_full, uint64_t* kv_empty, int rec, int stage_bytes) {
+                       uint64_t* kv_empty, int rec, int stage_bytes) {
       conv.init(t);
       bool ready = false;
-      for (int j = 0; j < nkv; ++j) {
+      const int steps = nkv + (is_v ? 0 : 2);
+      for (int j = 0; j < steps; ++j) {
         const int ls = j % n_ld, ks = j % n_kv;
         // usually already found ready at the end of the last tile
         if (!__all_sync(0xffffffffu, ready)) {
-          if (!poll_wait_warp(&ld_full[ls], (j / n_ld) & 1, abort, a.status, lim)) break;
+          if (j < nkv && !poll_wait_warp(&ld_full[ls], (j / n_ld) & 1, abort, a.status, lim)) break;
           if (j >= n_kv && !poll_wait_warp(&kv_empty[ks], ((j / n_kv) - 1) & 1, abort, a.status, lim)) break;
         }
-        const uint32_t dst = tiles + ks * kKVTile;
+        if (j < nkv) {
+          const uint32_t dst = tiles + ks * kKVTile;
 #pragma unroll 2
-        for (int p = 0; p < 4; ++p) {
-          const int r = r0 + 8 * p, e = it.jb + 4 * j + (r >> 4);
-          const bool live = e < it.je && it.block_at(e) * kBlock + (r & 15) < it.kv_len;
-          conv.row(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, dst, r, t, live);
+          for (int p = 0; p < rows; p += 8) {
+            const int r = r0 + p, e = it.jb + 4 * j + (r >> 4);
+            const bool live = e < it.je && it.block_at(e) * kBlock + (r & 15) < it.kv_len;
+            conv.row(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, dst, r, t, live);
+          }
         }
         const int jn = j + 1;
         ready = mbar_test(&ld_full[jn % n_ld], (jn / n_ld) & 1);
@@ -443,23 +452,25 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&ld_empty[ls]);
-          mbar_arrive(&kv_full[ks]);
+          if (j < nkv) mbar_arrive(&ld_empty[ls]);
+          const int on = is_v ? j : j - 2;
+          if (on >= 0)
+            mbar_arrive(&bars[GEO::bReady + on % GEO::kReady]);
+          else if (j < nkv)
+            mbar_arrive(&bars[GEO::bK01 + j]);
         }
       }
     };
     const uint32_t codes = sbase + (is_v ? GEO::kOffCV : GEO::kOffCK), dst = sbase + (is_v ? GEO::kOffV : GEO::kOffK);
     uint64_t* const ld_full = bars + GEO::bLdFull + (is_v ? LK : 0);
     uint64_t* const ld_empty = bars + GEO::bLdEmpty + (is_v ? LK : 0);
-    uint64_t* const kv_full = bars + GEO::bKvFull + (is_v ? NK : 0);
     uint64_t* const kv_empty = bars + GEO::bKvEmpty + (is_v ? NK : 0);
     // one copy of the loop where K and V have the same format: the instruction caches
     // hold four different loops per sub-partition as it is
     if (KB == VB || !is_v)
-      convert(Converter<L, KB>{}, codes, dst, is_v ? LV : LK, is_v ? NV : NK, ld_full, ld_empty, kv_full, kv_empty, GEO::kRecK,
-              GEO::kStageK);
+      convert(Converter<L, KB>{}, codes, dst, is_v ? LV : LK, is_v ? NV : NK, ld_full, ld_empty, kv_empty, GEO::kRecK, GEO::kStageK);
     else
-      convert(Converter<L, VB>{}, codes, dst, LV, NV, ld_full, ld_empty, kv_full, kv_empty, GEO::kRecV, GEO::kStageV);
+      convert(Converter<L, VB>{}, codes, dst, LV, NV, ld_full, ld_empty, kv_empty, GEO::kRecV, GEO::kStageV);
   } else if (warp == kProdWarp || warp == kProdWarpV) {
     // ------------------------------------------------------------ producers
     const bool pv = warp != kProdWarp;
@@ -516,31 +527,27 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         for (int kk = 0; kk < BN / 16; ++kk)
           mma_bf16_ts(tO, p + 8 * kk, v + ((kk * 2048) >> 4), idPV, (j > 0 || kk > 0) ? 1u : 0u);
       };
-      auto wait_k = [&](int j) { return poll_wait(&bars[GEO::bKvFull + j % NK], (j / NK) & 1, abort, a.status, lim); };
-      auto wait_v = [&](int j) {
-        return poll_wait(&bars[GEO::bKvFull + NK + j % NV], (j / NV) & 1, abort, a.status, lim);
-      };
-      bool ok = nkv > 0 && poll_wait(&bars[GEO::bQReady + x], 0, abort, a.status, lim) && wait_k(0);
+      bool ok = nkv > 0 && poll_wait(&bars[GEO::bQReady + x], 0, abort, a.status, lim) &&
+                poll_wait(&bars[GEO::bK01], 0, abort, a.status, lim);
       if (ok) {
         tc_fence_after();
         issue_s(0);
-        if (nkv > 1 && (ok = wait_k(1))) {
+        if (nkv > 1 && (ok = poll_wait(&bars[GEO::bK01 + 1], 0, abort, a.status, lim))) {
           tc_fence_after();
           issue_s(1);
         }
       }
       // A test of a barrier takes this thread over 100 cycles even where its phase has
-      // completed, and a tile's issue is what it has time for: V(j) and K(j+2) are tested
-      // while the MMAs of tile j - 1 are still being issued, and waited for only if that failed.
-      bool v_ready = false, k_ready = false;
+      // completed, and a tile's issue is what it has time for: the tiles of step j + 1 are
+      // tested before S(j+2) is issued, and waited for only if that failed.
+      bool ready = false;
       for (int j = 0; j < nkv && ok; ++j) {
-        if (!v_ready && !(ok = wait_v(j))) break;
-        if (j + 2 < nkv && !k_ready && !(ok = wait_k(j + 2))) break;
+        if (!ready && !(ok = poll_wait(&bars[GEO::bReady + j % GEO::kReady], (j / GEO::kReady) & 1, abort, a.status, lim)))
+          break;
         if (!(ok = poll_wait(&bars[GEO::bPFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim))) break;
         tc_fence_after();
         issue_pv(j);
-        v_ready = j + 1 < nkv && mbar_test(&bars[GEO::bKvFull + NK + (j + 1) % NV], ((j + 1) / NV) & 1);
-        k_ready = j + 3 < nkv && mbar_test(&bars[GEO::bKvFull + (j + 3) % NK], ((j + 3) / NK) & 1);
+        ready = j + 1 < nkv && mbar_test(&bars[GEO::bReady + (j + 1) % GEO::kReady], ((j + 1) / GEO::kReady) & 1);
         if (j + 2 < nkv) {
           issue_s(j + 2);
         } else if (j + 2 == nkv) {
