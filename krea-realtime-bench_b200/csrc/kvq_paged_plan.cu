@@ -103,20 +103,20 @@ static void cut_rows(const std::vector<Unit>& units, int n_heads, int64_t n_resi
 // Many rows: one CTA per item and SM, started in the order of the list, long units first.
 // Which units are cut into parts, and into how many, is chosen by simulating that list
 // on the SMs for a few ways to cut it: none; all units, the units behind the last full
-// wave, or those and one wave more, into pieces of about 1/1 to 1/4 of an SM's share of
-// them. Costs in tiles of 64 tokens: kItemCost for an item (fill, epilogue), kPartCost
-// more for a part's partial sums and kJoinCost for each part that the last one joins.
+// wave, or those and one wave more, into the smallest equal pieces of which there are
+// at most one to three waves. Costs in tiles of 64 tokens, measured (a tile of two Q
+// tiles takes about 2100 cycles): kItemCost for an item (fill, epilogue), kPartCost
+// more for a part's partial sums, kJoinCost and kJoinPart per part for the join.
 // Lists of more than kSimWaves waves are left whole: the last wave is a small share.
-constexpr double kItemCost = 4.0, kPartCost = 1.5, kJoinCost = 0.5;
+constexpr double kItemCost = 4.0, kPartCost = 0.5, kJoinCost = 1.5, kJoinPart = 0.5;
 constexpr int kMinTiles = 4, kMaxTileParts = 32, kSimWaves = 8;
 
 struct Cut {
-  size_t from;   // units (heads multiplied) from this one on are cut
-  double piece;  // into pieces of about this many tiles
+  size_t from;    // units (heads multiplied) from this one on are cut
+  int64_t piece;  // into the fewest parts of at most this many tiles (0: none are)
   int parts(size_t i, int64_t t) const {
     if (i < from || piece <= 0) return 1;
-    const int64_t n = static_cast<int64_t>(static_cast<double>(t) / piece + 0.5);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({n, t / kMinTiles, kMaxTileParts})));
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((t + piece - 1) / piece, kMaxTileParts)));
   }
 };
 
@@ -133,7 +133,7 @@ static double simulate(const std::vector<Unit>& units, int n_heads, int n_sms, c
       const double cost = pace * static_cast<double>(t) / parts + kItemCost + (parts > 1 ? kPartCost : 0.0);
       for (int k = 0; k < parts; ++k) {
         std::pop_heap(busy.begin(), busy.end(), later);
-        busy.back() += cost + (parts > 1 && k + 1 == parts ? kJoinCost * parts : 0.0);
+        busy.back() += cost + (parts > 1 && k + 1 == parts ? kJoinCost + kJoinPart * parts : 0.0);
         end = std::max(end, busy.back());
         std::push_heap(busy.begin(), busy.end(), later);
       }
@@ -146,20 +146,26 @@ static void cut_tiles(std::vector<Unit>& units, int n_heads, int n_sms, Plan* p)
   if (units.empty()) return;
   std::stable_sort(units.begin(), units.end(), [](const Unit& a, const Unit& b) { return a.n > b.n; });
   const size_t n = units.size() * n_heads, wave = static_cast<size_t>(n_sms);
-  Cut best{n, 0.0};
+  Cut best{n, 0};
   if (n <= kSimWaves * wave) {
     double least = simulate(units, n_heads, n_sms, best);
     const size_t rest = n % wave;
     const size_t tail[3] = {n, rest, rest + wave};
     for (int m = 0; m < 3; ++m) {
       if (tail[m] == 0 || tail[m] > n || (m > 0 && tail[m] == n)) continue;
-      double work = 0.0;
-      size_t i = 0;
-      for (const Unit& u : units)
-        for (int h = 0; h < n_heads; ++h, ++i)
-          if (i >= n - tail[m]) work += (u.n + 3) / 4;
-      for (int k = 1; k <= 4; ++k) {
-        const Cut c{n - tail[m], work / (static_cast<double>(wave) * k)};
+      for (int k = 1; k <= 3; ++k) {
+        // the smallest piece that gives at most k waves
+        Cut c{n - tail[m], 0};
+        int64_t lo = kMinTiles, hi = (units.front().n + 3) / 4 + 1;
+        while (lo < hi) {
+          c.piece = (lo + hi) / 2;
+          size_t pieces = 0, i = 0;
+          for (const Unit& u : units)
+            for (int h = 0; h < n_heads; ++h, ++i)
+              if (i >= c.from) pieces += c.parts(i, (u.n + 3) / 4);
+          if (pieces <= wave * k) hi = c.piece; else lo = c.piece + 1;
+        }
+        c.piece = lo;
         const double end = simulate(units, n_heads, n_sms, c);
         if (end < least * 0.98) {  // a cut has to be worth something
           least = end;

@@ -172,6 +172,71 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   const int nkv = (n_blk + 3) / 4;
   const int n_conv = nq == 2 ? 2 : 4;  // converter warps of a tensor: without a second Q tile its softmax warps help
 
+  // where row n of the item reads its query and writes its output
+  auto place = [&](int n, int64_t& tok, int& h) {
+    const int row = it.row0 + n, i = row / a.group;
+    tok = it.q_first + i;
+    h = it.head * a.group + row - i * a.group;
+  };
+  // Offset of row n's head in q (0: out); a division, so each lane makes one and rows are
+  // passed around by shuffles.
+  auto q_offset = [&](int n, int64_t stride) {
+    int64_t tok;
+    int h;
+    place(min(n, it.n_rows - 1), tok, h);
+    return tok * stride + h * D;
+  };
+  // A warp's n_out (at most 32) output rows, n0.. of the item, staged in the Q buffer, to
+  // global memory: half a warp per row, 256 contiguous bytes.
+  auto store_rows = [&](int n0, int n_out) {
+    const int64_t mine = q_offset(n0 + lane, a.out_stride);
+#pragma unroll 4
+    for (int k = 0; k < n_out / 2; ++k) {
+      const int i = 2 * k + (lane >> 4), n = n0 + i, rr = n & (BM - 1), c = lane & 15;
+      const int64_t to = __shfl_sync(0xffffffffu, mine, i);
+      const uint32_t stage = sbase + GEO::kOffQ + (n >> 7) * kQTile;
+      if (n < it.n_rows)
+        st_global_v4(a.out + to + 8 * c, ld_shared_v4(stage + (c >> 3) * kQAtom + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)));
+    }
+  };
+  auto stage_chunk = [&](uint32_t stage, int r, int ch, const float* v, float inv) {
+    st_shared_v4(stage + (ch >> 3) * kQAtom + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
+                 pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv),
+                 pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
+  };
+  auto store_lse = [&](int n, float m, float l) {
+    if (a.lse && n < it.n_rows) {
+      int64_t tok;
+      int h;
+      place(n, tok, h);
+      a.lse[tok * a.n_q_heads + h] = l == 0.0f ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
+    }
+  };
+
+  // Under way before the barriers are set up: the Q rows, gathered by the eight softmax
+  // warps (two rows at a time), and the producers' first look-ups.
+  int64_t where = 0;  // producer lane i: the pool block of list entry 32 k + i
+  auto look_up = [&](int j) {
+    const int e = it.jb + 4 * j + lane;
+    bool ok;
+    if (e < it.je) where = a.p.block(it.seq, it.head, it.block_at(e), ok);
+  };
+  if (warp < 8) {
+    const int64_t mine = q_offset(16 * (lane >> 1) + 2 * warp + (lane & 1), a.q_stride);
+#pragma unroll 4
+    for (int k = 0; k < 8 * nq; ++k) {
+      const int n = 16 * k + (tid >> 4), c = tid & 15, r = n & (BM - 1);
+      const int64_t from = __shfl_sync(0xffffffffu, mine, 2 * k + (lane >> 4));
+      const uint32_t dst = sbase + GEO::kOffQ + (n >> 7) * kQTile + (c >> 3) * kQAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+      if (n < it.n_rows)
+        cp_async16(dst, a.q + from + 8 * c);
+      else
+        st_shared_v4(dst, 0, 0, 0, 0);
+    }
+  } else if (warp == kProdWarp || warp == kProdWarpV) {
+    look_up(0);
+  }
+
   if (tid == 0) {
     for (int i = 0; i < LK + LV; ++i) {
       mbar_init(&bars[GEO::bLdFull + i], 1);
@@ -202,55 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // where row n of the item reads its query and writes its output
-  auto place = [&](int n, int64_t& tok, int& h) {
-    const int row = it.row0 + n, i = row / a.group;
-    tok = it.q_first + i;
-    h = it.head * a.group + row - i * a.group;
-  };
-  // A warp's 32 output rows (rows n0.. of the item, rr0.. of the Q tile), staged in
-  // the Q buffer, to global memory: half a warp per row, 256 contiguous bytes.
-  auto store_rows = [&](uint32_t stage, int rr0, int n0) {
-#pragma unroll 4
-    for (int k = 0; k < 16; ++k) {
-      const int rr = rr0 + 2 * k + (lane >> 4), n = n0 + 2 * k + (lane >> 4), c = lane & 15;
-      if (n < it.n_rows) {
-        int64_t tok;
-        int h;
-        place(n, tok, h);
-        const uint4 v = ld_shared_v4(stage + (c >> 3) * kQAtom + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
-        st_global_v4(a.out + tok * a.out_stride + h * D + 8 * c, v);
-      }
-    }
-  };
-  auto stage_chunk = [&](uint32_t stage, int r, int ch, const float* v, float inv) {
-    st_shared_v4(stage + (ch >> 3) * kQAtom + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
-                 pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv),
-                 pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
-  };
-  auto store_lse = [&](int n, float m, float l) {
-    if (a.lse && n < it.n_rows) {
-      int64_t tok;
-      int h;
-      place(n, tok, h);
-      a.lse[tok * a.n_q_heads + h] = l == 0.0f ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
-    }
-  };
-
   if (warp < 8) {
-    // ------------------------------------------------------------ Q, by all eight softmax warps
-    for (int k = 0; k < 8 * nq; ++k) {
-      const int n = 16 * k + (tid >> 4), c = tid & 15, r = n & (BM - 1);
-      const uint32_t dst = sbase + GEO::kOffQ + (n >> 7) * kQTile + (c >> 3) * kQAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-      if (n < it.n_rows) {
-        int64_t tok;
-        int h;
-        place(n, tok, h);
-        cp_async16(dst, a.q + tok * a.q_stride + h * D + 8 * c);
-      } else {
-        st_shared_v4(dst, 0, 0, 0, 0);
-      }
-    }
     asm volatile("cp.async.wait_all;" ::: "memory");
     fence_proxy_async_smem();
     __syncwarp();
@@ -413,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         for (int c = 0; c < 4; ++c) stage_chunk(stage, r, 4 * k + c, v + 8 * c, inv);
       }
       __syncwarp();
-      store_rows(stage, (warp & 3) * 32, x * BM + (warp & 3) * 32);
+      store_rows(warp * 32, 32);
     }
   } else if (warp < kProdWarp) {
     // ------------------------------------------------------------ converters
@@ -480,15 +497,10 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     uint64_t* full = bars + GEO::bLdFull + (pv ? LK : 0);
     uint64_t* empty = bars + GEO::bLdEmpty + (pv ? LK : 0);
     const uint32_t base = sbase + (pv ? GEO::kOffCV : GEO::kOffCK);
-    int64_t where = 0;  // lane i: the pool block of list entry 32 k + i
     int issued = 0;
     for (int j = 0; j < nkv; ++j) {
       const int ls = j % n_ld;
-      if ((j & 7) == 0) {
-        const int e = it.jb + 4 * j + lane;
-        bool ok;
-        if (e < it.je) where = a.p.block(it.seq, it.head, it.block_at(e), ok);
-      }
+      if (j > 0 && (j & 7) == 0) look_up(j);
       if (j >= n_ld && !poll_wait_warp(&empty[ls], ((j / n_ld) - 1) & 1, abort, a.status, lim)) break;
       const int nb = min(4, n_blk - 4 * j);
       if (lane == 0) mbar_arrive_expect_tx(&full[ls], nb * rec);
@@ -576,40 +588,47 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       if (*last) a.ctr[it.unit] = 0u;  // ready for the next launch
     }
     __syncthreads();
-    if (*last && warp < 4 * nq) {
+    if (*last) {
+      // All 16 warps: a thread has one row and a half (two Q tiles) or a quarter of its
+      // columns, so that the loads of eight float4 and two parts are in flight.
       __threadfence();
-      const int x = warp >> 2, r = tid - x * BM, n = tid;
+      const int n = tid & (nq * BM - 1), x = n >> 7, r = n & (BM - 1);
+      const int n_col = 16 * nq / 2, c0 = (tid / (nq * BM)) * n_col;  // float4 columns of this thread
       const int64_t pstride = static_cast<int64_t>(2) * 33 * BM;
       const float4* src = reinterpret_cast<const float4*>(a.ws) + (static_cast<int64_t>(it.slot) * 2 + x) * 33 * BM + r;
       float mx = -1.0e30f, lsum = 0.0f;
+#pragma unroll 4
       for (int p = 0; p < it.parts; ++p) mx = fmaxf(mx, __ldcg(src + p * pstride + 32 * BM).x);
+#pragma unroll 4
       for (int p = 0; p < it.parts; ++p) {
         const float4 ml = __ldcg(src + p * pstride + 32 * BM);
         lsum = fmaf(ml.y, ex2f(ml.x - mx), lsum);
       }
       const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-      store_lse(n, mx, lsum);
+      if (c0 == 0) store_lse(n, mx, lsum);
       const uint32_t stage = sbase + GEO::kOffQ + x * kQTile;
 #pragma unroll 1
-      for (int ch = 0; ch < 16; ++ch) {
-        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      for (int g = c0; g < c0 + n_col; g += 8) {
+        float acc[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[i] = 0.0f;
 #pragma unroll 2
         for (int p = 0; p < it.parts; ++p) {
           const float f = ex2f(__ldcg(src + p * pstride + 32 * BM).x - mx);
-          const float4 v0 = __ldcg(src + p * pstride + (2 * ch) * BM), v1 = __ldcg(src + p * pstride + (2 * ch + 1) * BM);
-          acc[0] = fmaf(v0.x, f, acc[0]);
-          acc[1] = fmaf(v0.y, f, acc[1]);
-          acc[2] = fmaf(v0.z, f, acc[2]);
-          acc[3] = fmaf(v0.w, f, acc[3]);
-          acc[4] = fmaf(v1.x, f, acc[4]);
-          acc[5] = fmaf(v1.y, f, acc[5]);
-          acc[6] = fmaf(v1.z, f, acc[6]);
-          acc[7] = fmaf(v1.w, f, acc[7]);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float4 v = __ldcg(src + p * pstride + (g + c) * BM);
+            acc[4 * c] = fmaf(v.x, f, acc[4 * c]);
+            acc[4 * c + 1] = fmaf(v.y, f, acc[4 * c + 1]);
+            acc[4 * c + 2] = fmaf(v.z, f, acc[4 * c + 2]);
+            acc[4 * c + 3] = fmaf(v.w, f, acc[4 * c + 3]);
+          }
         }
-        stage_chunk(stage, r, ch, acc, inv);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) stage_chunk(stage, r, g / 2 + c, acc + 8 * c, inv);
       }
-      __syncwarp();
-      store_rows(stage, (warp & 3) * 32, x * BM + (warp & 3) * 32);
+      __syncthreads();
+      store_rows(warp * 8 * nq, 8 * nq);
     }
   }
 }
