@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include "kvq_paged.cuh"
 #include "kvq_sm100.cuh"
@@ -103,6 +104,82 @@ __device__ __forceinline__ uint32_t int8_pair(uint32_t x) {
   uint32_t d;
   asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(d) : "r"(x), "r"(0x00800080u), "r"(0x43804380u));  // (x & m) ^ o
   return hsub2(and_or(x, 0x007F007Fu, 0x43004300u), d);
+}
+
+// Keys, and the queries they meet, are multiplied as fp16 rather than bf16: an int4 code
+// times a bf16 scale has eleven significant bits, which fp16 holds and bf16 rounds to
+// eight (that rounding, on the logits, was most of the output's error). fp16 ends at 65504
+// and thins out below 2^-14, so a token whose largest key scale lies beyond
+// [kKeyScaleLeast, kKeyScaleMost] is multiplied as if its scales were 2^-e times as large,
+// and a query row likewise; the logits get the power of two back in fp32, which changes
+// no other row's or token's bits.
+__device__ __forceinline__ uint32_t h16mul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t h16fma2(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), *reinterpret_cast<__half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t h16add2(uint32_t a, uint32_t b) {
+  const __half2 r = __hadd2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Codes at the same places as above -> f16x2 (q, q), exact: 1024 + code - 1032, and
+// (1024 + 16 code) / 16 - 72; for int8 1024 + code - 1152.
+__device__ __forceinline__ uint32_t int4_low_f16(uint32_t x) {
+  return h16add2(and_or(x, 0x000F000Fu, 0x64006400u), 0xE408E408u);
+}
+__device__ __forceinline__ uint32_t int4_high_f16(uint32_t x) {
+  return h16fma2(and_or(x, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
+}
+__device__ __forceinline__ uint32_t int8_pair_f16(uint32_t x) {
+  return h16add2(and_or(x, 0x00FF00FFu, 0x64006400u), 0xE480E480u);
+}
+constexpr uint32_t kKeyScaleLeast = 0x3880, kKeyScaleMost = 0x4400;  // bf16 2^-14, 512 (127 * 512 < 65504)
+constexpr uint32_t kQueryLeast = 0x3B80, kQueryMost = 0x4700;        // bf16 2^-8, 2^15
+// bits of a bf16 >= 0 outside [least, most]
+__device__ __forceinline__ bool beyond(uint32_t bits, uint32_t least, uint32_t most) { return bits - least > most - least; }
+// 2^e, |e| <= 126
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+// The exponent to take out of a token whose largest scale has these bits, of a query row
+// whose largest magnitude has: to [256, 512) and [2^14, 2^15) above, to [1, 2) below.
+__device__ __forceinline__ int key_exponent(uint32_t bits) {
+  if (bits == 0 || !beyond(bits, kKeyScaleLeast, kKeyScaleMost)) return 0;
+  const int e = static_cast<int>(bits >> 7) - 127;
+  return bits > kKeyScaleMost ? min(e - 8, 119) : max(e, -110);
+}
+__device__ __forceinline__ int query_exponent(uint32_t bits) {
+  if (bits == 0 || !beyond(bits, kQueryLeast, kQueryMost)) return 0;
+  const int e = static_cast<int>(bits >> 7) - 127;
+  return bits > kQueryMost ? e - 14 : max(e, -110);
+}
+// Largest finite magnitude among eight bf16, as bits.
+__device__ __forceinline__ uint32_t most_of(const uint4& v) {
+  uint32_t m = 0;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = w[i] & 0x7FFFu, hi = (w[i] >> 16) & 0x7FFFu;
+    m = max(m, lo < 0x7F80u ? lo : 0u);
+    m = max(m, hi < 0x7F80u ? hi : 0u);
+  }
+  return m;
+}
+// Eight bf16 times 2^-e -> fp16 (exact for normal results).
+__device__ __forceinline__ uint4 to_f16(const uint4& v, int e) {
+  const float f = pow2i(-e);
+  uint4 o;
+  o.x = pack_f16x2(bf16lo_to_f32(v.x) * f, bf16hi_to_f32(v.x) * f);
+  o.y = pack_f16x2(bf16lo_to_f32(v.y) * f, bf16hi_to_f32(v.y) * f);
+  o.z = pack_f16x2(bf16lo_to_f32(v.z) * f, bf16hi_to_f32(v.z) * f);
+  o.w = pack_f16x2(bf16lo_to_f32(v.w) * f, bf16hi_to_f32(v.w) * f);
+  return o;
 }
 
 // Most channel groups that an aligned run of N channels meets.

@@ -6,7 +6,7 @@
 // other; warp w takes every fourth pair of 16-token storage blocks of a piece. A block's K
 // and V records are contiguous, so a stage of the warp's ring is filled by four bulk
 // copies (no tensor map) while the other stage is worked on; the warps never wait for
-// each other inside a piece. Per block (tokens j, rows n, channels c; mma.sync m16n8k16, bf16 in, fp32 out):
+// each other inside a piece. Per block (tokens j, rows n, channels c; mma.sync m16n8k16, fp32 out):
 //   S^T[j, n] = sum_c K[j, c] q[n, c]      A = K from registers, B = q held in registers
 //   p = 2^(S^T scale - m_n)                m_n lags the true maximum by at most 8: it moves
 //                                          (and O, l are rescaled) only when some logit
@@ -54,6 +54,13 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                                          uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -167,16 +174,24 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
     }
     if (n_mine > 0) issue(0);
     uint32_t qf[NT][8][2];
+    float sc[NT][2];  // softmax scale of rows 8 nt + 2t, + 2t + 1, with the power of two taken from the row
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      uint32_t most = max(max(most_of(qv[nt][0]), most_of(qv[nt][1])), max(most_of(qv[nt][2]), most_of(qv[nt][3])));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int e = query_exponent(most);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sc[nt][i] = a.scale_log2 * pow2i(__shfl_sync(0xffffffffu, e, 4 * (2 * t + i)));
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const uint4 v = 8 * nt + g < it.n_rows ? qv[nt][w] : make_uint4(0, 0, 0, 0);
+        const uint4 v = 8 * nt + g < it.n_rows ? to_f16(qv[nt][w], e) : make_uint4(0, 0, 0, 0);
         qf[nt][2 * w][0] = __byte_perm(v.x, v.z, 0x5410);
         qf[nt][2 * w][1] = __byte_perm(v.x, v.z, 0x7632);
         qf[nt][2 * w + 1][0] = __byte_perm(v.y, v.w, 0x5410);
         qf[nt][2 * w + 1][1] = __byte_perm(v.y, v.w, 0x7632);
       }
+    }
 
     // what the rows 8 nt + 2t, + 2t + 1 see, and what all rows of the item see
     Seen see[NT][2];
@@ -229,7 +244,8 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[nt][bb][e] = 0.0f;
-        uint32_t kw[2][KB == 4 ? 4 : 8], ks01[2], ks23[2];
+        uint32_t kw[2][KB == 4 ? 4 : 8], ks01[2], ks23[2], kx[2];
+        float kscale[2][KG];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const uint32_t src = k_codes + at + bb * (GEO::kStage / 2) + 8 * r * Rec<L, KB>::CW;
@@ -245,12 +261,29 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           uint32_t x[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) x[q] = q < KG ? ld_shared_u16(sc + 2 * (KG == 1 ? kbase : min(kbase + q, G - 1))) : 0u;
-          ks01[r] = KG == 1 ? __byte_perm(x[0], 0, 0x1010) : __byte_perm(x[0], x[1], 0x5410);
-          if constexpr (KG > 2) ks23[r] = __byte_perm(x[2], x[3], 0x5410);
-          if constexpr (KB == 4) {  // for q / 4
-            ks01[r] = hmul2(ks01[r], kFour);
-            if constexpr (KG > 2) ks23[r] = hmul2(ks23[r], kFour);
+          kx[r] = max(max(x[0], x[1]), max(x[2], x[3]));
+#pragma unroll
+          for (int q = 0; q < KG; ++q) kscale[r][q] = __uint_as_float(x[q] << 16);
+        }
+        // rare: a token whose scales leave fp16's range (kKeyScaleLeast, kKeyScaleMost)
+        const bool wide = __any_sync(0xffffffffu, beyond(kx[0], kKeyScaleLeast, kKeyScaleMost) ||
+                                                      beyond(kx[1], kKeyScaleLeast, kKeyScaleMost));
+        float back[2];
+        if (wide) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            kx[r] = max(kx[r], __shfl_xor_sync(0xffffffffu, kx[r], 1));
+            kx[r] = max(kx[r], __shfl_xor_sync(0xffffffffu, kx[r], 2));
+            const int e = key_exponent(kx[r]);
+            back[r] = pow2i(e);
+#pragma unroll
+            for (int q = 0; q < KG; ++q) kscale[r][q] *= pow2i(-e);
           }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          ks01[r] = pack_f16x2(kscale[r][0], kscale[r][KG > 1 ? 1 : 0]);
+          if constexpr (KG > 2) ks23[r] = pack_f16x2(kscale[r][2], kscale[r][KG > 3 ? 3 : 2]);
         }
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -262,20 +295,26 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
               uint32_t v;
               if constexpr (KB == 4) {
                 const uint32_t x = j < 2 ? kw[r][w] : kw[r][w] >> 8;
-                v = (j & 1) ? int4_high(x) : int4_low(x);
+                v = (j & 1) ? int4_high_f16(x) : int4_low_f16(x);
               } else {
-                v = int8_pair(__byte_perm(kw[r][2 * w], kw[r][2 * w + 1], j | j << 4 | (4 + j) << 8 | (4 + j) << 12));
+                v = int8_pair_f16(__byte_perm(kw[r][2 * w], kw[r][2 * w + 1], j | j << 4 | (4 + j) << 8 | (4 + j) << 12));
               }
               uint32_t sp = ks01[r];
               if constexpr (KG > 1) sp = __byte_perm(ks01[r], KG > 2 ? ks23[r] : 0u, ksel[4 * w + j]);
-              f[r][j] = hmul2(v, sp);
+              f[r][j] = h16mul2(v, sp);
             }
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816(s[nt][bb], f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], qf[nt][2 * w + h][0],
-                       qf[nt][2 * w + h][1]);
+              mma16816_f16(s[nt][bb], f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], qf[nt][2 * w + h][0],
+                           qf[nt][2 * w + h][1]);
+        }
+        if (wide) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[nt][bb][e] *= back[e >> 1];
         }
       }
 
@@ -293,8 +332,8 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
               if (!(j < v.hi && (j >= v.lo || j < v.kept)) || (bb && !two)) s[nt][bb][e] = -INFINITY;
             }
         }
-        const float mx0 = fmaxf(fmaxf(s[nt][0][0], s[nt][0][2]), fmaxf(s[nt][1][0], s[nt][1][2])) * a.scale_log2;
-        const float mx1 = fmaxf(fmaxf(s[nt][0][1], s[nt][0][3]), fmaxf(s[nt][1][1], s[nt][1][3])) * a.scale_log2;
+        const float mx0 = fmaxf(fmaxf(s[nt][0][0], s[nt][0][2]), fmaxf(s[nt][1][0], s[nt][1][2])) * sc[nt][0];
+        const float mx1 = fmaxf(fmaxf(s[nt][0][1], s[nt][0][3]), fmaxf(s[nt][1][1], s[nt][1][3])) * sc[nt][1];
         if (__any_sync(0xffffffffu, mx0 > m[nt][0] + 8.0f || mx1 > m[nt][1] + 8.0f)) {
           float n0 = mx0, n1 = mx1;
 #pragma unroll
@@ -321,7 +360,7 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
         for (int bb = 0; bb < 2; ++bb) {
           float p[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = ex2f(fmaf(s[nt][bb][e], a.scale_log2, -m[nt][e & 1]));
+          for (int e = 0; e < 4; ++e) p[e] = ex2f(fmaf(s[nt][bb][e], sc[nt][e & 1], -m[nt][e & 1]));
           l[nt][0] += p[0] + p[2];
           l[nt][1] += p[1] + p[3];
           pf[nt][bb][0] = transpose8x8(pack_bf16x2(p[0], p[1]));

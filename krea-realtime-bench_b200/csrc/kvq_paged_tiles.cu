@@ -18,8 +18,8 @@
 // of sight. A tile that some row of the Q tile does not see whole takes a masked step
 // (a 64-bit mask per row; a masked logit is -inf); the running maximum starts at -1e30,
 // so a row without any visible token ends with l = 0 and is stored as 0.
-// K, V, P are rounded to bf16 for the MMA: codes * scale as kvq_paged_read returns
-// them, weights once; S, m, l, O are fp32.
+// Roundings: K and Q as fp16 for S (exact for int4 codes; see kKeyScaleMost), P and V as
+// bf16 for PV (V as kvq_paged_read returns it); S, m, l, O are fp32.
 #include <cmath>
 
 #include "kvq_paged_dev.cuh"
@@ -60,8 +60,13 @@ struct Geo {
                        bKvEmpty = bReady + kReady, bQReady = bKvEmpty + NK + NV, bSFull = bQReady + 2,
                        bPFull = bSFull + 4, bOReady = bPFull + 4, bOFinal = bOReady + 2, bMmaDone = bOFinal + 2,
                        kNumBars = bMmaDone + 2;
-  static constexpr int kOffMisc = kOffBar + kNumBars * 8;
-  static constexpr int kSmemBytes = kOffMisc + 32 + 1024;  // + alignment slack
+  static constexpr int kOffMisc = (kOffBar + kNumBars * 8 + 15) / 16 * 16;
+  // of the last kExp key tiles: the exponent taken out of each token, and a byte per
+  // converter warp that says whether there is any. A tile's are written again only after
+  // S(j + kExp - 4) has completed, behind P(j + kExp - 6) of every softmax warp.
+  static constexpr int kExp = 6;
+  static constexpr int kOffExp = kOffMisc + 32, kOffWide = kOffExp + kExp * BN;
+  static constexpr int kSmemBytes = kOffWide + 4 * kExp + 1024;  // + alignment slack
   static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM must fit");
   static_assert(kOffCK % 16 == 0 && kOffCV % 16 == 0, "bulk copies");
 };
@@ -72,17 +77,14 @@ __device__ __forceinline__ uint32_t tile_off(int r, int c) {
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
-// Converters: four lanes per row, lane t channels 32t..32t+31.
-template <class L, int BITS>
+// Converters: four lanes per row, lane t channels 32t..32t+31. Keys to fp16, values to bf16.
+template <class L, int BITS, bool KEY>
 struct Converter {
   static constexpr int KG = most_groups<L, 32>();
   int base;
@@ -100,8 +102,9 @@ struct Converter {
       }
     }
   }
-  // One row: record block `rec`, row `rr` of it, to row r of the bf16 tile at dst.
-  __device__ __forceinline__ void row(uint32_t rec, int rr, uint32_t dst, int r, int t, bool live) const {
+  // One row: record block `rec`, row `rr` of it, to row r of the tile at dst. For keys
+  // returns the exponent taken out of the row (kKeyScaleMost).
+  __device__ __forceinline__ int row(uint32_t rec, int rr, uint32_t dst, int r, int t, bool live) const {
     using R = Rec<L, BITS>;
     uint32_t w[BITS];  // 4 or 8 words of codes
     const uint32_t src = rec + rr * R::CW + t * (R::CW / 4);
@@ -114,42 +117,68 @@ struct Converter {
       w[4 * i + 3] = v.w;
     }
     const uint32_t sc = rec + R::kCodes + rr * L::G * 2;
-    uint32_t s01, s23 = 0;
-    if constexpr (KG == 1) {
-      s01 = __byte_perm(ld_shared_u16(sc + 2 * base), 0, 0x1010);
-    } else {
-      uint32_t x[4];
+    uint32_t x[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) x[q] = q < KG ? ld_shared_u16(sc + 2 * min(base + q, L::G - 1)) : 0u;
-      s01 = __byte_perm(x[0], x[1], 0x5410);
+    for (int q = 0; q < 4; ++q) {
+      x[q] = q < KG ? ld_shared_u16(sc + 2 * (KG == 1 ? base : min(base + q, L::G - 1))) : 0u;
+      if (!live) x[q] = 0;  // rows past the end hold anything: as zeros they add nothing
+    }
+    uint32_t s01, s23 = 0;
+    int e = 0;
+    if constexpr (KEY) {
+      float f[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) f[q] = __uint_as_float(x[q] << 16);
+      uint32_t most = max(max(x[0], x[1]), max(x[2], x[3]));
+      if (__any_sync(0xffffffffu, beyond(most, kKeyScaleLeast, kKeyScaleMost))) {
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        e = key_exponent(most);
+#pragma unroll
+        for (int q = 0; q < KG; ++q) f[q] *= pow2i(-e);
+      }
+      s01 = pack_f16x2(f[0], f[KG == 1 ? 0 : 1]);
+      if constexpr (KG > 2) s23 = pack_f16x2(f[2], f[3]);
+    } else {
+      s01 = KG == 1 ? x[0] * 0x10001u : __byte_perm(x[0], x[1], 0x5410);
       if constexpr (KG > 2) s23 = __byte_perm(x[2], x[3], 0x5410);
+      if constexpr (BITS == 4) {  // for q / 4
+        s01 = hmul2(s01, kFour);
+        if constexpr (KG > 2) s23 = hmul2(s23, kFour);
+      }
     }
-    if constexpr (BITS == 4) {
-      s01 = hmul2(s01, kFour);
-      s23 = hmul2(s23, kFour);
-    }
-    if (!live) s01 = s23 = 0;  // rows past the end hold anything: as zeros they add nothing
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int hi = t & 2;  // word i ^ hi
       uint32_t o[4];
       if constexpr (BITS == 4) {
-        const uint32_t x = hi ? w[i ^ 2] : w[i], y = x >> 4;
+        const uint32_t v = hi ? w[i ^ 2] : w[i], y = v >> 4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = int4_low(__byte_perm(x, y, (4 + j) << 8 | j));
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t b = __byte_perm(v, y, (4 + j) << 8 | j);
+          o[j] = KEY ? int4_low_f16(b) : int4_low(b);
+        }
       } else {
-        const uint32_t x = hi ? w[2 * (i ^ 2)] : w[2 * i], y = hi ? w[2 * (i ^ 2) + 1] : w[2 * i + 1];
-        o[0] = int8_pair(__byte_perm(x, 0, 0x4140));
-        o[1] = int8_pair(__byte_perm(x, 0, 0x4342));
-        o[2] = int8_pair(__byte_perm(y, 0, 0x4140));
-        o[3] = int8_pair(__byte_perm(y, 0, 0x4342));
+        const uint32_t v = hi ? w[2 * (i ^ 2)] : w[2 * i], y = hi ? w[2 * (i ^ 2) + 1] : w[2 * i + 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t b = __byte_perm(j < 2 ? v : y, 0, (j & 1) ? 0x4342 : 0x4140);
+          o[j] = KEY ? int8_pair_f16(b) : int8_pair(b);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = hmul2(o[j], KG == 1 ? s01 : __byte_perm(s01, s23, sel[KG == 1 ? 0 : 4 * i + j]));
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t sp = KG == 1 ? s01 : __byte_perm(s01, s23, sel[KG == 1 ? 0 : 4 * i + j]);
+        o[j] = KEY ? h16mul2(o[j], sp) : hmul2(o[j], sp);
+      }
       st_shared_v4(dst + tile_off(r, 4 * t + (i ^ hi)), o[0], o[1], o[2], o[3]);
     }
+    return e;
   }
 };
+
+// idesc_bf16 of the S product with fp16 for both operands.
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n) { return idesc_bf16(m, n, 0) & ~((7u << 7) | (7u << 10)); }
 
 template <class L, int KB, int VB>
 __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constant__ AttnArgs a) {
@@ -213,8 +242,16 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     }
   };
 
-  // Under way before the barriers are set up: the Q rows, gathered by the eight softmax
-  // warps (two rows at a time), and the producers' first look-ups.
+  // The exponent to take out of a query row of which each lane of half a warp has a part.
+  auto row_exponent = [&](uint32_t most) {
+    if (!__any_sync(0xffffffffu, beyond(most, kQueryLeast, kQueryMost))) return 0;
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
+    return query_exponent(most);
+  };
+  // Ahead of the set-up of the barriers: the Q rows, gathered by the eight softmax warps
+  // (two rows at a time) and converted to fp16, and the producers' first look-ups.
+  int q_wide = 0;     // whether a power of two was taken out of any query row
   int64_t where = 0;  // producer lane i: the pool block of list entry 32 k + i
   auto look_up = [&](int j) {
     const int e = it.jb + 4 * j + lane;
@@ -228,10 +265,12 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       const int n = 16 * k + (tid >> 4), c = tid & 15, r = n & (BM - 1);
       const int64_t from = __shfl_sync(0xffffffffu, mine, 2 * k + (lane >> 4));
       const uint32_t dst = sbase + GEO::kOffQ + (n >> 7) * kQTile + (c >> 3) * kQAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-      if (n < it.n_rows)
-        cp_async16(dst, a.q + from + 8 * c);
-      else
-        st_shared_v4(dst, 0, 0, 0, 0);
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (n < it.n_rows) v = ld_global_nc_v4(a.q + from + 8 * c);
+      const int e = row_exponent(most_of(v));
+      q_wide |= e;
+      if (n < it.n_rows) v = to_f16(v, e);
+      st_shared_v4(dst, v.x, v.y, v.z, v.w);
     }
   } else if (warp == kProdWarp || warp == kProdWarpV) {
     look_up(0);
@@ -256,6 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       mbar_init(&bars[GEO::bMmaDone + x], 1);
     }
     *abort = 0;
+    for (int i = 0; i < GEO::kExp; ++i) *reinterpret_cast<uint32_t*>(smem + GEO::kOffWide + 4 * i) = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -263,12 +303,11 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  q_wide = __syncthreads_or(q_wide);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
   if (warp < 8) {
-    asm volatile("cp.async.wait_all;" ::: "memory");
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
@@ -290,22 +329,37 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     const Seen fin = seen_by(a, it.start + (it.row0 + n_last) / a.group, it.kv_len);
     float m = -1.0e30f, l = 0.0f;
     bool ok = true, s_ready = false;  // s_ready: S of the coming tile was already found complete
-    auto step = [&](const int j, auto masked) -> bool {
+    // this row's softmax scale, with the power of two taken out of its query
+    float row_scale = a.scale_log2;
+    if (q_wide) {
+      int64_t tok;
+      int h;
+      place(min(n, it.n_rows - 1), tok, h);
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + tok * a.q_stride + h * D);
+      uint32_t most = 0;
+#pragma unroll 4
+      for (int c = 0; c < 16; ++c) most = max(most, most_of(ld_global_nc_v4(src + c)));
+      row_scale *= pow2i(query_exponent(most));
+    }
+    auto step = [&](const int j, const bool wide, auto masked) -> bool {
       constexpr bool MASK = decltype(masked)::value;
       const uint32_t tS = tS0 + 64 * (j & 1);
-      if (!__all_sync(0xffffffffu, s_ready) &&
-          !poll_wait_warp(&bars[GEO::bSFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim))
-        return false;
-      // S_x(j) complete: this Q tile no longer reads K stage j, and PV_x(j-2) (issued
-      // before it) is complete: nor V stage j-2
-      if ((warp & 3) == 0 && lane == 0) {
-        mbar_arrive(&bars[GEO::bKvEmpty + j % NK]);
-        if (j >= 2) mbar_arrive(&bars[GEO::bKvEmpty + NK + (j - 2) % NV]);
-      }
-      tc_fence_after();
       uint32_t s0[32], s1[32];
       tmem_ld32x2_wait(tS, tS + 32, s0, s1);
       if constexpr (MASK) {
+        if (wide) {  // powers of two taken out of the tile's tokens
+          const uint32_t at = sbase + GEO::kOffExp + (j % GEO::kExp) * BN;
+#pragma unroll
+          for (int c = 0; c < 32; c += 16) {
+            const uint4 u = ld_shared_v4(at + c), v = ld_shared_v4(at + 32 + c);
+            const uint32_t eu[4] = {u.x, u.y, u.z, u.w}, ev[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              s0[c + i] = __float_as_uint(__uint_as_float(s0[c + i]) * pow2i(static_cast<int8_t>(eu[i >> 2] >> (8 * (i & 3)))));
+              s1[c + i] = __float_as_uint(__uint_as_float(s1[c + i]) * pow2i(static_cast<int8_t>(ev[i >> 2] >> (8 * (i & 3)))));
+            }
+          }
+        }
         uint32_t mk[2] = {0, 0};  // bit c: column c is seen
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -329,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
 #pragma unroll
       for (int c = 0; c < 32; ++c) pm[c & 7] = fmax3(pm[c & 7], __uint_as_float(s0[c]), __uint_as_float(s1[c]));
       const float mt =
-          fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * a.scale_log2;
+          fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * row_scale;
       bool rescale = false;
       float alpha = 1.0f;
       if (j == 0) {
@@ -342,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       }
       const float nm = -m;
       uint32_t pw[32];
-      const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(nm, nm);
+      const float2 sc2 = make_float2(row_scale, row_scale), nm2 = make_float2(nm, nm);
       float2 sum2 = make_float2(0.0f, 0.0f);
       auto half = [&](const uint32_t (&sv)[32], int base) {
 #pragma unroll
@@ -384,11 +438,25 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       if (lane == 0) mbar_arrive(&bars[GEO::bPFull + 2 * x + (j & 1)]);
       return true;
     };
-    for (int j = 0; j < nkv && ok; ++j) {
+    for (int j = 0; j < nkv; ++j) {
+      if (!__all_sync(0xffffffffu, s_ready) &&
+          !poll_wait_warp(&bars[GEO::bSFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim)) {
+        ok = false;
+        break;
+      }
+      // S_x(j) complete: this Q tile no longer reads K stage j, and PV_x(j-2) (issued
+      // before it) is complete: nor V stage j-2
+      if ((warp & 3) == 0 && lane == 0) {
+        mbar_arrive(&bars[GEO::bKvEmpty + j % NK]);
+        if (j >= 2) mbar_arrive(&bars[GEO::bKvEmpty + NK + (j - 2) % NV]);
+      }
+      tc_fence_after();
+      const bool wide = *reinterpret_cast<volatile uint32_t*>(smem + GEO::kOffWide + 4 * (j % GEO::kExp)) != 0;
       const int e0 = it.jb + 4 * j;
       const int ta = it.block_at(e0) * kBlock, tz = it.block_at(e0 + 3) * kBlock + kBlock;
-      const bool whole = e0 + 4 <= it.je && tz <= first.hi && (ta >= fin.lo || tz <= first.kept);
-      ok = whole ? step(j, std::false_type{}) : step(j, std::true_type{});
+      const bool whole = !wide && e0 + 4 <= it.je && tz <= first.hi && (ta >= fin.lo || tz <= first.kept);
+      ok = whole ? step(j, wide, std::false_type{}) : step(j, wide, std::true_type{});
+      if (!ok) break;
     }
     const bool done = ok && nkv > 0 && poll_wait_warp(&bars[GEO::bOFinal + x], 0, abort, a.status, lim);
     if (it.parts > 1) {
@@ -456,11 +524,20 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         }
         if (j < nkv) {
           const uint32_t dst = tiles + ks * kKVTile;
+          int any = 0;
 #pragma unroll 2
           for (int p = 0; p < rows; p += 8) {
             const int r = r0 + p, e = it.jb + 4 * j + (r >> 4);
             const bool live = e < it.je && it.block_at(e) * kBlock + (r & 15) < it.kv_len;
-            conv.row(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, dst, r, t, live);
+            const int x = conv.row(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, dst, r, t, live);
+            if (!is_v) {
+              any |= x;
+              if (t == 0) smem[GEO::kOffExp + (j % GEO::kExp) * BN + r] = static_cast<uint8_t>(x);
+            }
+          }
+          if (!is_v) {
+            any = __any_sync(0xffffffffu, any != 0);
+            if (lane == 0) smem[GEO::kOffWide + 4 * (j % GEO::kExp) + r0 / rows] = static_cast<uint8_t>(any);
           }
         }
         const int jn = j + 1;
@@ -482,12 +559,10 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     uint64_t* const ld_full = bars + GEO::bLdFull + (is_v ? LK : 0);
     uint64_t* const ld_empty = bars + GEO::bLdEmpty + (is_v ? LK : 0);
     uint64_t* const kv_empty = bars + GEO::bKvEmpty + (is_v ? NK : 0);
-    // one copy of the loop where K and V have the same format: the instruction caches
-    // hold four different loops per sub-partition as it is
-    if (KB == VB || !is_v)
-      convert(Converter<L, KB>{}, codes, dst, is_v ? LV : LK, is_v ? NV : NK, ld_full, ld_empty, kv_empty, GEO::kRecK, GEO::kStageK);
+    if (!is_v)
+      convert(Converter<L, KB, true>{}, codes, dst, LK, NK, ld_full, ld_empty, kv_empty, GEO::kRecK, GEO::kStageK);
     else
-      convert(Converter<L, VB>{}, codes, dst, LV, NV, ld_full, ld_empty, kv_empty, GEO::kRecV, GEO::kStageV);
+      convert(Converter<L, VB, false>{}, codes, dst, LV, NV, ld_full, ld_empty, kv_empty, GEO::kRecV, GEO::kStageV);
   } else if (warp == kProdWarp || warp == kProdWarpV) {
     // ------------------------------------------------------------ producers
     const bool pv = warp != kProdWarp;
@@ -517,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     // ------------------------------------------------------------ MMA issuers
     const int x = warp - kMmaWarp;
     if (lane == 0 && x < nq) {
-      constexpr uint32_t idS = idesc_bf16(BM, BN, 0);
+      constexpr uint32_t idS = idesc_f16(BM, BN);
       constexpr uint32_t idPV = idesc_bf16(BM, D, 1);
       const uint32_t tS0 = tmem + kColS + 128 * x, tO = tmem + kColO + 128 * x;
       // descriptors address shared memory in units of 16 bytes

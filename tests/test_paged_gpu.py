@@ -426,3 +426,40 @@ def test_cuda_graph():
         a = out.clone()
         cache.append(k, v, batch)
         assert torch.equal(paged.attention(x, cache, batch), a)
+
+
+@pytest.mark.parametrize("q", [1, 12, 150])
+@pytest.mark.parametrize("k_bits,v_bits,mode", [(4, 4, "blind32"), (8, 8, "bands4")])
+def test_magnitudes_beyond_half_precision(q, k_bits, v_bits, mode):
+    """Keys, values and queries whose magnitudes pass 65504 or are tiny, in some tokens and
+    rows and not in others; logits stay moderate through softmax_scale."""
+    n = 300
+    cache, batch, table = make([n], [q], heads=1, page=32, k_bits=k_bits, v_bits=v_bits, mode=mode)
+    whole = paged.PagedBatch(table, [n], [n], 32, device="cuda:0")
+    for ks, vs, qs in ((1e6, 1.0, 1e-6), (1.0, 1e7, 1.0), (1e-5, 1e-6, 1e5), (1e12, 1e-3, 1e-12), (1e-3, 1e30, 1e6)):
+        kk, vv = rows_of(n, 1, 3, ks), rows_of(n, 1, 4, vs)
+        kk[::3] *= 1e-3
+        vv[1::4] *= 1e-3
+        x = (torch.randn(q, 4, 128) * qs).bfloat16()
+        x[::2] *= 0.25
+        cache.append(kk.cuda(), vv.cuda(), whole)
+        k, v = stored(kk, k_bits, cache.bands), stored(vv, v_bits, cache.bands)
+        check(x.cuda(), cache, batch, k, v, scale=0.09 / (ks * qs))
+
+
+def test_huge_tokens_do_not_touch_rows_that_do_not_see_them():
+    """Tokens past the range of half precision, between others of the same storage block."""
+    n, q = 200, 150
+    cache, batch, table = make([n], [q], heads=1)
+    whole = paged.PagedBatch(table, [n], [n], 16, device="cuda:0")
+    kk, vv = rows_of(n, 1, 3), rows_of(n, 1, 4)
+    x = torch.randn(q, 4, 128).bfloat16().cuda()
+    cache.append(kk.cuda(), vv.cuda(), whole)
+    a = paged.attention(x, cache, batch)
+    kk[120] *= 1e6
+    vv[123] *= 1e9
+    cache.append(kk.cuda(), vv.cuda(), whole)
+    b = paged.attention(x, cache, batch)
+    assert torch.equal(a[:70], b[:70])  # positions 50..119
+    k, v = stored(kk, 4, cache.bands), stored(vv, 4, cache.bands)
+    check(x, cache, batch, k, v, scale=0.09e-6)
