@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cmath>
+
 #include "kvq_paged.cuh"
 #include "kvq_sm100.cuh"
 
@@ -80,23 +82,17 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
                                    *reinterpret_cast<__nv_bfloat162*>(&c));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// int4 codes (code = q + 8) at bits 0-3 and 16-19, or 4-7 and 20-23, of a word -> bf16x2
-// (q / 4, q / 4), exact, one logic operation and one FMA each and no shift:
-//   low   ored into the mantissa of 128: 128 + code, times 1/4, minus 34;
-//   high  bits 4-7 of a bf16 are its lowest exponent bit and the top of its mantissa, and
-//         a bf16 with that exponent or none is linear in its bits: code * 2^-129, times
-//         2^127, minus 2.
-// With four times the scale the product is q * s, rounded once.
 // (x & m) | o as one instruction: from the C expression the compiler made two.
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t o) {
   uint32_t y;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(m), "r"(o));
   return y;
 }
+// int4 codes (code = q + 8) at bits 0-3 and 16-19 of a word -> bf16x2 (q / 4, q / 4), exact:
+// 128 + code, times 1/4, minus 34. With four times the scale the product is q * s, rounded once.
 __device__ __forceinline__ uint32_t int4_low(uint32_t x) {
   return hfma2(and_or(x, 0x000F000Fu, 0x43004300u), 0x3E803E80u, 0xC208C208u);
 }
-__device__ __forceinline__ uint32_t int4_high(uint32_t x) { return hfma2(x & 0x00F000F0u, 0x7F007F00u, 0xC000C000u); }
 constexpr uint32_t kFour = 0x40804080u;  // bf16x2 (4, 4)
 // Bytes at bits 0-7 and 16-23 (code = q + 128) -> bf16x2 (q, q). The low seven bits give
 // 128 + code % 128, from which 256 is taken, or 128 where the top bit is set.
@@ -106,13 +102,14 @@ __device__ __forceinline__ uint32_t int8_pair(uint32_t x) {
   return hsub2(and_or(x, 0x007F007Fu, 0x43004300u), d);
 }
 
-// Keys, and the queries they meet, are multiplied as fp16 rather than bf16: an int4 code
-// times a bf16 scale has eleven significant bits, which fp16 holds and bf16 rounds to
-// eight (that rounding, on the logits, was most of the output's error). fp16 ends at 65504
-// and thins out below 2^-14, so a token whose largest key scale lies beyond
-// [kKeyScaleLeast, kKeyScaleMost] is multiplied as if its scales were 2^-e times as large,
-// and a query row likewise; the logits get the power of two back in fp32, which changes
-// no other row's or token's bits.
+// The attention multiplies in fp16 rather than bf16: an int4 code times a bf16 scale has
+// eleven significant bits, which fp16 holds and bf16 rounds to eight; with bf16 products
+// the output's error against 64 bits was 3.7e-3, of which the rounding of the output is
+// 1.7e-3. fp16 ends at 65504 and thins out below 2^-14, so a token whose largest key or
+// value scale lies beyond [kScaleLeast, kScaleMost] is multiplied as if its scales were
+// 2^-e times as large, and a query row likewise: logits get the power of two back in
+// fp32, softmax weights get a value's, relative to a power of two F that each output row
+// keeps for itself. Tokens and rows that have none keep their bits.
 __device__ __forceinline__ uint32_t h16mul2(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
@@ -141,18 +138,18 @@ __device__ __forceinline__ uint32_t int4_high_f16(uint32_t x) {
 __device__ __forceinline__ uint32_t int8_pair_f16(uint32_t x) {
   return h16add2(and_or(x, 0x00FF00FFu, 0x64006400u), 0xE480E480u);
 }
-constexpr uint32_t kKeyScaleLeast = 0x3880, kKeyScaleMost = 0x4400;  // bf16 2^-14, 512 (127 * 512 < 65504)
+constexpr uint32_t kScaleLeast = 0x3880, kScaleMost = 0x4400;  // bf16 2^-14, 512 (127 * 512 < 65504)
 constexpr uint32_t kQueryLeast = 0x3B80, kQueryMost = 0x4700;        // bf16 2^-8, 2^15
 // bits of a bf16 >= 0 outside [least, most]
 __device__ __forceinline__ bool beyond(uint32_t bits, uint32_t least, uint32_t most) { return bits - least > most - least; }
 // 2^e, |e| <= 126
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
-// The exponent to take out of a token whose largest scale has these bits, of a query row
+// Exponents to take out of a token whose largest scale has these bits, and of a query row
 // whose largest magnitude has: to [256, 512) and [2^14, 2^15) above, to [1, 2) below.
-__device__ __forceinline__ int key_exponent(uint32_t bits) {
-  if (bits == 0 || !beyond(bits, kKeyScaleLeast, kKeyScaleMost)) return 0;
+__device__ __forceinline__ int scale_exponent(uint32_t bits) {
+  if (bits == 0 || !beyond(bits, kScaleLeast, kScaleMost)) return 0;
   const int e = static_cast<int>(bits >> 7) - 127;
-  return bits > kKeyScaleMost ? min(e - 8, 119) : max(e, -110);
+  return bits > kScaleMost ? min(e - 8, 119) : max(e, -110);
 }
 __device__ __forceinline__ int query_exponent(uint32_t bits) {
   if (bits == 0 || !beyond(bits, kQueryLeast, kQueryMost)) return 0;
@@ -170,6 +167,14 @@ __device__ __forceinline__ uint32_t most_of(const uint4& v) {
     m = max(m, hi < 0x7F80u ? hi : 0u);
   }
   return m;
+}
+// The F of an output row once a weight times its value's power of two has been 2^top, given
+// F so far; a row that has seen nothing yet (fresh) may take a lower one than 0. Leaves
+// room below fp16's end; 0 where that does, so that ordinary rows end up there.
+__device__ __forceinline__ float next_f(float f, float top, bool fresh) {
+  const float need = ceilf(top) - 14.0f;
+  const float n = fresh ? need : fmaxf(f, need);
+  return top == -INFINITY ? f : (n > -15.0f && n < 0.0f ? 0.0f : n);
 }
 // Eight bf16 times 2^-e -> fp16 (exact for normal results).
 __device__ __forceinline__ uint4 to_f16(const uint4& v, int e) {

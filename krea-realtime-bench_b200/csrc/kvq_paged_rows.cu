@@ -16,8 +16,9 @@
 // the dequantized tile in shared memory (2 x 256 bytes per row through the shared-
 // memory port, more than it moves at memory speed); mma.sync takes it from registers.
 // Codes become values in registers, two per instruction: code bits are ored into the
-// mantissa of bf16 128 and the offset subtracted (exact), then times the bf16 scale
-// with one rounding, the value that kvq_paged_read returns. The order of channels and
+// mantissa of fp16 1024 and the offset subtracted (exact), then times the scale, exact for
+// int4; see kScaleLeast for what fp16 does not hold. p is rounded to fp16, S, m, l and O
+// are fp32. The order of channels and
 // of tokens inside a fragment is free as long as A and B agree: lane (g, t) = (lane /
 // 4, lane % 4) holds channels 32t..32t+31 of K rows and channels 16g..16g+15 of V
 // rows, 8 or 16 contiguous bytes of shared memory.
@@ -51,13 +52,6 @@ struct RowGeo {
 };
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                         uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma16816_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -205,7 +199,8 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
     const Seen first = seen_by(a, it.start + it.row0 / a.group, it.kv_len);
     const Seen final_ = seen_by(a, it.start + (it.row0 + it.n_rows - 1) / a.group, it.kv_len);
 
-    float o[NT][8][4], m[NT][2], l[NT][2];
+    float o[NT][8][4], m[NT][2], l[NT][2], F[NT][2];  // O is kept divided by 2^F
+    bool f_any = false;                               // whether any row's F is not 0
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -213,7 +208,7 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.0f;
       m[nt][0] = m[nt][1] = -1.0e30f;
-      l[nt][0] = l[nt][1] = 0.0f;
+      l[nt][0] = l[nt][1] = F[nt][0] = F[nt][1] = 0.0f;
     }
 
     for (int k = 0; k < n_mine; ++k) {
@@ -265,16 +260,16 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
 #pragma unroll
           for (int q = 0; q < KG; ++q) kscale[r][q] = __uint_as_float(x[q] << 16);
         }
-        // rare: a token whose scales leave fp16's range (kKeyScaleLeast, kKeyScaleMost)
-        const bool wide = __any_sync(0xffffffffu, beyond(kx[0], kKeyScaleLeast, kKeyScaleMost) ||
-                                                      beyond(kx[1], kKeyScaleLeast, kKeyScaleMost));
+        // rare: a token whose scales leave fp16's range (kScaleLeast, kScaleMost)
+        const bool wide = __any_sync(0xffffffffu, beyond(kx[0], kScaleLeast, kScaleMost) ||
+                                                      beyond(kx[1], kScaleLeast, kScaleMost));
         float back[2];
         if (wide) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             kx[r] = max(kx[r], __shfl_xor_sync(0xffffffffu, kx[r], 1));
             kx[r] = max(kx[r], __shfl_xor_sync(0xffffffffu, kx[r], 2));
-            const int e = key_exponent(kx[r]);
+            const int e = scale_exponent(kx[r]);
             back[r] = pow2i(e);
 #pragma unroll
             for (int q = 0; q < KG; ++q) kscale[r][q] *= pow2i(-e);
@@ -307,7 +302,7 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816_f16(s[nt][bb], f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], qf[nt][2 * w + h][0],
+              mma16816(s[nt][bb], f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], qf[nt][2 * w + h][0],
                            qf[nt][2 * w + h][1]);
         }
         if (wide) {
@@ -318,8 +313,59 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
         }
       }
 
+      // ---- V's scales, of this lane's tokens: S rows 2t, 2t + 1, 8 + 2t, 9 + 2t
+      uint32_t vs[2][2][VG];
+      bool wide_v = false;
+      float ve[2][2];  // where wide_v: exponents taken out of the tokens of S rows g, 8 + g
+#pragma unroll
+      for (int bb = 0; bb < 2; ++bb) {
+        uint32_t x[4][VG], most[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t from = ((u & 1) ? v_scales1 : v_scales0) + at + bb * (GEO::kStage / 2) + (u >> 1) * 8 * G * 2;
+#pragma unroll
+          for (int q = 0; q < VG; ++q) {
+            x[u][q] = ld_shared_u16(from + 2 * (VG == 1 ? vbase : min(vbase + q, G - 1)));
+            // rows past the end hold anything: as zeros they add nothing
+            if (!whole && ((bb ? tz : ta) + ((u & 1) ? vt1 : vt0) + (u >> 1) * 8 >= it.kv_len || (bb && !two))) x[u][q] = 0;
+            most[u] = max(most[u], x[u][q]);
+          }
+        }
+        float f[4][VG];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int q = 0; q < VG; ++q) f[u][q] = __uint_as_float(x[u][q] << 16);
+        ve[bb][0] = ve[bb][1] = 0.0f;
+        const uint32_t hi = max(max(most[0], most[1]), max(most[2], most[3]));
+        const uint32_t lo = min(min(most[0], most[1]), min(most[2], most[3]));
+        if (__any_sync(0xffffffffu, hi > kScaleMost || lo < kScaleLeast)) {
+          int e[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) most[u] = max(most[u], __shfl_xor_sync(0xffffffffu, most[u], d));
+            e[u] = scale_exponent(most[u]);
+#pragma unroll
+            for (int q = 0; q < VG; ++q) f[u][q] *= pow2i(-e[u]);
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int ea = __shfl_sync(0xffffffffu, e[2 * r], g >> 1), eb = __shfl_sync(0xffffffffu, e[2 * r + 1], g >> 1);
+            ve[bb][r] = static_cast<float>((g & 1) ? eb : ea);
+          }
+          wide_v = __any_sync(0xffffffffu, ve[bb][0] != 0.0f || ve[bb][1] != 0.0f) || wide_v;
+        }
+#pragma unroll
+        for (int q = 0; q < VG; ++q) {
+          vs[bb][0][q] = pack_f16x2(f[0][q], f[1][q]);
+          vs[bb][1][q] = pack_f16x2(f[2][q], f[3][q]);
+        }
+      }
+
       // ---- softmax weights
       uint32_t pf[NT][2][2];
+      bool fresh[NT][2];  // rows that have seen nothing yet
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if (!whole) {
@@ -334,6 +380,8 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
         }
         const float mx0 = fmaxf(fmaxf(s[nt][0][0], s[nt][0][2]), fmaxf(s[nt][1][0], s[nt][1][2])) * sc[nt][0];
         const float mx1 = fmaxf(fmaxf(s[nt][0][1], s[nt][0][3]), fmaxf(s[nt][1][1], s[nt][1][3])) * sc[nt][1];
+        fresh[nt][0] = m[nt][0] < -1.0e29f;
+        fresh[nt][1] = m[nt][1] < -1.0e29f;
         if (__any_sync(0xffffffffu, mx0 > m[nt][0] + 8.0f || mx1 > m[nt][1] + 8.0f)) {
           float n0 = mx0, n1 = mx1;
 #pragma unroll
@@ -363,16 +411,51 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           for (int e = 0; e < 4; ++e) p[e] = ex2f(fmaf(s[nt][bb][e], sc[nt][e & 1], -m[nt][e & 1]));
           l[nt][0] += p[0] + p[2];
           l[nt][1] += p[1] + p[3];
-          pf[nt][bb][0] = transpose8x8(pack_bf16x2(p[0], p[1]));
-          pf[nt][bb][1] = transpose8x8(pack_bf16x2(p[2], p[3]));
+          pf[nt][bb][0] = transpose8x8(pack_f16x2(p[0], p[1]));
+          pf[nt][bb][1] = transpose8x8(pack_f16x2(p[2], p[3]));
+        }
+      }
+      if (wide_v || f_any) {
+        f_any = false;
+        // weights times the powers of two taken out of the values, relative to 2^F, in log2:
+        // y = s * scale - m + e. F grows where 2^(y - F) would leave fp16.
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int bb = 0; bb < 2; ++bb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s[nt][bb][e] = fmaf(s[nt][bb][e], sc[nt][e & 1], -m[nt][e & 1]) + ve[bb][e >> 1];
+              top[e & 1] = fmaxf(top[e & 1], s[nt][bb][e]);
+            }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], d));
+            const float Fn = next_f(F[nt][i], top[i], fresh[nt][i]);
+            const float back = ex2f(F[nt][i] - Fn);
+            F[nt][i] = Fn;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              o[nt][c][i] *= back;
+              o[nt][c][2 + i] *= back;
+            }
+          }
+#pragma unroll
+          for (int bb = 0; bb < 2; ++bb)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              pf[nt][bb][r] = transpose8x8(pack_f16x2(ex2f(s[nt][bb][2 * r] - F[nt][0]), ex2f(s[nt][bb][2 * r + 1] - F[nt][1])));
+          f_any = __any_sync(0xffffffffu, F[nt][0] != 0.0f || F[nt][1] != 0.0f) || f_any;
         }
       }
 
-      // ---- O^T: this lane's tokens are S rows 2t, 2t + 1, 8 + 2t, 9 + 2t
+      // ---- O^T
 #pragma unroll
       for (int bb = 0; bb < 2; ++bb) {
         const uint32_t off = at + bb * (GEO::kStage / 2);
-        uint32_t vw[4][VB == 4 ? 2 : 4], vs[2][VG];
+        uint32_t vw[4][VB == 4 ? 2 : 4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const uint32_t src = ((u & 1) ? v_codes1 : v_codes0) + off + (u >> 1) * 8 * Rec<L, VB>::CW;
@@ -389,40 +472,23 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           }
         }
 #pragma unroll
-        for (int q = 0; q < VG; ++q) {
-          uint32_t x[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const uint32_t sc = ((u & 1) ? v_scales1 : v_scales0) + off + (u >> 1) * 8 * G * 2;
-            x[u] = ld_shared_u16(sc + 2 * (VG == 1 ? vbase : min(vbase + q, G - 1)));
-            // rows past the end hold anything: as zeros they add nothing
-            if (!whole && ((bb ? tz : ta) + ((u & 1) ? vt1 : vt0) + (u >> 1) * 8 >= it.kv_len || (bb && !two))) x[u] = 0;
-          }
-          vs[0][q] = __byte_perm(x[0], x[1], 0x5410);
-          vs[1][q] = __byte_perm(x[2], x[3], 0x5410);
-          if constexpr (VB == 4) {  // for q / 4
-            vs[0][q] = hmul2(vs[0][q], kFour);
-            vs[1][q] = hmul2(vs[1][q], kFour);
-          }
-        }
-#pragma unroll
         for (int i = 0; i < 8; ++i) {  // channels 16g + 2i (rows g) and 16g + 2i + 1 (rows 8 + g)
           uint32_t f[2][2];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            uint32_t sp = vs[u][0];
-            if (VG > 1) sp = i >= ve1 ? vs[u][VG > 1 ? 1 : 0] : sp;
-            if (VG > 2) sp = i >= ve2 ? vs[u][VG > 2 ? 2 : 0] : sp;
+            uint32_t sp = vs[bb][u][0];
+            if (VG > 1) sp = i >= ve1 ? vs[bb][u][VG > 1 ? 1 : 0] : sp;
+            if (VG > 2) sp = i >= ve2 ? vs[bb][u][VG > 2 ? 2 : 0] : sp;
             if constexpr (VB == 4) {
               const int b = i & 3;  // the byte with both channels, of either token
               const uint32_t x = __byte_perm(vw[2 * u][i >> 2], vw[2 * u + 1][i >> 2], b | b << 4 | (4 + b) << 8 | (4 + b) << 12);
-              f[u][0] = hmul2(int4_low(x), sp);
-              f[u][1] = hmul2(int4_high(x), sp);
+              f[u][0] = h16mul2(int4_low_f16(x), sp);
+              f[u][1] = h16mul2(int4_high_f16(x), sp);
             } else {
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int c = 2 * i + e, b = c & 3;
-                f[u][e] = hmul2(int8_pair(__byte_perm(vw[2 * u][c >> 2], vw[2 * u + 1][c >> 2],
+                f[u][e] = h16mul2(int8_pair_f16(__byte_perm(vw[2 * u][c >> 2], vw[2 * u + 1][c >> 2],
                                                       b | b << 4 | (4 + b) << 8 | (4 + b) << 12)), sp);
               }
             }
@@ -450,10 +516,12 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           sm_ml[(warp * kRows + n) * 2] = m[nt][e];
           sm_ml[(warp * kRows + n) * 2 + 1] = x;
         }
+        const float of = ex2f(F[nt][e]);
         float4* dst = reinterpret_cast<float4*>(mine + n * D + 16 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          dst[i] = make_float4(o[nt][2 * i][e], o[nt][2 * i][2 + e], o[nt][2 * i + 1][e], o[nt][2 * i + 1][2 + e]);
+          dst[i] = make_float4(o[nt][2 * i][e] * of, o[nt][2 * i][2 + e] * of, o[nt][2 * i + 1][e] * of,
+                               o[nt][2 * i + 1][2 + e] * of);
       }
     }
     __syncthreads();

@@ -8,7 +8,7 @@
 //   warps 0-3 / 4-7  softmax of Q tile 0 / 1: thread r owns row r (TMEM lane r); all
 //                    eight first gather the Q rows (cp.async into the MMA's layout)
 //   warps 8-9/10-11  converters of K / V: four lanes per row, 32 channels each, codes and
-//                    scales from the staged records to 128B-swizzled bf16 tiles
+//                    scales from the staged records to 128B-swizzled fp16 tiles
 //   warps 12 / 15    producers of K / V: a storage block is contiguous, one bulk copy
 //   warps 13 / 14    one thread each issuing the tcgen05.mma of Q tile 0 / 1:
 //                    S_x = Q_x K^T (M128 N64 K128), O_x += P_x V (M128 N128 K64, P in TMEM)
@@ -18,8 +18,8 @@
 // of sight. A tile that some row of the Q tile does not see whole takes a masked step
 // (a 64-bit mask per row; a masked logit is -inf); the running maximum starts at -1e30,
 // so a row without any visible token ends with l = 0 and is stored as 0.
-// Roundings: K and Q as fp16 for S (exact for int4 codes; see kKeyScaleMost), P and V as
-// bf16 for PV (V as kvq_paged_read returns it); S, m, l, O are fp32.
+// Roundings: Q, K, V and P are fp16 for the MMAs (K and V exact for int4 codes; see
+// kScaleLeast); S, m, l, O are fp32.
 #include <cmath>
 
 #include "kvq_paged_dev.cuh"
@@ -38,9 +38,9 @@ constexpr int kAtom = BN * 128;
 constexpr int kQTile = BM * D * 2;
 constexpr int kQAtom = BM * 128;
 
-// Shared memory: bf16 stages of K and V, staged records, the Q tiles. Four bf16
+// Shared memory: fp16 stages of K and V, staged records, the Q tiles. Four fp16
 // stages per tensor and three staged tiles where the codes are small; int8 codes leave
-// room for two, and with both tensors int8 for three bf16 stages of V.
+// room for two, and with both tensors int8 for three fp16 stages of V.
 template <class L, int KB, int VB>
 struct Geo {
   static constexpr int kRecK = Rec<L, KB>::kBytes, kRecV = Rec<L, VB>::kBytes;
@@ -56,17 +56,19 @@ struct Geo {
   static constexpr int kOffCV = kOffCK + LK * kStageK;
   static constexpr int kOffBar = (kOffCV + LV * kStageV + 15) / 16 * 16;
   // barriers; index + stages of K for V
-  static constexpr int bLdFull = 0, bLdEmpty = bLdFull + LK + LV, bK01 = bLdEmpty + LK + LV, bReady = bK01 + 2,
+  static constexpr int bLdFull = 0, bLdEmpty = bLdFull + LK + LV, bReady = bLdEmpty + LK + LV,
                        bKvEmpty = bReady + kReady, bQReady = bKvEmpty + NK + NV, bSFull = bQReady + 2,
                        bPFull = bSFull + 4, bOReady = bPFull + 4, bOFinal = bOReady + 2, bMmaDone = bOFinal + 2,
                        kNumBars = bMmaDone + 2;
   static constexpr int kOffMisc = (kOffBar + kNumBars * 8 + 15) / 16 * 16;
-  // of the last kExp key tiles: the exponent taken out of each token, and a byte per
-  // converter warp that says whether there is any. A tile's are written again only after
-  // S(j + kExp - 4) has completed, behind P(j + kExp - 6) of every softmax warp.
-  static constexpr int kExp = 6;
-  static constexpr int kOffExp = kOffMisc + 32, kOffWide = kOffExp + kExp * BN;
-  static constexpr int kSmemBytes = kOffWide + 4 * kExp + 1024;  // + alignment slack
+  // Of the last kExpK key tiles and kExpV value tiles: the exponent taken out of each token,
+  // and a byte per converter warp that says whether there is any. K's of a tile are written
+  // again only after S(j + kExpK - 4), V's after S(j + 2), each issued behind P(j) of
+  // every softmax warp.
+  static constexpr int kExpK = 6, kExpV = 4;
+  static constexpr int kOffExpK = kOffMisc + 32, kOffExpV = kOffExpK + kExpK * BN;
+  static constexpr int kOffWideK = kOffExpV + kExpV * BN, kOffWideV = kOffWideK + 4 * kExpK;
+  static constexpr int kSmemBytes = kOffWideV + 4 * kExpV;
   static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM must fit");
   static_assert(kOffCK % 16 == 0 && kOffCV % 16 == 0, "bulk copies");
 };
@@ -83,8 +85,8 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
-// Converters: four lanes per row, lane t channels 32t..32t+31. Keys to fp16, values to bf16.
-template <class L, int BITS, bool KEY>
+// Converters: four lanes per row, lane t channels 32t..32t+31.
+template <class L, int BITS>
 struct Converter {
   static constexpr int KG = most_groups<L, 32>();
   int base;
@@ -102,8 +104,8 @@ struct Converter {
       }
     }
   }
-  // One row: record block `rec`, row `rr` of it, to row r of the tile at dst. For keys
-  // returns the exponent taken out of the row (kKeyScaleMost).
+  // One row: record block `rec`, row `rr` of it, to row r of the tile at dst. Returns the
+  // exponent taken out of the row (kScaleLeast, kScaleMost).
   __device__ __forceinline__ int row(uint32_t rec, int rr, uint32_t dst, int r, int t, bool live) const {
     using R = Rec<L, BITS>;
     uint32_t w[BITS];  // 4 or 8 words of codes
@@ -125,28 +127,19 @@ struct Converter {
     }
     uint32_t s01, s23 = 0;
     int e = 0;
-    if constexpr (KEY) {
-      float f[4];
+    float f[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) f[q] = __uint_as_float(x[q] << 16);
-      uint32_t most = max(max(x[0], x[1]), max(x[2], x[3]));
-      if (__any_sync(0xffffffffu, beyond(most, kKeyScaleLeast, kKeyScaleMost))) {
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        e = key_exponent(most);
+    for (int q = 0; q < 4; ++q) f[q] = __uint_as_float(x[q] << 16);
+    uint32_t most = max(max(x[0], x[1]), max(x[2], x[3]));
+    if (__any_sync(0xffffffffu, beyond(most, kScaleLeast, kScaleMost))) {
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      e = scale_exponent(most);
 #pragma unroll
-        for (int q = 0; q < KG; ++q) f[q] *= pow2i(-e);
-      }
-      s01 = pack_f16x2(f[0], f[KG == 1 ? 0 : 1]);
-      if constexpr (KG > 2) s23 = pack_f16x2(f[2], f[3]);
-    } else {
-      s01 = KG == 1 ? x[0] * 0x10001u : __byte_perm(x[0], x[1], 0x5410);
-      if constexpr (KG > 2) s23 = __byte_perm(x[2], x[3], 0x5410);
-      if constexpr (BITS == 4) {  // for q / 4
-        s01 = hmul2(s01, kFour);
-        if constexpr (KG > 2) s23 = hmul2(s23, kFour);
-      }
+      for (int q = 0; q < KG; ++q) f[q] *= pow2i(-e);
     }
+    s01 = pack_f16x2(f[0], f[KG == 1 ? 0 : 1]);
+    if constexpr (KG > 2) s23 = pack_f16x2(f[2], f[3]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int hi = t & 2;  // word i ^ hi
@@ -156,20 +149,20 @@ struct Converter {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t b = __byte_perm(v, y, (4 + j) << 8 | j);
-          o[j] = KEY ? int4_low_f16(b) : int4_low(b);
+          o[j] = int4_low_f16(b);
         }
       } else {
         const uint32_t v = hi ? w[2 * (i ^ 2)] : w[2 * i], y = hi ? w[2 * (i ^ 2) + 1] : w[2 * i + 1];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t b = __byte_perm(j < 2 ? v : y, 0, (j & 1) ? 0x4342 : 0x4140);
-          o[j] = KEY ? int8_pair_f16(b) : int8_pair(b);
+          o[j] = int8_pair_f16(b);
         }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t sp = KG == 1 ? s01 : __byte_perm(s01, s23, sel[KG == 1 ? 0 : 4 * i + j]);
-        o[j] = KEY ? h16mul2(o[j], sp) : hmul2(o[j], sp);
+        o[j] = h16mul2(o[j], sp);
       }
       st_shared_v4(dst + tile_off(r, 4 * t + (i ^ hi)), o[0], o[1], o[2], o[3]);
     }
@@ -177,16 +170,21 @@ struct Converter {
   }
 };
 
-// idesc_bf16 of the S product with fp16 for both operands.
-__host__ __device__ constexpr uint32_t idesc_f16(int m, int n) { return idesc_bf16(m, n, 0) & ~((7u << 7) | (7u << 10)); }
+// idesc_bf16 with fp16 for both operands.
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, int b_mn_major) {
+  return idesc_bf16(m, n, b_mn_major) & ~((7u << 7) | (7u << 10));
+}
 
 template <class L, int KB, int VB>
 __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constant__ AttnArgs a) {
   using GEO = Geo<L, KB, VB>;
   constexpr int NK = GEO::NK, NV = GEO::NV, LK = GEO::LK, LV = GEO::LV;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
+  if (sbase & 1023) {  // the swizzled tiles need it
+    if (threadIdx.x == 0) atomicExch(a.status, kDevTimeout);
+    return;
+  }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + GEO::kOffBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + GEO::kOffMisc);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + GEO::kOffMisc + 8);
@@ -284,7 +282,6 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     for (int i = 0; i < NK + NV; ++i) mbar_init(&bars[GEO::bKvEmpty + i], nq);
     for (int i = 0; i < GEO::kReady; ++i) mbar_init(&bars[GEO::bReady + i], 2 * n_conv);
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&bars[GEO::bK01 + x], n_conv);
       mbar_init(&bars[GEO::bQReady + x], 8);  // the eight gathering warps
       mbar_init(&bars[GEO::bSFull + 2 * x], 1);
       mbar_init(&bars[GEO::bSFull + 2 * x + 1], 1);
@@ -295,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       mbar_init(&bars[GEO::bMmaDone + x], 1);
     }
     *abort = 0;
-    for (int i = 0; i < GEO::kExp; ++i) *reinterpret_cast<uint32_t*>(smem + GEO::kOffWide + 4 * i) = 0;
+    for (int i = 0; i < GEO::kExpK + GEO::kExpV; ++i) *reinterpret_cast<uint32_t*>(smem + GEO::kOffWideK + 4 * i) = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -327,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     const Seen see = seen_by(a, it.start + (it.row0 + min(n, it.n_rows - 1)) / a.group, it.kv_len);
     const Seen first = seen_by(a, it.start + (it.row0 + x * BM) / a.group, it.kv_len);
     const Seen fin = seen_by(a, it.start + (it.row0 + n_last) / a.group, it.kv_len);
-    float m = -1.0e30f, l = 0.0f;
+    float m = -1.0e30f, l = 0.0f, F = 0.0f;  // O is kept divided by 2^F
     bool ok = true, s_ready = false;  // s_ready: S of the coming tile was already found complete
     // this row's softmax scale, with the power of two taken out of its query
     float row_scale = a.scale_log2;
@@ -341,14 +338,14 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       for (int c = 0; c < 16; ++c) most = max(most, most_of(ld_global_nc_v4(src + c)));
       row_scale *= pow2i(query_exponent(most));
     }
-    auto step = [&](const int j, const bool wide, auto masked) -> bool {
+    auto step = [&](const int j, const bool wide_k, const bool wide_v, auto masked) -> bool {
       constexpr bool MASK = decltype(masked)::value;
       const uint32_t tS = tS0 + 64 * (j & 1);
       uint32_t s0[32], s1[32];
       tmem_ld32x2_wait(tS, tS + 32, s0, s1);
       if constexpr (MASK) {
-        if (wide) {  // powers of two taken out of the tile's tokens
-          const uint32_t at = sbase + GEO::kOffExp + (j % GEO::kExp) * BN;
+        if (wide_k) {  // powers of two taken out of the tile's keys
+          const uint32_t at = sbase + GEO::kOffExpK + (j % GEO::kExpK) * BN;
 #pragma unroll
           for (int c = 0; c < 32; c += 16) {
             const uint4 u = ld_shared_v4(at + c), v = ld_shared_v4(at + 32 + c);
@@ -385,6 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       const float mt =
           fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * row_scale;
       bool rescale = false;
+      const bool fresh = m < -1.0e29f;
       float alpha = 1.0f;
       if (j == 0) {
         m = fmaxf(m, mt);
@@ -395,6 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         l *= alpha;
       }
       const float nm = -m;
+      float alpha_o = alpha;
       uint32_t pw[32];
       const float2 sc2 = make_float2(row_scale, row_scale), nm2 = make_float2(nm, nm);
       float2 sum2 = make_float2(0.0f, 0.0f);
@@ -405,12 +404,52 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
               __ffma2_rn(make_float2(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), sc2, nm2);
           const float p0 = ex2f(xx.x), p1 = ex2f(xx.y);
           sum2 = __fadd2_rn(sum2, make_float2(p0, p1));
-          pw[base / 2 + c] = pack_bf16x2(p0, p1);
+          pw[base / 2 + c] = pack_f16x2(p0, p1);
         }
       };
       half(s0, 0);
-      tmem_st16(tS, pw);
-      half(s1, 32);
+      if constexpr (MASK) {
+        half(s1, 32);
+        if (__any_sync(0xffffffffu, wide_v || F != 0.0f)) {
+          // weights times the powers of two taken out of the values, relative to 2^F, in
+          // log2: y = s * scale - m + e. F grows where 2^(y - F) would leave fp16.
+          const uint32_t at = sbase + GEO::kOffExpV + (j % GEO::kExpV) * BN;
+          auto exps_of = [&](int c, float (&e)[16]) {
+            const uint4 u = wide_v ? ld_shared_v4(at + c) : make_uint4(0, 0, 0, 0);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) e[i] = static_cast<float>(static_cast<int8_t>(w[i >> 2] >> (8 * (i & 3))));
+          };
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 32; c += 16) {
+            float e0[16], e1[16];
+            exps_of(c, e0);
+            exps_of(32 + c, e1);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              s0[c + i] = __float_as_uint(fmaf(__uint_as_float(s0[c + i]), row_scale, nm) + e0[i]);
+              s1[c + i] = __float_as_uint(fmaf(__uint_as_float(s1[c + i]), row_scale, nm) + e1[i]);
+              top = fmax3(top, __uint_as_float(s0[c + i]), __uint_as_float(s1[c + i]));
+            }
+          }
+          const float Fn = next_f(F, top, fresh);
+          if (Fn != F) {
+            alpha_o *= ex2f(F - Fn);
+            rescale = j > 0;
+            F = Fn;
+          }
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            pw[c] = pack_f16x2(ex2f(__uint_as_float(s0[2 * c]) - F), ex2f(__uint_as_float(s0[2 * c + 1]) - F));
+            pw[16 + c] = pack_f16x2(ex2f(__uint_as_float(s1[2 * c]) - F), ex2f(__uint_as_float(s1[2 * c + 1]) - F));
+          }
+        }
+        tmem_st16(tS, pw);
+      } else {
+        tmem_st16(tS, pw);
+        half(s1, 32);
+      }
       tmem_st16(tS + 16, pw + 16);
       l += sum2.x + sum2.y;
       if (__any_sync(0xffffffffu, rescale)) {
@@ -426,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
           uint32_t o[16];
           tmem_ld16_wait(tO + 16 * k, o);
 #pragma unroll
-          for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+          for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha_o);
           tmem_st16(tO + 16 * k, o);
         }
         tmem_wait_st();
@@ -451,13 +490,16 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         if (j >= 2) mbar_arrive(&bars[GEO::bKvEmpty + NK + (j - 2) % NV]);
       }
       tc_fence_after();
-      const bool wide = *reinterpret_cast<volatile uint32_t*>(smem + GEO::kOffWide + 4 * (j % GEO::kExp)) != 0;
+      const bool wide_k = *reinterpret_cast<volatile uint32_t*>(smem + GEO::kOffWideK + 4 * (j % GEO::kExpK)) != 0;
+      const bool wide_v = *reinterpret_cast<volatile uint32_t*>(smem + GEO::kOffWideV + 4 * (j % GEO::kExpV)) != 0;
       const int e0 = it.jb + 4 * j;
       const int ta = it.block_at(e0) * kBlock, tz = it.block_at(e0 + 3) * kBlock + kBlock;
-      const bool whole = !wide && e0 + 4 <= it.je && tz <= first.hi && (ta >= fin.lo || tz <= first.kept);
-      ok = whole ? step(j, wide, std::false_type{}) : step(j, wide, std::true_type{});
+      const bool whole = e0 + 4 <= it.je && tz <= first.hi && (ta >= fin.lo || tz <= first.kept);
+      ok = __all_sync(0xffffffffu, whole && !wide_k && !wide_v && F == 0.0f) ? step(j, false, false, std::false_type{})
+                                                                             : step(j, wide_k, wide_v, std::true_type{});
       if (!ok) break;
     }
+    const float of = ex2f(F);
     const bool done = ok && nkv > 0 && poll_wait_warp(&bars[GEO::bOFinal + x], 0, abort, a.status, lim);
     if (it.parts > 1) {
       // one part of a unit: unnormalised O row, m and l for the join. float4 column c of
@@ -470,8 +512,8 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         if (done) tmem_ld32_wait(tO + 32 * k, o);
 #pragma unroll
         for (int c = 0; c < 8; ++c)
-          dst[(8 * k + c) * BM] = done ? make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]),
-                                                     __uint_as_float(o[4 * c + 2]), __uint_as_float(o[4 * c + 3]))
+          dst[(8 * k + c) * BM] = done ? make_float4(__uint_as_float(o[4 * c]) * of, __uint_as_float(o[4 * c + 1]) * of,
+                                                     __uint_as_float(o[4 * c + 2]) * of, __uint_as_float(o[4 * c + 3]) * of)
                                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
       dst[32 * BM] = make_float4(m, l, 0.0f, 0.0f);
@@ -479,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     } else if (done || (nkv == 0 && poll_wait_warp(&bars[GEO::bQReady + x], 0, abort, a.status, lim))) {
       // (no tiles: Q_x has landed before its buffer is reused below)
       tc_fence_after();
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float inv = l == 0.0f ? 0.0f : of / l;
       store_lse(n, m, l);
       const uint32_t stage = sbase + GEO::kOffQ + x * kQTile;  // Q_x is no longer read
 #pragma unroll 1
@@ -502,56 +544,44 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     }
   } else if (warp < kProdWarp) {
     // ------------------------------------------------------------ converters
-    // V(j) and K(j+2), the two tiles that the MMAs issued at step j read, count on one
-    // barrier, so an MMA thread waits once: K(j) arrives on barrier j - 2, K(0) and
-    // K(1) on their own. Two steps past its last tile the K side arrives for the tiles that
-    // there are not. A barrier is not reused early: K(j+6) and V(j+4) are converted
-    // only after S(j+2) has completed, which was issued behind a wait for barrier j.
+    // K(j) and V(j) count on one barrier, which the MMA threads wait for before S(j): V a
+    // little early, so that softmax step j finds V's exponents as well as K's. A barrier is
+    // not reused early: K(j+4) and V(j+4) are converted only after S(j) has completed.
     const int is_v = (warp >> 1) & 1;
     const int rows = 64 / n_conv;  // of this warp
     const int t = lane & 3, r0 = ((warp & 1) + (warp < kConvWarp0 ? 2 : 0)) * rows + (lane >> 2);
     auto convert = [&](auto conv, uint32_t codes, uint32_t tiles, int n_ld, int n_kv, uint64_t* ld_full, uint64_t* ld_empty,
-                       uint64_t* kv_empty, int rec, int stage_bytes) {
+                       uint64_t* kv_empty, uint8_t* exps, uint8_t* wide, int n_exp, int rec, int stage_bytes) {
       conv.init(t);
       bool ready = false;
-      const int steps = nkv + (is_v ? 0 : 2);
-      for (int j = 0; j < steps; ++j) {
+      for (int j = 0; j < nkv; ++j) {
         const int ls = j % n_ld, ks = j % n_kv;
         // usually already found ready at the end of the last tile
         if (!__all_sync(0xffffffffu, ready)) {
-          if (j < nkv && !poll_wait_warp(&ld_full[ls], (j / n_ld) & 1, abort, a.status, lim)) break;
+          if (!poll_wait_warp(&ld_full[ls], (j / n_ld) & 1, abort, a.status, lim)) break;
           if (j >= n_kv && !poll_wait_warp(&kv_empty[ks], ((j / n_kv) - 1) & 1, abort, a.status, lim)) break;
         }
-        if (j < nkv) {
-          const uint32_t dst = tiles + ks * kKVTile;
-          int any = 0;
+        const uint32_t dst = tiles + ks * kKVTile;
+        const int slot = j % n_exp;
+        int any = 0;
 #pragma unroll 2
-          for (int p = 0; p < rows; p += 8) {
-            const int r = r0 + p, e = it.jb + 4 * j + (r >> 4);
-            const bool live = e < it.je && it.block_at(e) * kBlock + (r & 15) < it.kv_len;
-            const int x = conv.row(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, dst, r, t, live);
-            if (!is_v) {
-              any |= x;
-              if (t == 0) smem[GEO::kOffExp + (j % GEO::kExp) * BN + r] = static_cast<uint8_t>(x);
-            }
-          }
-          if (!is_v) {
-            any = __any_sync(0xffffffffu, any != 0);
-            if (lane == 0) smem[GEO::kOffWide + 4 * (j % GEO::kExp) + r0 / rows] = static_cast<uint8_t>(any);
-          }
+        for (int p = 0; p < rows; p += 8) {
+          const int r = r0 + p, e = it.jb + 4 * j + (r >> 4);
+          const bool live = e < it.je && it.block_at(e) * kBlock + (r & 15) < it.kv_len;
+          const int x = conv.row(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, dst, r, t, live);
+          any |= x;
+          if (t == 0) exps[slot * BN + r] = static_cast<uint8_t>(x);
         }
+        any = __any_sync(0xffffffffu, any != 0);
+        if (lane == 0) wide[4 * slot + r0 / rows] = static_cast<uint8_t>(any);
         const int jn = j + 1;
         ready = mbar_test(&ld_full[jn % n_ld], (jn / n_ld) & 1);
         ready = (jn < n_kv || mbar_test(&kv_empty[jn % n_kv], ((jn / n_kv) - 1) & 1)) && ready && jn < nkv;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          if (j < nkv) mbar_arrive(&ld_empty[ls]);
-          const int on = is_v ? j : j - 2;
-          if (on >= 0)
-            mbar_arrive(&bars[GEO::bReady + on % GEO::kReady]);
-          else if (j < nkv)
-            mbar_arrive(&bars[GEO::bK01 + j]);
+          mbar_arrive(&ld_empty[ls]);
+          mbar_arrive(&bars[GEO::bReady + j % GEO::kReady]);
         }
       }
     };
@@ -559,10 +589,17 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     uint64_t* const ld_full = bars + GEO::bLdFull + (is_v ? LK : 0);
     uint64_t* const ld_empty = bars + GEO::bLdEmpty + (is_v ? LK : 0);
     uint64_t* const kv_empty = bars + GEO::bKvEmpty + (is_v ? NK : 0);
-    if (!is_v)
-      convert(Converter<L, KB, true>{}, codes, dst, LK, NK, ld_full, ld_empty, kv_empty, GEO::kRecK, GEO::kStageK);
+    uint8_t* const exps = smem + (is_v ? GEO::kOffExpV : GEO::kOffExpK);
+    uint8_t* const wide = smem + (is_v ? GEO::kOffWideV : GEO::kOffWideK);
+    const int n_exp = is_v ? GEO::kExpV : GEO::kExpK;
+    // one copy of the loop where K and V have the same format: the instruction caches
+    // hold four different loops per sub-partition as it is
+    if (KB == VB || !is_v)
+      convert(Converter<L, KB>{}, codes, dst, is_v ? LV : LK, is_v ? NV : NK, ld_full, ld_empty, kv_empty, exps, wide, n_exp,
+              GEO::kRecK, GEO::kStageK);
     else
-      convert(Converter<L, VB, false>{}, codes, dst, LV, NV, ld_full, ld_empty, kv_empty, GEO::kRecV, GEO::kStageV);
+      convert(Converter<L, VB>{}, codes, dst, LV, NV, ld_full, ld_empty, kv_empty, exps, wide, n_exp, GEO::kRecV,
+              GEO::kStageV);
   } else if (warp == kProdWarp || warp == kProdWarpV) {
     // ------------------------------------------------------------ producers
     const bool pv = warp != kProdWarp;
@@ -592,8 +629,8 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     // ------------------------------------------------------------ MMA issuers
     const int x = warp - kMmaWarp;
     if (lane == 0 && x < nq) {
-      constexpr uint32_t idS = idesc_f16(BM, BN);
-      constexpr uint32_t idPV = idesc_bf16(BM, D, 1);
+      constexpr uint32_t idS = idesc_f16(BM, BN, 0);
+      constexpr uint32_t idPV = idesc_f16(BM, D, 1);
       const uint32_t tS0 = tmem + kColS + 128 * x, tO = tmem + kColO + 128 * x;
       // descriptors address shared memory in units of 16 bytes
       const uint64_t dq = smem_desc_sw128(sbase + GEO::kOffQ + x * kQTile, 16, 1024);
@@ -614,28 +651,27 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         for (int kk = 0; kk < BN / 16; ++kk)
           mma_bf16_ts(tO, p + 8 * kk, v + ((kk * 2048) >> 4), idPV, (j > 0 || kk > 0) ? 1u : 0u);
       };
-      bool ok = nkv > 0 && poll_wait(&bars[GEO::bQReady + x], 0, abort, a.status, lim) &&
-                poll_wait(&bars[GEO::bK01], 0, abort, a.status, lim);
-      if (ok) {
+      auto wait_ready = [&](int j) {
+        return poll_wait(&bars[GEO::bReady + j % GEO::kReady], (j / GEO::kReady) & 1, abort, a.status, lim);
+      };
+      bool ok = nkv > 0 && poll_wait(&bars[GEO::bQReady + x], 0, abort, a.status, lim);
+      for (int j = 0; j < 2 && j < nkv && ok; ++j) {
+        if (!(ok = wait_ready(j))) break;
         tc_fence_after();
-        issue_s(0);
-        if (nkv > 1 && (ok = poll_wait(&bars[GEO::bK01 + 1], 0, abort, a.status, lim))) {
-          tc_fence_after();
-          issue_s(1);
-        }
+        issue_s(j);
       }
       // A test of a barrier takes this thread over 100 cycles even where its phase has
-      // completed, and a tile's issue is what it has time for: the tiles of step j + 1 are
-      // tested before S(j+2) is issued, and waited for only if that failed.
-      bool ready = false;
+      // completed, and a tile's issue is what it has time for: the next tile's is tested
+      // before S(j+2) is issued, and waited for only if that failed.
+      bool ready = nkv > 2 && ok && mbar_test(&bars[GEO::bReady + 2], 0);
       for (int j = 0; j < nkv && ok; ++j) {
-        if (!ready && !(ok = poll_wait(&bars[GEO::bReady + j % GEO::kReady], (j / GEO::kReady) & 1, abort, a.status, lim)))
-          break;
         if (!(ok = poll_wait(&bars[GEO::bPFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim))) break;
         tc_fence_after();
         issue_pv(j);
-        ready = j + 1 < nkv && mbar_test(&bars[GEO::bReady + (j + 1) % GEO::kReady], ((j + 1) / GEO::kReady) & 1);
         if (j + 2 < nkv) {
+          if (!ready && !(ok = wait_ready(j + 2))) break;
+          ready = j + 3 < nkv && mbar_test(&bars[GEO::bReady + (j + 3) % GEO::kReady], ((j + 3) / GEO::kReady) & 1);
+          tc_fence_after();
           issue_s(j + 2);
         } else if (j + 2 == nkv) {
           mma_commit(&bars[GEO::bOReady + x]);

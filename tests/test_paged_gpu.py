@@ -1,17 +1,19 @@
 """Paged quantized cache (kvq.paged) on the GPU against plain forms: append bit-exact to
 the storage oracle, read exact, attention against its definition in 64 bits.
 
-Tolerances of the attention, derived from its roundings (u = 2^-9, half a bf16 step):
-the kernel may round each K and V value to bf16 (relative u), each softmax weight to bf16
-(u) and the output to bf16 (u). A K rounding moves a logit by at most
-d = scale * u * sum_c |q_c K_c|, a weight by a factor exp(+-2 d). So per output element
-  |err| <= u |o| + (2 u + 2 d_max + 2e-5) * sum_j w_j |V_j|      (2e-5: fp32 sums and exp)
-always. As the roundings are independent, with a standard deviation of u / sqrt(3) at most
-each, the error's expected square is, per element,
-  u^2/3 (o^2 + sum_j w_j^2 (2 V_j^2 + (V_j - o)^2 scale^2 sum_c (q_c K_jc)^2))
-and the 2-norm of a case's error is held to three times the root of their sum: a case has
-at least 128 elements, but one row's weights are shared by them and may rest on a few
-tokens. A single wrongly seen or missed token exceeds that at every length used here.
+Tolerances of the attention, derived from its roundings: the output to bf16 (relative
+U = 2^-8, half a step at the bottom of a binade), each K and V value and each softmax weight to
+fp16 (u = 2^-11; a weight below fp16's normal range, of which the largest is at least 1,
+absolutely 2^-25). A K rounding moves a logit by at most d = scale * u * sum_c |q_c K_c|, a
+weight by a factor exp(+-2 d). So per output element, with L = sum_j exp(x_j - max x)
+  |err| <= U |o| + (2 u + 2 d_max + 2e-5) * sum_j w_j |V_j| + 2^-25 sum_j |V_j| / L
+(2e-5: fp32 sums and exp) always. As the roundings are independent, with a standard
+deviation of at most a bound / sqrt(3) each, the error's expected square is, per element,
+  U^2/3 o^2 + u^2/3 sum_j w_j^2 (2 V_j^2 + (V_j - o)^2 scale^2 sum_c (q_c K_jc)^2)
+and the 2-norm of a case's error is held to three times the root of their sum (and the
+absolute parts above): a case has at least 128 elements, but one row's weights are shared by
+them and may rest on a few tokens. A single wrongly seen or missed token exceeds that at every
+length used here.
 """
 import numpy as np
 import pytest
@@ -23,7 +25,7 @@ from quant_kv import _band_edges
 
 pytestmark = pytest.mark.gpu
 
-U = 2.0 ** -9
+U, UH = 2.0 ** -8, 2.0 ** -11
 FORMATS = [(4, 4), (8, 4), (8, 8)]
 MODES = ["bands", "bands2", "bands4", "blind32", "blind64"]
 
@@ -105,18 +107,21 @@ def reference(q, k, v, kv, ql, heads, causal, window, sink, scale=None):
             see &= (j > pos - window) | (j < sink)
         for h in range(q.shape[1]):
             x = (q[f:f + m, h] @ kb[:, h // group].T) * scale
-            d = scale * U * (q[f:f + m, h].abs() @ kb[:, h // group].abs().T)
+            d = scale * UH * (q[f:f + m, h].abs() @ kb[:, h // group].abs().T)
             x = x.masked_fill(~see, -np.inf)
             some = see.any(1)
             w = torch.where(some[:, None], torch.softmax(x, 1), torch.zeros(()).double())
             out[f:f + m, h] = w @ vb[:, h // group]
             lse[f:f + m, h] = torch.where(some, torch.logsumexp(x, 1), torch.tensor(-np.inf).double())
             dm = torch.where(see, d, torch.zeros(()).double()).amax(1, keepdim=True) if n else torch.zeros(m, 1)
-            bound[f:f + m, h] = U * out[f:f + m, h].abs() + (2 * U + 2 * dm + 2e-5) * (w @ vb[:, h // group].abs())
+            rel = torch.where(see, torch.exp(x - x.amax(1, keepdim=True)), torch.zeros(()).double()) if n else x
+            small = 2.0 ** -25 * (see.double() @ vb[:, h // group].abs()) / rel.sum(1, keepdim=True).clamp(min=1)
+            floor = 2e-5 * (w @ vb[:, h // group].abs()) + small
+            bound[f:f + m, h] = U * out[f:f + m, h].abs() + (2 * UH + 2 * dm) * (w @ vb[:, h // group].abs()) + floor
             vh, oh, w2 = vb[:, h // group], out[f:f + m, h], w * w
             ws = w2 * scale * scale * (q[f:f + m, h].square() @ kb[:, h // group].square().T)
-            var[f:f + m, h] = U * U / 3 * (oh.square() + 2 * (w2 @ vh.square()) + ws @ vh.square() - 2 * oh * (ws @ vh)
-                                           + oh.square() * ws.sum(1, keepdim=True))
+            var[f:f + m, h] = U * U / 3 * oh.square() + floor.square() + UH * UH / 3 * (
+                2 * (w2 @ vh.square()) + ws @ vh.square() - 2 * oh * (ws @ vh) + oh.square() * ws.sum(1, keepdim=True))
         f, t = f + m, t + n
     return out, lse, bound, var
 
