@@ -37,6 +37,9 @@ constexpr int kRowThreads = 32 * kWarps;
 template <class L, int KB, int VB, int NT>
 struct RowGeo {
   static constexpr int kRecK = Rec<L, KB>::kBytes, kRecV = Rec<L, VB>::kBytes;
+  // most channel groups of a lane's 32 key channels, of its 16 value channels
+  static constexpr int kKG = most_groups<L, 32>(), kVG = most_groups<L, 16>();
+  static_assert(kKG <= 4 && kVG <= 3, "group selection");
   static constexpr int kStage = 2 * (kRecK + kRecV);  // two storage blocks
   static constexpr int kStages = 2;
   static constexpr int kRing = kStages * kStage;  // one warp's
@@ -44,9 +47,9 @@ struct RowGeo {
   static constexpr int kOffBar = kOffML + kWarps * 8 * NT * 8;
   static constexpr int kOffMisc = kOffBar + kWarps * kStages * 8;
   static constexpr int kSmemBytes = kOffMisc + 16;
-  // resident blocks: shared memory, and registers (128 a thread for four, 168 for three)
+  // resident blocks: shared memory, and registers (168 a thread for three, 255 for two; with four, and spills, 5 to 20 % slower)
   static constexpr int kFit = (228 * 1024) / (kSmemBytes + 1024);
-  static constexpr int kCtas = kFit < (NT == 1 ? 4 : 3) ? kFit : (NT == 1 ? 4 : 3);
+  static constexpr int kCtas = kFit < (NT == 1 ? 3 : 2) ? kFit : (NT == 1 ? 3 : 2);
   static_assert(kRing >= 8 * NT * D * 4, "the join fits a warp's ring");
   static_assert(kRecK % 16 == 0 && kStage % 16 == 0, "bulk copies");
 };
@@ -66,10 +69,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 template <class L, int KB, int VB, int NT>
 __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) rows_kernel(const __grid_constant__ AttnArgs a) {
   using GEO = RowGeo<L, KB, VB, NT>;
-  constexpr int G = L::G;
   static_assert(GEO::kStages == 2, "stage and phase below");
-  constexpr int KG = most_groups<L, 32>(), VG = most_groups<L, 16>();
-  static_assert(KG <= 4 && VG <= 3, "group selection");
   constexpr int kRows = 8 * NT;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -87,8 +87,8 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
 
   // this lane's channel groups: K channels 32t.., V channels 16g..
   const int kbase = group_at<L>(32 * t), vbase = group_at<L>(16 * g);
-  uint32_t ksel[KG == 1 ? 1 : 16];
-  if constexpr (KG > 1) {
+  uint32_t ksel[GEO::kKG == 1 ? 1 : 16];
+  if constexpr (GEO::kKG > 1) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int c = 32 * t + 8 * (i >> 2) + (i & 3);
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
   }
   // first channel pair of this lane's second and third V group (8: none)
   int ve1 = 8, ve2 = 8;
-  if constexpr (VG > 1) {
+  if constexpr (GEO::kVG > 1) {
 #pragma unroll
     for (int i = 7; i >= 0; --i) {
       const int l = group_at<L>(16 * g + 2 * i) - vbase;
@@ -115,11 +115,11 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
   const uint32_t copy_dst = smem_u32(ring) + ((lane >> 1) & 1) * (GEO::kStage / 2) + ((lane & 1) ? GEO::kRecK : 0);
   // this lane's K row and V rows inside a stage, codes and scales
   const uint32_t k_codes = smem_u32(ring) + token_of(g) * Rec<L, KB>::CW + t * (KB * 4);
-  const uint32_t k_scales = smem_u32(ring) + Rec<L, KB>::kCodes + token_of(g) * G * 2;
+  const uint32_t k_scales = smem_u32(ring) + Rec<L, KB>::kCodes + token_of(g) * L::G * 2;
   const int vt0 = token_of(2 * t), vt1 = token_of(2 * t + 1);  // and 8 more
   const uint32_t v_ring = smem_u32(ring) + GEO::kRecK;
   const uint32_t v_codes0 = v_ring + vt0 * Rec<L, VB>::CW + g * (2 * VB), v_codes1 = v_codes0 + (vt1 - vt0) * Rec<L, VB>::CW;
-  const uint32_t v_scales0 = v_ring + Rec<L, VB>::kCodes + vt0 * G * 2, v_scales1 = v_scales0 + (vt1 - vt0) * G * 2;
+  const uint32_t v_scales0 = v_ring + Rec<L, VB>::kCodes + vt0 * L::G * 2, v_scales1 = v_scales0 + (vt1 - vt0) * L::G * 2;
 
   pdl_wait();
   pdl_launch_dependents();
@@ -231,19 +231,20 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
       const int ta = it.block_at(e0) * kBlock, tz = it.block_at(e0 + 1) * kBlock;  // first tokens of the blocks
       const bool whole = two && tz + kBlock <= first.hi && (ta >= final_.lo || tz + kBlock <= first.kept);
 
-      // ---- S^T
-      float s[NT][2][4];
-#pragma unroll
-      for (int bb = 0; bb < 2; ++bb) {
+      // ---- S^T of storage block bb. EXACT: with a power of two taken out of the tokens beyond
+      // (kScaleLeast, kScaleMost); else as if there were none, keeping the scales' extremes.
+      uint32_t least = kScaleLeast, most = 0;
+      auto scores = [&](const uint32_t off, float (&acc)[NT][4], auto exact) {
+        constexpr bool EXACT = decltype(exact)::value;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][bb][e] = 0.0f;
-        uint32_t kw[2][KB == 4 ? 4 : 8], ks01[2], ks23[2], kx[2];
-        float kscale[2][KG];
+          for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
+        uint32_t kw[2][KB == 4 ? 4 : 8], ks01[2], ks23[2];
+        float back[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t src = k_codes + at + bb * (GEO::kStage / 2) + 8 * r * Rec<L, KB>::CW;
+          const uint32_t src = k_codes + off + 8 * r * Rec<L, KB>::CW;
 #pragma unroll
           for (int w = 0; w < KB / 4; ++w) {
             const uint4 v = ld_shared_v4(src + 16 * w);
@@ -252,33 +253,29 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
             kw[r][4 * w + 2] = v.z;
             kw[r][4 * w + 3] = v.w;
           }
-          const uint32_t sc = k_scales + at + bb * (GEO::kStage / 2) + 8 * r * G * 2;
-          uint32_t x[4];
+          const uint32_t from = k_scales + off + 8 * r * L::G * 2;
+          uint32_t x[GEO::kKG], top = 0;
+          float f[GEO::kKG];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) x[q] = q < KG ? ld_shared_u16(sc + 2 * (KG == 1 ? kbase : min(kbase + q, G - 1))) : 0u;
-          kx[r] = max(max(x[0], x[1]), max(x[2], x[3]));
-#pragma unroll
-          for (int q = 0; q < KG; ++q) kscale[r][q] = __uint_as_float(x[q] << 16);
-        }
-        // rare: a token whose scales leave fp16's range (kScaleLeast, kScaleMost)
-        const bool wide = __any_sync(0xffffffffu, beyond(kx[0], kScaleLeast, kScaleMost) ||
-                                                      beyond(kx[1], kScaleLeast, kScaleMost));
-        float back[2];
-        if (wide) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            kx[r] = max(kx[r], __shfl_xor_sync(0xffffffffu, kx[r], 1));
-            kx[r] = max(kx[r], __shfl_xor_sync(0xffffffffu, kx[r], 2));
-            const int e = scale_exponent(kx[r]);
+          for (int q = 0; q < GEO::kKG; ++q) {
+            x[q] = ld_shared_u16(from + 2 * (GEO::kKG == 1 ? kbase : min(kbase + q, L::G - 1)));
+            top = max(top, x[q]);
+            f[q] = __uint_as_float(x[q] << 16);
+          }
+          if constexpr (EXACT) {
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = scale_exponent(top);
             back[r] = pow2i(e);
 #pragma unroll
-            for (int q = 0; q < KG; ++q) kscale[r][q] *= pow2i(-e);
+            for (int q = 0; q < GEO::kKG; ++q) f[q] *= pow2i(-e);
+          } else {
+            most = max(most, top);
+            least = min(least, top);
           }
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          ks01[r] = pack_f16x2(kscale[r][0], kscale[r][KG > 1 ? 1 : 0]);
-          if constexpr (KG > 2) ks23[r] = pack_f16x2(kscale[r][2], kscale[r][KG > 3 ? 3 : 2]);
+          ks01[r] = pack_f16x2(f[0], f[GEO::kKG > 1 ? 1 : 0]);
+          ks23[r] = 0;
+          if constexpr (GEO::kKG > 2) ks23[r] = pack_f16x2(f[2], f[GEO::kKG > 3 ? 3 : 2]);
         }
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -295,71 +292,99 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
                 v = int8_pair_f16(__byte_perm(kw[r][2 * w], kw[r][2 * w + 1], j | j << 4 | (4 + j) << 8 | (4 + j) << 12));
               }
               uint32_t sp = ks01[r];
-              if constexpr (KG > 1) sp = __byte_perm(ks01[r], KG > 2 ? ks23[r] : 0u, ksel[4 * w + j]);
+              if constexpr (GEO::kKG > 1) sp = __byte_perm(ks01[r], ks23[r], ksel[4 * w + j]);
               f[r][j] = h16mul2(v, sp);
             }
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816(s[nt][bb], f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], qf[nt][2 * w + h][0],
-                           qf[nt][2 * w + h][1]);
+              mma16816(acc[nt], f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], qf[nt][2 * w + h][0],
+                       qf[nt][2 * w + h][1]);
         }
-        if (wide) {
+        if constexpr (EXACT) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[nt][bb][e] *= back[e >> 1];
+            for (int e = 0; e < 4; ++e) acc[nt][e] *= back[e >> 1];
         }
-      }
+      };
+      float s[2][NT][4];
+      scores(at, s[0], std::false_type{});
+      scores(at + GEO::kStage / 2, s[1], std::false_type{});
 
-      // ---- V's scales, of this lane's tokens: S rows 2t, 2t + 1, 8 + 2t, 9 + 2t
-      uint32_t vs[2][2][VG];
-      bool wide_v = false;
-      float ve[2][2];  // where wide_v: exponents taken out of the tokens of S rows g, 8 + g
-#pragma unroll
-      for (int bb = 0; bb < 2; ++bb) {
-        uint32_t x[4][VG], most[4] = {0, 0, 0, 0};
+      // ---- V's scales, of this lane's tokens: S rows 2t, 2t + 1, 8 + 2t, 9 + 2t, of block bb
+      auto value_scales = [&](const uint32_t off, const int first_token, const bool any_live, uint32_t (&vs)[2][GEO::kVG],
+                              float (&ve)[2], auto exact) {
+        constexpr bool EXACT = decltype(exact)::value;
+        float f[4][GEO::kVG];
+        int ex[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const uint32_t from = ((u & 1) ? v_scales1 : v_scales0) + at + bb * (GEO::kStage / 2) + (u >> 1) * 8 * G * 2;
+          const uint32_t from = ((u & 1) ? v_scales1 : v_scales0) + off + (u >> 1) * 8 * L::G * 2;
+          // rows past the end hold anything: as zeros they add nothing
+          const bool live = whole || (any_live && first_token + ((u & 1) ? vt1 : vt0) + (u >> 1) * 8 < it.kv_len);
+          uint32_t top = 0;
 #pragma unroll
-          for (int q = 0; q < VG; ++q) {
-            x[u][q] = ld_shared_u16(from + 2 * (VG == 1 ? vbase : min(vbase + q, G - 1)));
-            // rows past the end hold anything: as zeros they add nothing
-            if (!whole && ((bb ? tz : ta) + ((u & 1) ? vt1 : vt0) + (u >> 1) * 8 >= it.kv_len || (bb && !two))) x[u][q] = 0;
-            most[u] = max(most[u], x[u][q]);
+          for (int q = 0; q < GEO::kVG; ++q) {
+            uint32_t x = ld_shared_u16(from + 2 * (GEO::kVG == 1 ? vbase : min(vbase + q, L::G - 1)));
+            x = live ? x : 0;
+            top = max(top, x);
+            f[u][q] = __uint_as_float(x << 16);
+          }
+          if constexpr (EXACT) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+            ex[u] = scale_exponent(top);
+#pragma unroll
+            for (int q = 0; q < GEO::kVG; ++q) f[u][q] *= pow2i(-ex[u]);
+          } else {
+            most = max(most, top);
+            least = min(least, live ? top : kScaleLeast);
           }
         }
-        float f[4][VG];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int q = 0; q < VG; ++q) f[u][q] = __uint_as_float(x[u][q] << 16);
-        ve[bb][0] = ve[bb][1] = 0.0f;
-        const uint32_t hi = max(max(most[0], most[1]), max(most[2], most[3]));
-        const uint32_t lo = min(min(most[0], most[1]), min(most[2], most[3]));
-        if (__any_sync(0xffffffffu, hi > kScaleMost || lo < kScaleLeast)) {
-          int e[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) most[u] = max(most[u], __shfl_xor_sync(0xffffffffu, most[u], d));
-            e[u] = scale_exponent(most[u]);
-#pragma unroll
-            for (int q = 0; q < VG; ++q) f[u][q] *= pow2i(-e[u]);
-          }
+        if constexpr (EXACT) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const int ea = __shfl_sync(0xffffffffu, e[2 * r], g >> 1), eb = __shfl_sync(0xffffffffu, e[2 * r + 1], g >> 1);
-            ve[bb][r] = static_cast<float>((g & 1) ? eb : ea);
+            const int ea = __shfl_sync(0xffffffffu, ex[2 * r], g >> 1), eb = __shfl_sync(0xffffffffu, ex[2 * r + 1], g >> 1);
+            ve[r] = static_cast<float>((g & 1) ? eb : ea);
           }
-          wide_v = __any_sync(0xffffffffu, ve[bb][0] != 0.0f || ve[bb][1] != 0.0f) || wide_v;
         }
 #pragma unroll
-        for (int q = 0; q < VG; ++q) {
-          vs[bb][0][q] = pack_f16x2(f[0][q], f[1][q]);
-          vs[bb][1][q] = pack_f16x2(f[2][q], f[3][q]);
+        for (int q = 0; q < GEO::kVG; ++q) {
+          vs[0][q] = pack_f16x2(f[0][q], f[1][q]);
+          vs[1][q] = pack_f16x2(f[2][q], f[3][q]);
+        }
+      };
+      uint32_t vs[2][2][GEO::kVG];
+      float ve[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};  // exponents taken out of the tokens of S rows g, 8 + g
+      value_scales(at, ta, true, vs[0], ve[0], std::false_type{});
+      value_scales(at + GEO::kStage / 2, tz, two, vs[1], ve[1], std::false_type{});
+      bool wide_v = false;
+      if (__any_sync(0xffffffffu, most > kScaleMost || least < kScaleLeast)) {
+        // rare: once more, with the powers of two
+#pragma unroll 1
+        for (int bb = 0; bb < 2; ++bb) {
+          float sx[NT][4], vx[2];
+          uint32_t vsx[2][GEO::kVG];
+          scores(at + bb * (GEO::kStage / 2), sx, std::true_type{});
+          value_scales(at + bb * (GEO::kStage / 2), bb ? tz : ta, !bb || two, vsx, vx, std::true_type{});
+          wide_v = __any_sync(0xffffffffu, vx[0] != 0.0f || vx[1] != 0.0f) || wide_v;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            if (b == bb) {
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[b][nt][e] = sx[nt][e];
+#pragma unroll
+              for (int q = 0; q < GEO::kVG; ++q) {
+                vs[b][0][q] = vsx[0][q];
+                vs[b][1][q] = vsx[1][q];
+              }
+              ve[b][0] = vx[0];
+              ve[b][1] = vx[1];
+            }
         }
       }
 
@@ -375,11 +400,11 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
             for (int e = 0; e < 4; ++e) {
               const int j = (bb ? tz : ta) + 8 * (e >> 1) + token_of(g);
               const Seen& v = see[nt][e & 1];
-              if (!(j < v.hi && (j >= v.lo || j < v.kept)) || (bb && !two)) s[nt][bb][e] = -INFINITY;
+              if (!(j < v.hi && (j >= v.lo || j < v.kept)) || (bb && !two)) s[bb][nt][e] = -INFINITY;
             }
         }
-        const float mx0 = fmaxf(fmaxf(s[nt][0][0], s[nt][0][2]), fmaxf(s[nt][1][0], s[nt][1][2])) * sc[nt][0];
-        const float mx1 = fmaxf(fmaxf(s[nt][0][1], s[nt][0][3]), fmaxf(s[nt][1][1], s[nt][1][3])) * sc[nt][1];
+        const float mx0 = fmaxf(fmaxf(s[0][nt][0], s[0][nt][2]), fmaxf(s[1][nt][0], s[1][nt][2])) * sc[nt][0];
+        const float mx1 = fmaxf(fmaxf(s[0][nt][1], s[0][nt][3]), fmaxf(s[1][nt][1], s[1][nt][3])) * sc[nt][1];
         fresh[nt][0] = m[nt][0] < -1.0e29f;
         fresh[nt][1] = m[nt][1] < -1.0e29f;
         if (__any_sync(0xffffffffu, mx0 > m[nt][0] + 8.0f || mx1 > m[nt][1] + 8.0f)) {
@@ -408,7 +433,7 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
         for (int bb = 0; bb < 2; ++bb) {
           float p[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = ex2f(fmaf(s[nt][bb][e], sc[nt][e & 1], -m[nt][e & 1]));
+          for (int e = 0; e < 4; ++e) p[e] = ex2f(fmaf(s[bb][nt][e], sc[nt][e & 1], -m[nt][e & 1]));
           l[nt][0] += p[0] + p[2];
           l[nt][1] += p[1] + p[3];
           pf[nt][bb][0] = transpose8x8(pack_f16x2(p[0], p[1]));
@@ -426,8 +451,8 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           for (int bb = 0; bb < 2; ++bb)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              s[nt][bb][e] = fmaf(s[nt][bb][e], sc[nt][e & 1], -m[nt][e & 1]) + ve[bb][e >> 1];
-              top[e & 1] = fmaxf(top[e & 1], s[nt][bb][e]);
+              s[bb][nt][e] = fmaf(s[bb][nt][e], sc[nt][e & 1], -m[nt][e & 1]) + ve[bb][e >> 1];
+              top[e & 1] = fmaxf(top[e & 1], s[bb][nt][e]);
             }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -446,7 +471,7 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           for (int bb = 0; bb < 2; ++bb)
 #pragma unroll
             for (int r = 0; r < 2; ++r)
-              pf[nt][bb][r] = transpose8x8(pack_f16x2(ex2f(s[nt][bb][2 * r] - F[nt][0]), ex2f(s[nt][bb][2 * r + 1] - F[nt][1])));
+              pf[nt][bb][r] = transpose8x8(pack_f16x2(ex2f(s[bb][nt][2 * r] - F[nt][0]), ex2f(s[bb][nt][2 * r + 1] - F[nt][1])));
           f_any = __any_sync(0xffffffffu, F[nt][0] != 0.0f || F[nt][1] != 0.0f) || f_any;
         }
       }
@@ -477,8 +502,8 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             uint32_t sp = vs[bb][u][0];
-            if (VG > 1) sp = i >= ve1 ? vs[bb][u][VG > 1 ? 1 : 0] : sp;
-            if (VG > 2) sp = i >= ve2 ? vs[bb][u][VG > 2 ? 2 : 0] : sp;
+            if (GEO::kVG > 1) sp = i >= ve1 ? vs[bb][u][GEO::kVG > 1 ? 1 : 0] : sp;
+            if (GEO::kVG > 2) sp = i >= ve2 ? vs[bb][u][GEO::kVG > 2 ? 2 : 0] : sp;
             if constexpr (VB == 4) {
               const int b = i & 3;  // the byte with both channels, of either token
               const uint32_t x = __byte_perm(vw[2 * u][i >> 2], vw[2 * u + 1][i >> 2], b | b << 4 | (4 + b) << 8 | (4 + b) << 12);

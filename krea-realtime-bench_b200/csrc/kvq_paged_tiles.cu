@@ -40,15 +40,16 @@ constexpr int kQAtom = BM * 128;
 
 // Shared memory: fp16 stages of K and V, staged records, the Q tiles. Four fp16
 // stages per tensor and three staged tiles where the codes are small; int8 codes leave
-// room for two, and with both tensors int8 for three fp16 stages of V.
+// room for two, and with both tensors int8 for three fp16 stages of K (a K stage is free two
+// tiles before a V stage).
 template <class L, int KB, int VB>
 struct Geo {
   static constexpr int kRecK = Rec<L, KB>::kBytes, kRecV = Rec<L, VB>::kBytes;
   static constexpr int kStageK = 4 * kRecK, kStageV = 4 * kRecV;
-  static constexpr int NK = 4, NV = VB == 8 ? 3 : 4;
+  static constexpr int NK = VB == 8 ? 3 : 4, NV = 4;
   static constexpr int LK = KB == 8 ? 2 : 3, LV = KB == 8 ? 2 : 3;
   static constexpr int kReady = 4;
-  static_assert(NK == 4 && NV <= 4, "no tile may be converted before the barrier of the one kReady before it completes");
+  static_assert(NK <= 4 && NV == 4, "no tile may be converted before the barrier of the one kReady before it completes");
   static constexpr int kOffK = 0;
   static constexpr int kOffV = kOffK + NK * kKVTile;
   static constexpr int kOffQ = kOffV + NV * kKVTile;
@@ -63,7 +64,7 @@ struct Geo {
   static constexpr int kOffMisc = (kOffBar + kNumBars * 8 + 15) / 16 * 16;
   // Of the last kExpK key tiles and kExpV value tiles: the exponent taken out of each token,
   // and a byte per converter warp that says whether there is any. K's of a tile are written
-  // again only after S(j + kExpK - 4), V's after S(j + 2), each issued behind P(j) of
+  // again only after S(j + kExpK - NK), V's after S(j + 2), each issued behind P(j) of
   // every softmax warp.
   static constexpr int kExpK = 6, kExpV = 4;
   static constexpr int kOffExpK = kOffMisc + 32, kOffExpV = kOffExpK + kExpK * BN;
@@ -104,9 +105,12 @@ struct Converter {
       }
     }
   }
-  // One row: record block `rec`, row `rr` of it, to row r of the tile at dst. Returns the
-  // exponent taken out of the row (kScaleLeast, kScaleMost).
-  __device__ __forceinline__ int row(uint32_t rec, int rr, uint32_t dst, int r, int t, bool live) const {
+  // One row: record block `rec`, row `rr` of it, to row r of the tile at dst. EXACT: takes a
+  // power of two out of a row beyond (kScaleLeast, kScaleMost) and returns its exponent;
+  // else converts as if there were none and keeps this lane's extremes of live rows' scales.
+  template <bool EXACT>
+  __device__ __forceinline__ int row(uint32_t rec, int rr, uint32_t dst, int r, int t, bool live, uint32_t& least,
+                                     uint32_t& most) const {
     using R = Rec<L, BITS>;
     uint32_t w[BITS];  // 4 or 8 words of codes
     const uint32_t src = rec + rr * R::CW + t * (R::CW / 4);
@@ -119,24 +123,27 @@ struct Converter {
       w[4 * i + 3] = v.w;
     }
     const uint32_t sc = rec + R::kCodes + rr * L::G * 2;
-    uint32_t x[4];
+    uint32_t x[KG], top = 0;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      x[q] = q < KG ? ld_shared_u16(sc + 2 * (KG == 1 ? base : min(base + q, L::G - 1))) : 0u;
-      if (!live) x[q] = 0;  // rows past the end hold anything: as zeros they add nothing
+    for (int q = 0; q < KG; ++q) {
+      x[q] = ld_shared_u16(sc + 2 * (KG == 1 ? base : min(base + q, L::G - 1)));
+      top = max(top, x[q]);
     }
+    float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int q = 0; q < KG; ++q) f[q] = live ? __uint_as_float(x[q] << 16) : 0.0f;  // rows past the end hold anything
     uint32_t s01, s23 = 0;
     int e = 0;
-    float f[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) f[q] = __uint_as_float(x[q] << 16);
-    uint32_t most = max(max(x[0], x[1]), max(x[2], x[3]));
-    if (__any_sync(0xffffffffu, beyond(most, kScaleLeast, kScaleMost))) {
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      e = scale_exponent(most);
+    if constexpr (EXACT) {
+      top = live ? top : 0;
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      e = scale_exponent(top);
 #pragma unroll
       for (int q = 0; q < KG; ++q) f[q] *= pow2i(-e);
+    } else if (live) {
+      most = max(most, top);
+      least = min(least, top);
     }
     s01 = pack_f16x2(f[0], f[KG == 1 ? 0 : 1]);
     if constexpr (KG > 2) s23 = pack_f16x2(f[2], f[3]);
@@ -338,7 +345,11 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       for (int c = 0; c < 16; ++c) most = max(most, most_of(ld_global_nc_v4(src + c)));
       row_scale *= pow2i(query_exponent(most));
     }
-    auto step = [&](const int j, const bool wide_k, const bool wide_v, auto masked) -> bool {
+    // wide_k, wide_v: a byte per converter warp of the tile, and whose rows' exponents count
+    auto exps16 = [&](uint32_t wide, uint32_t at, int block) {
+      return (wide >> (8 * (n_conv == 2 ? block >> 1 : block))) & 255u ? ld_shared_v4(at + 16 * block) : make_uint4(0, 0, 0, 0);
+    };
+    auto step = [&](const int j, const uint32_t wide_k, const uint32_t wide_v, auto masked) -> bool {
       constexpr bool MASK = decltype(masked)::value;
       const uint32_t tS = tS0 + 64 * (j & 1);
       uint32_t s0[32], s1[32];
@@ -348,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
           const uint32_t at = sbase + GEO::kOffExpK + (j % GEO::kExpK) * BN;
 #pragma unroll
           for (int c = 0; c < 32; c += 16) {
-            const uint4 u = ld_shared_v4(at + c), v = ld_shared_v4(at + 32 + c);
+            const uint4 u = exps16(wide_k, at, c / 16), v = exps16(wide_k, at, 2 + c / 16);
             const uint32_t eu[4] = {u.x, u.y, u.z, u.w}, ev[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -410,12 +421,12 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       half(s0, 0);
       if constexpr (MASK) {
         half(s1, 32);
-        if (__any_sync(0xffffffffu, wide_v || F != 0.0f)) {
+        if (__any_sync(0xffffffffu, wide_v != 0 || F != 0.0f)) {
           // weights times the powers of two taken out of the values, relative to 2^F, in
           // log2: y = s * scale - m + e. F grows where 2^(y - F) would leave fp16.
           const uint32_t at = sbase + GEO::kOffExpV + (j % GEO::kExpV) * BN;
           auto exps_of = [&](int c, float (&e)[16]) {
-            const uint4 u = wide_v ? ld_shared_v4(at + c) : make_uint4(0, 0, 0, 0);
+            const uint4 u = exps16(wide_v, at, c / 16);
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
             for (int i = 0; i < 16; ++i) e[i] = static_cast<float>(static_cast<int8_t>(w[i >> 2] >> (8 * (i & 3))));
@@ -490,12 +501,12 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         if (j >= 2) mbar_arrive(&bars[GEO::bKvEmpty + NK + (j - 2) % NV]);
       }
       tc_fence_after();
-      const bool wide_k = *reinterpret_cast<volatile uint32_t*>(smem + GEO::kOffWideK + 4 * (j % GEO::kExpK)) != 0;
-      const bool wide_v = *reinterpret_cast<volatile uint32_t*>(smem + GEO::kOffWideV + 4 * (j % GEO::kExpV)) != 0;
+      const uint32_t wide_k = *reinterpret_cast<volatile uint32_t*>(smem + GEO::kOffWideK + 4 * (j % GEO::kExpK));
+      const uint32_t wide_v = *reinterpret_cast<volatile uint32_t*>(smem + GEO::kOffWideV + 4 * (j % GEO::kExpV));
       const int e0 = it.jb + 4 * j;
       const int ta = it.block_at(e0) * kBlock, tz = it.block_at(e0 + 3) * kBlock + kBlock;
       const bool whole = e0 + 4 <= it.je && tz <= first.hi && (ta >= fin.lo || tz <= first.kept);
-      ok = __all_sync(0xffffffffu, whole && !wide_k && !wide_v && F == 0.0f) ? step(j, false, false, std::false_type{})
+      ok = __all_sync(0xffffffffu, whole && wide_k == 0 && wide_v == 0 && F == 0.0f) ? step(j, 0, 0, std::false_type{})
                                                                              : step(j, wide_k, wide_v, std::true_type{});
       if (!ok) break;
     }
@@ -563,16 +574,26 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         }
         const uint32_t dst = tiles + ks * kKVTile;
         const int slot = j % n_exp;
-        int any = 0;
-#pragma unroll 2
-        for (int p = 0; p < rows; p += 8) {
-          const int r = r0 + p, e = it.jb + 4 * j + (r >> 4);
-          const bool live = e < it.je && it.block_at(e) * kBlock + (r & 15) < it.kv_len;
-          const int x = conv.row(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, dst, r, t, live);
-          any |= x;
-          if (t == 0) exps[slot * BN + r] = static_cast<uint8_t>(x);
-        }
-        any = __any_sync(0xffffffffu, any != 0);
+        uint32_t least = kScaleLeast, most = 0;
+        auto convert_rows = [&](auto exact) {
+          constexpr bool EXACT = decltype(exact)::value;
+          int any = 0;
+#pragma unroll(EXACT ? 1 : 2)
+          for (int p = 0; p < rows; p += 8) {
+            const int r = r0 + p, e = it.jb + 4 * j + (r >> 4);
+            const bool live = e < it.je && it.block_at(e) * kBlock + (r & 15) < it.kv_len;
+            const int x = conv.template row<EXACT>(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, dst, r, t, live, least,
+                                                   most);
+            if constexpr (EXACT) {
+              any |= x;
+              if (t == 0) exps[slot * BN + r] = static_cast<uint8_t>(x);
+            }
+          }
+          return any;
+        };
+        int any = convert_rows(std::false_type{});
+        if (__any_sync(0xffffffffu, most > kScaleMost || least < kScaleLeast))
+          any = __any_sync(0xffffffffu, convert_rows(std::true_type{}) != 0);
         if (lane == 0) wide[4 * slot + r0 / rows] = static_cast<uint8_t>(any);
         const int jn = j + 1;
         ready = mbar_test(&ld_full[jn % n_ld], (jn / n_ld) & 1);
