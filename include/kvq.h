@@ -386,7 +386,8 @@ typedef struct {
 /*
  * Writes the plan to out (HOST int32[capacity], to be copied to the device; NULL:
  * only *info is filled). Of the cache only its format counts, not its pages. kv_lens,
- * q_lens: HOST int32[n_seqs]. n_sms: SMs of the device that will run it. KVQ_ERR_ARG where capacity < info->words.
+ * q_lens: HOST int32[n_seqs]. n_sms: SMs of the device that will run it. KVQ_ERR_ARG
+ * where capacity < info->words.
  */
 KVQ_API int kvq_paged_plan(const kvq_paged_cache* cache, const int32_t* kv_lens, const int32_t* q_lens, int n_seqs,
                            int n_q_heads, int causal, int64_t window, int64_t sink, int n_sms, int32_t* out,
@@ -397,7 +398,8 @@ KVQ_API int kvq_paged_plan(const kvq_paged_cache* cache, const int32_t* kv_lens,
  * query i of a sequence stands at position p = kv_len - q_len + i and sees tokens
  *   j < kv_len,  j <= p if causal,  j > p - window or j < sink if window > 0;
  * out = sum_j w_j V_j, w = softmax(q . K_j * softmax_scale) over the tokens it sees
- * (softmax_scale <= 0: 1/sqrt(head_dim)); 0 (lse -inf) where it sees none.
+ * (softmax_scale <= 0: 1/sqrt(head_dim); at most 1e38); 0 (lse -inf) where it sees
+ * none. Logits beyond fp32's range give NaN.
  *   q, out  bf16 [n_new][n_q_heads][head_dim], token strides in elements; query head
  *           h reads KV head h / (n_q_heads / n_heads)
  *   lse     fp32 [n_new][n_q_heads] or NULL: natural log of the sum of exponentials

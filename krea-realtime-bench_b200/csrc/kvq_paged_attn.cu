@@ -19,7 +19,7 @@ extern "C" int kvq_paged_attention(const void* q, int64_t q_token_stride, const 
   KVQ_REQUIRE(n_q_heads >= 1 && n_q_heads <= 65535 && n_q_heads % cache->n_heads == 0, KVQ_ERR_ARG,
               "%d query heads are not a multiple of %d KV heads", n_q_heads, cache->n_heads);
   KVQ_REQUIRE(window >= 0 && sink >= 0, KVQ_ERR_ARG, "window and sink must be >= 0");
-  KVQ_REQUIRE(std::isfinite(softmax_scale), KVQ_ERR_ARG, "softmax_scale must be finite");
+  KVQ_REQUIRE(std::fabs(softmax_scale) <= 1e38f, KVQ_ERR_ARG, "softmax_scale must be at most 1e38");
   if (batch->n_seqs == 0 || batch->n_new == 0) return KVQ_OK;
   KVQ_REQUIRE(q && out, KVQ_ERR_ARG, "NULL q or out pointer");
   KVQ_REQUIRE(q_token_stride >= (int64_t)n_q_heads * paged::D && out_token_stride >= (int64_t)n_q_heads * paged::D,

@@ -15,7 +15,6 @@ stored as QuantKVTensor stores them: int4 or int8 codes with one bf16 scale per
 from __future__ import annotations
 
 import ctypes
-import math
 
 import numpy as np
 import torch
@@ -99,6 +98,8 @@ class PagedBatch:
             raise ValueError("block_table has a page id that is not a page of any pool")
         self.device, self.page_size, self.n_seqs = dev, int(page_size), n
         self._plans = {}
+        kv.setflags(write=False)
+        ql.setflags(write=False)
         self.kv_lens, self.q_lens = kv, ql
         self.n_new, self.n_tokens = int(ql.sum()), int(kv.sum())
         self.n_pages_needed = int(ids.max()) + 1 if ids.size else 0
@@ -198,15 +199,20 @@ class _Plan:
 
     def args(self, raw: int):
         """(info, plan, workspace, counters) for a launch on the current stream, raw."""
-        got = self._work.get(raw)
+        # A captured launch gets a workspace of its graph's own (and counters that each replay
+        # clears): the graph may be replayed beside launches of this stream, and memory that is
+        # cleared in a graph is not cleared for a launch outside of it.
+        capturing = self.info.n_units > 0 and torch.cuda.is_current_stream_capturing()
+        got = None if capturing else self._work.get(raw)
         if got is None:
             n, c = self.info.workspace_bytes, self.info.n_units
             # counters count up to a unit's parts and are set back by the last one
             ws = torch.empty(max(n, 1), dtype=torch.uint8, device=self.device)
             counters = torch.zeros(max(c, 1), dtype=torch.int32, device=self.device)
-            self._keep.append((ws, counters))
-            got = self._work[raw] = (ctypes.byref(self.info), self.items.data.data_ptr(), ws.data_ptr(),
-                                     counters.data_ptr())
+            got = ctypes.byref(self.info), self.items.data.data_ptr(), ws.data_ptr(), counters.data_ptr()
+            if not capturing:
+                self._keep.append((ws, counters))
+                self._work[raw] = got
         if raw != self.items.stream:
             self.items.use()
         return got
@@ -344,7 +350,8 @@ def attention(q: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, causal: b
     Query i of a sequence stands at position p = kv_len - q_len + i; it sees tokens
     j <= p if causal (else all), of those the last `window` (0: all) and the first
     `sink`. A query that sees nothing gives 0, and -inf. Query head h reads KV head
-    h / (n_q_heads / n_heads); softmax_scale defaults to 1 / sqrt(128)."""
+    h / (n_q_heads / n_heads); softmax_scale defaults to 1 / sqrt(128). Logits beyond
+    fp32's range give NaN."""
     if not isinstance(cache, PagedKVCache):
         raise TypeError(f"expected a PagedKVCache, got {type(cache).__name__}")
     cache._check(batch)
@@ -359,8 +366,9 @@ def attention(q: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, causal: b
     if sink and not window:
         raise ValueError("sink keeps the first tokens of a window: give window too")
     scale = 0.0 if softmax_scale is None else float(softmax_scale)
-    if softmax_scale is not None and not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError(f"softmax_scale must be a positive number, got {softmax_scale}")
+    # least: the kernels hold it in fp32, where a smaller one is 0
+    if softmax_scale is not None and not 1e-38 <= scale <= 1e38:
+        raise ValueError(f"softmax_scale must be between 1e-38 and 1e38, got {softmax_scale}")
     shape, device = (batch.n_new, heads, cache.head_dim), cache.device
     q, qs = _rows(q, shape, device, "q")
     if out is None:
