@@ -468,3 +468,72 @@ def test_huge_tokens_do_not_touch_rows_that_do_not_see_them():
     assert torch.equal(a[:70], b[:70])  # positions 50..119
     k, v = stored(kk, 4, cache.bands), stored(vv, 4, cache.bands)
     check(x, cache, batch, k, v, scale=0.09e-6)
+
+
+@pytest.mark.parametrize("q", [1, 130])
+def test_graph_captured_on_a_stream_that_is_used_outside_of_it(q):
+    """Split units: launches outside a graph, on the stream it was captured on and before
+    its first replay, and replays agree with a launch on another stream."""
+    n = 5000
+    cache, batch, table = make([n], [q], heads=1)
+    fill(cache, table, [n])
+    x = rows_of(q, 1, 9).cuda()
+    want = paged.attention(x, cache, batch)
+    torch.cuda.synchronize()
+    st, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        a = paged.attention(x, cache, batch)
+        b = paged.attention(x, cache, batch)
+    with torch.cuda.stream(st):
+        c = paged.attention(x, cache, batch)
+    torch.cuda.synchronize()
+    assert torch.equal(c, want)
+    for _ in range(2):
+        a.zero_(), b.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, want) and torch.equal(b, want)
+    assert torch.equal(paged.attention(x, cache, batch), want)
+
+
+def test_refusals():
+    cache, batch, table = make([40, 20], [3, 2], heads=2)
+    q, k = rows_of(5, 4, 1).cuda(), rows_of(5, 2, 2).cuda()
+
+    def refuses(match, fn, *args, exc=ValueError, **kw):
+        with pytest.raises(exc, match=match):
+            fn(*args, **kw)
+
+    refuses("not a multiple", paged.attention, q[:, :3], cache, batch)
+    refuses("q must be", paged.attention, q[:4], cache, batch)
+    refuses("q must be", paged.attention, q[0], cache, batch, exc=TypeError)
+    refuses("bfloat16", paged.attention, q.float(), cache, batch, exc=TypeError)
+    refuses("CPU|cuda", paged.attention, q.cpu(), cache, batch, exc=(RuntimeError, ValueError))
+    refuses("PagedKVCache", paged.attention, q, batch, cache, exc=TypeError)
+    refuses("PagedBatch", cache.append, k, k, table, exc=TypeError)
+    refuses(">= 0", paged.attention, q, cache, batch, window=-1)
+    refuses("window too", paged.attention, q, cache, batch, sink=4)
+    for scale in (0.0, -1.0, float("nan"), float("inf"), 1e-50, 1e39):
+        refuses("softmax_scale", paged.attention, q, cache, batch, softmax_scale=scale)
+    refuses("out must have", paged.attention, q, cache, batch, out=torch.empty(5, 4, 256, device="cuda", dtype=torch.bfloat16)[..., ::2])
+    refuses("k must be", cache.append, k[:4], k, batch)
+    refuses("v must be", cache.append, k, q, batch)
+    other = paged.PagedBatch(table, [40, 20], [3, 2], 32, device="cuda:0")
+    refuses("pages of 32", cache.read, other)
+    far = paged.PagedBatch([[1000, 3, 4], [5, 6, 0]], [40, 20], [3, 2], 16, device="cuda:0")
+    refuses("names page 1000", cache.read, far)
+    early = paged.PagedBatch(table, [40, 20], [41, 2], 16, device="cuda:0")
+    refuses("every new token has a position", cache.append, rows_of(43, 2, 3).cuda(), rows_of(43, 2, 3).cuda(), early)
+    refuses("every new token has a position", cache.read, early, new_only=True)
+    twice = paged.PagedBatch([[0, 1, 2], [3, 2, 0]], [40, 20], [3, 2], 16, device="cuda:0")
+    refuses("more than once", cache.append, k, k, twice)
+    with pytest.raises(ValueError):
+        batch.kv_lens[0] = 7
+    g = torch.cuda.CUDAGraph()
+    fresh = paged.PagedBatch(table, [40, 20], [3, 2], 16, device="cuda:0")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):  # a first use in a capture cannot upload its plan
+        with pytest.raises(RuntimeError, match="before the capture"):
+            paged.attention(q, cache, fresh)
+        y = q + 1
+    assert y.shape == q.shape
