@@ -31,7 +31,7 @@ namespace tiles {
 
 constexpr int BM = 128, BN = 64;
 constexpr int kThreads = 512;
-constexpr int kConvWarp0 = 8, kProdWarp = 12, kMmaWarp = 13, kProdWarpV = 15;
+constexpr int kProdWarp = 12, kMmaWarp = 13, kProdWarpV = 15;
 constexpr uint32_t kTmemCols = 512, kColO = 0, kColS = 256;
 constexpr int kKVTile = BN * D * 2;  // 16 KB: two SWIZZLE_128B atoms (channels 0-63, 64-127)
 constexpr int kAtom = BN * 128;
@@ -53,21 +53,26 @@ struct Geo {
   static_assert(NK <= 4 && NV <= 5, "no tile may be converted before the barrier of the one kReady before it completes");
   static constexpr int kOffK = 0;
   static constexpr int kOffV = kOffK + NK * kKVTile;
+  // Q tile 1, then Q tile 0: an item of one Q tile has two more stages of V in the other's place
+  static constexpr int NV1 = NV + kQTile / kKVTile;
   static constexpr int kOffQ = kOffV + NV * kKVTile;
   static constexpr int kOffCK = kOffQ + 2 * kQTile;
   static constexpr int kOffCV = kOffCK + LK * kStageK;
   static constexpr int kOffBar = (kOffCV + LV * kStageV + 15) / 16 * 16;
   // barriers; index + stages of K for V
   static constexpr int bLdFull = 0, bLdEmpty = bLdFull + LK + LV, bReady = bLdEmpty + LK + LV,
-                       bKvEmpty = bReady + kReady, bQReady = bKvEmpty + NK + NV, bSFull = bQReady + 2,
+                       bKvEmpty = bReady + kReady, bQReady = bKvEmpty + NK + NV1, bSFull = bQReady + 2,
                        bPFull = bSFull + 4, bOReady = bPFull + 4, bOFinal = bOReady + 2, bMmaDone = bOFinal + 2,
                        kNumBars = bMmaDone + 2;
   static constexpr int kOffMisc = (kOffBar + kNumBars * 8 + 15) / 16 * 16;
   // Of the last kExpK key tiles and kExpV value tiles: the exponent taken out of each token,
-  // and a byte per converter warp that says whether there is any. K's of a tile are written
-  // again only after S(j + kExpK - NK), V's after S(j + 2), each issued behind P(j) of
-  // every softmax warp.
-  static constexpr int kExpK = NK + 2, kExpV = NV;
+  // and a byte per converter warp that says whether there is any. A slot is written again
+  // only after softmax step j has ended: tile j + 8 is converted after S(j + 8 - NK) or, with
+  // up to NV1 stages, after S(j + 5) has been found complete by its softmax warps, and with it
+  // every step up to the fifth before it has ended, in each order of the two Q tiles' or
+  // the two shares' steps.
+  static constexpr int kExpK = 8, kExpV = 8;
+  static_assert(kExpK >= NK + 5 && kExpV >= NV1 + 1, "rings of exponents");
   static constexpr int kOffExpK = kOffMisc + 32, kOffExpV = kOffExpK + kExpK * BN;
   static constexpr int kOffWideK = kOffExpV + kExpV * BN, kOffWideV = kOffWideK + 4 * kExpK;
   static constexpr int kSmemBytes = kOffWideV + 4 * kExpV;
@@ -205,7 +210,10 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   const int nq = it.n_rows > BM ? 2 : 1;
   const int n_blk = it.je - it.jb;  // entries of the block list
   const int nkv = (n_blk + 3) / 4;
-  const int n_conv = nq == 2 ? 2 : 4;  // converter warps of a tensor: without a second Q tile its softmax warps help
+  // With one Q tile its two sets of softmax warps share the KV tiles: set (and MMA thread) x
+  // takes tiles x, x + 2, ..., and the two partial results are joined at the end.
+  const bool shared = nq == 1;
+  const int stride = shared ? 2 : 1, n_vs = shared ? GEO::NV1 : NV;
 
   // where row n of the item reads its query and writes its output
   auto place = [&](int n, int64_t& tok, int& h) {
@@ -221,6 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     place(min(n, it.n_rows - 1), tok, h);
     return tok * stride + h * D;
   };
+  auto q_at = [](int x) { return static_cast<uint32_t>(GEO::kOffQ + (1 - x) * kQTile); };
   // A warp's n_out (at most 32) output rows, n0.. of the item, staged in the Q buffer, to
   // global memory: half a warp per row, 256 contiguous bytes.
   auto store_rows = [&](int n0, int n_out) {
@@ -229,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     for (int k = 0; k < n_out / 2; ++k) {
       const int i = 2 * k + (lane >> 4), n = n0 + i, rr = n & (BM - 1), c = lane & 15;
       const int64_t to = __shfl_sync(0xffffffffu, mine, i);
-      const uint32_t stage = sbase + GEO::kOffQ + (n >> 7) * kQTile;
+      const uint32_t stage = sbase + q_at(n >> 7);
       if (n < it.n_rows)
         st_global_v4(a.out + to + 8 * c, ld_shared_v4(stage + (c >> 3) * kQAtom + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)));
     }
@@ -270,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     for (int k = 0; k < 8 * nq; ++k) {
       const int n = 16 * k + (tid >> 4), c = tid & 15, r = n & (BM - 1);
       const int64_t from = __shfl_sync(0xffffffffu, mine, 2 * k + (lane >> 4));
-      const uint32_t dst = sbase + GEO::kOffQ + (n >> 7) * kQTile + (c >> 3) * kQAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+      const uint32_t dst = sbase + q_at(n >> 7) + (c >> 3) * kQAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4);
       uint4 v = make_uint4(0, 0, 0, 0);
       if (n < it.n_rows) v = ld_global_nc_v4(a.q + from + 8 * c);
       const int e = row_exponent(most_of(v));
@@ -285,10 +294,10 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   if (tid == 0) {
     for (int i = 0; i < LK + LV; ++i) {
       mbar_init(&bars[GEO::bLdFull + i], 1);
-      mbar_init(&bars[GEO::bLdEmpty + i], n_conv);
+      mbar_init(&bars[GEO::bLdEmpty + i], 2);  // a tensor's converter warps
     }
-    for (int i = 0; i < NK + NV; ++i) mbar_init(&bars[GEO::bKvEmpty + i], nq);
-    for (int i = 0; i < GEO::kReady; ++i) mbar_init(&bars[GEO::bReady + i], 2 * n_conv);
+    for (int i = 0; i < NK + GEO::NV1; ++i) mbar_init(&bars[GEO::bKvEmpty + i], nq);
+    for (int i = 0; i < GEO::kReady; ++i) mbar_init(&bars[GEO::bReady + i], 4);
     for (int x = 0; x < 2; ++x) {
       mbar_init(&bars[GEO::bQReady + x], 8);  // the eight gathering warps
       mbar_init(&bars[GEO::bSFull + 2 * x], 1);
@@ -320,17 +329,19 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       mbar_arrive(&bars[GEO::bQReady + 1]);
     }
   }
-  if (warp < 4 * nq) {
-    // ------------------------------------------------------------ softmax (Q tile x)
+  if (warp < 8) {
+    // ------------------------------------------------ softmax (Q tile or share of the tiles x)
     const int x = warp >> 2;
     const int r = tid - x * BM;
-    const int n = x * BM + r;
+    const int xq = shared ? 0 : x;  // Q tile
+    const int n = xq * BM + r;
+    const int n_mine = shared ? (nkv - x + 1) / 2 : nkv;  // KV tiles of set x
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tO = tmem + lane_off + kColO + 128 * x;
     const uint32_t tS0 = tmem + lane_off + kColS + 128 * x;
-    const int n_last = min(x * BM + BM, it.n_rows) - 1;
+    const int n_last = min(xq * BM + BM, it.n_rows) - 1;
     const Seen see = seen_by(a, it.start + (it.row0 + min(n, it.n_rows - 1)) / a.group, it.kv_len);
-    const Seen first = seen_by(a, it.start + (it.row0 + x * BM) / a.group, it.kv_len);
+    const Seen first = seen_by(a, it.start + (it.row0 + xq * BM) / a.group, it.kv_len);
     const Seen fin = seen_by(a, it.start + (it.row0 + n_last) / a.group, it.kv_len);
     float m = -1.0e30f, l = 0.0f, F = 0.0f;  // O is kept divided by 2^F
     bool ok = true, s_ready = false;  // s_ready: S of the coming tile was already found complete
@@ -348,11 +359,12 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     }
     // wide_k, wide_v: a byte per converter warp of the tile, and whose rows' exponents count
     auto exps16 = [&](uint32_t wide, uint32_t at, int block) {
-      return (wide >> (8 * (n_conv == 2 ? block >> 1 : block))) & 255u ? ld_shared_v4(at + 16 * block) : make_uint4(0, 0, 0, 0);
+      return (wide >> (8 * (block >> 1))) & 255u ? ld_shared_v4(at + 16 * block) : make_uint4(0, 0, 0, 0);
     };
-    auto step = [&](const int j, const uint32_t wide_k, const uint32_t wide_v, auto masked) -> bool {
+    // step i of this set, tile j
+    auto step = [&](const int i_, const int j, const uint32_t wide_k, const uint32_t wide_v, auto masked) -> bool {
       constexpr bool MASK = decltype(masked)::value;
-      const uint32_t tS = tS0 + 64 * (j & 1);
+      const uint32_t tS = tS0 + 64 * (i_ & 1);
       uint32_t s0[32], s1[32];
       tmem_ld32x2_wait(tS, tS + 32, s0, s1);
       if constexpr (MASK) {
@@ -396,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       bool rescale = false;
       const bool fresh = m < -1.0e29f;
       float alpha = 1.0f;
-      if (j == 0) {
+      if (i_ == 0) {
         m = fmaxf(m, mt);
       } else if (mt > m + 8.0f) {
         rescale = true;
@@ -448,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
           const float Fn = next_f(F, top, fresh);
           if (Fn != F) {
             alpha_o *= ex2f(F - Fn);
-            rescale = j > 0;
+            rescale = i_ > 0;
             F = Fn;
           }
 #pragma unroll
@@ -465,11 +477,11 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       tmem_st16(tS + 16, pw + 16);
       l += sum2.x + sum2.y;
       if (__any_sync(0xffffffffu, rescale)) {
-        // O_x must hold every product up to PV_x(j-1) before it is rescaled: wait for
-        // S_x(j+1), issued behind PV_x(j-1), or at the last tile for the commit behind it
-        const bool tail = j + 1 == nkv;
-        if (!poll_wait_warp(&bars[tail ? GEO::bOReady + x : GEO::bSFull + 2 * x + ((j + 1) & 1)],
-                            tail ? 0u : static_cast<uint32_t>(((j + 1) >> 1) & 1), abort, a.status, lim))
+        // O_x must hold every product up to PV_x(i-1) before it is rescaled: wait for
+        // S_x(i+1), issued behind PV_x(i-1), or at the last tile for the commit behind it
+        const bool tail = i_ + 1 == n_mine;
+        if (!poll_wait_warp(&bars[tail ? GEO::bOReady + x : GEO::bSFull + 2 * x + ((i_ + 1) & 1)],
+                            tail ? 0u : static_cast<uint32_t>(((i_ + 1) >> 1) & 1), abort, a.status, lim))
           return false;
         tc_fence_after();
 #pragma unroll 1
@@ -482,24 +494,30 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         }
         tmem_wait_st();
       }
-      s_ready = j + 1 < nkv && mbar_test(&bars[GEO::bSFull + 2 * x + ((j + 1) & 1)], ((j + 1) >> 1) & 1);
+      s_ready = i_ + 1 < n_mine && mbar_test(&bars[GEO::bSFull + 2 * x + ((i_ + 1) & 1)], ((i_ + 1) >> 1) & 1);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[GEO::bPFull + 2 * x + (j & 1)]);
+      if (lane == 0) mbar_arrive(&bars[GEO::bPFull + 2 * x + (i_ & 1)]);
       return true;
     };
-    for (int j = 0; j < nkv; ++j) {
+    int vs = shared ? x : 0;  // V stage of this set's tile i - 2
+    for (int i = 0; i < n_mine; ++i) {
+      const int j = shared ? 2 * i + x : i;
       if (!__all_sync(0xffffffffu, s_ready) &&
-          !poll_wait_warp(&bars[GEO::bSFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim)) {
+          !poll_wait_warp(&bars[GEO::bSFull + 2 * x + (i & 1)], (i >> 1) & 1, abort, a.status, lim)) {
         ok = false;
         break;
       }
-      // S_x(j) complete: this Q tile no longer reads K stage j, and PV_x(j-2) (issued
-      // before it) is complete: nor V stage j-2
+      // S_x(i) complete: set x no longer reads its K stage, and PV_x(i-2) (issued before
+      // it) is complete: nor that V stage
       if ((warp & 3) == 0 && lane == 0) {
         mbar_arrive(&bars[GEO::bKvEmpty + j % NK]);
-        if (j >= 2) mbar_arrive(&bars[GEO::bKvEmpty + NK + (j - 2) % NV]);
+        if (i >= 2) {
+          mbar_arrive(&bars[GEO::bKvEmpty + NK + vs]);
+          vs += stride;
+          if (vs >= n_vs) vs -= n_vs;
+        }
       }
       tc_fence_after();
       const uint32_t wide_k = *reinterpret_cast<volatile uint32_t*>(smem + GEO::kOffWideK + 4 * (j % GEO::kExpK));
@@ -507,52 +525,98 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       const int e0 = it.jb + 4 * j;
       const int ta = it.block_at(e0) * kBlock, tz = it.block_at(e0 + 3) * kBlock + kBlock;
       const bool whole = e0 + 4 <= it.je && tz <= first.hi && (ta >= fin.lo || tz <= first.kept);
-      ok = __all_sync(0xffffffffu, whole && wide_k == 0 && wide_v == 0 && F == 0.0f) ? step(j, 0, 0, std::false_type{})
-                                                                             : step(j, wide_k, wide_v, std::true_type{});
+      ok = __all_sync(0xffffffffu, whole && wide_k == 0 && wide_v == 0 && F == 0.0f) 
+               ? step(i, j, 0, 0, std::false_type{})
+               : step(i, j, wide_k, wide_v, std::true_type{});
       if (!ok) break;
     }
-    const float of = ex2f(F);
-    const bool done = ok && nkv > 0 && poll_wait_warp(&bars[GEO::bOFinal + x], 0, abort, a.status, lim);
-    if (it.parts > 1) {
-      // one part of a unit: unnormalised O row, m and l for the join. float4 column c of
-      // row r at [c][r]: a warp's 32 rows are contiguous
-      tc_fence_after();
-      float4* dst = reinterpret_cast<float4*>(a.ws) + (static_cast<int64_t>(it.slot + it.part) * 2 + x) * 33 * BM + r;
+    float of = ex2f(F);  // what the row of O is multiplied by, and the other set's
+    float of1 = 0.0f;
+    bool done = ok && n_mine > 0 && poll_wait_warp(&bars[GEO::bOFinal + x], 0, abort, a.status, lim);
+    // Shared tiles: set 1 leaves its row in the stages of K and V, float4 column c of row r
+    // at [c][r] and (m, l) behind them, and set 0 adds it to its own. No MMA reads the
+    // stages any more.
+    const uint32_t other = sbase + GEO::kOffK + r * 16;
+    if (shared && nkv > 0) {
+      if (x == 1) {
+        if (poll_wait_warp(&bars[GEO::bOFinal], 0, abort, a.status, lim)) {
+          tc_fence_after();
 #pragma unroll 1
-      for (int k = 0; k < 4; ++k) {
-        uint32_t o[32];
-        if (done) tmem_ld32_wait(tO + 32 * k, o);
+          for (int k = 0; k < 4 && done; ++k) {
+            uint32_t o[32];
+            tmem_ld32_wait(tO + 32 * k, o);
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          dst[(8 * k + c) * BM] = done ? make_float4(__uint_as_float(o[4 * c]) * of, __uint_as_float(o[4 * c + 1]) * of,
-                                                     __uint_as_float(o[4 * c + 2]) * of, __uint_as_float(o[4 * c + 3]) * of)
-                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      }
-      dst[32 * BM] = make_float4(m, l, 0.0f, 0.0f);
-      __threadfence();
-    } else if (done || (nkv == 0 && poll_wait_warp(&bars[GEO::bQReady + x], 0, abort, a.status, lim))) {
-      // (no tiles: Q_x has landed before its buffer is reused below)
-      tc_fence_after();
-      const float inv = l == 0.0f ? 0.0f : of / l;
-      store_lse(n, m, l);
-      const uint32_t stage = sbase + GEO::kOffQ + x * kQTile;  // Q_x is no longer read
-#pragma unroll 1
-      for (int k = 0; k < 4; ++k) {
-        uint32_t o[32];
-        if (done) {
-          tmem_ld32_wait(tO + 32 * k, o);
-        } else {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] = 0;
+            for (int c = 0; c < 8; ++c)
+              st_shared_v4(other + (8 * k + c) * BM * 16, o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+          }
+          st_shared_v4(other + 32 * BM * 16, __float_as_uint(m), __float_as_uint(l), __float_as_uint(of), 0);
         }
-        float v[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(o[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) stage_chunk(stage, r, 4 * k + c, v + 8 * c, inv);
       }
-      __syncwarp();
-      store_rows(warp * 32, 32);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (x == 0) {
+        const uint4 u = ld_shared_v4(other + 32 * BM * 16);
+        const float m1 = __uint_as_float(u.x), l1 = __uint_as_float(u.y), mx = fmaxf(m, m1);
+        const float f = ex2f(m - mx), f1 = ex2f(m1 - mx);
+        m = mx;
+        l = l * f + l1 * f1;
+        of *= f;
+        of1 = __uint_as_float(u.z) * f1;
+      }
+    }
+    const bool both = shared && nkv > 1;  // set 1 had tiles
+    // 32 columns of the row of O, unnormalised
+    auto fetch = [&](int k, float (&v)[32]) {
+      if (done) {
+        uint32_t o[32];
+        tmem_ld32_wait(tO + 32 * k, o);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(o[c]) * of;
+        if (both) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint4 u = ld_shared_v4(other + (8 * k + c) * BM * 16);
+            v[4 * c] = fmaf(__uint_as_float(u.x), of1, v[4 * c]);
+            v[4 * c + 1] = fmaf(__uint_as_float(u.y), of1, v[4 * c + 1]);
+            v[4 * c + 2] = fmaf(__uint_as_float(u.z), of1, v[4 * c + 2]);
+            v[4 * c + 3] = fmaf(__uint_as_float(u.w), of1, v[4 * c + 3]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = 0.0f;
+      }
+    };
+    if (x < nq) {
+      if (it.parts > 1) {
+        // one part of a unit: unnormalised O row, m and l for the join. float4 column c of
+        // row r at [c][r]: a warp's 32 rows are contiguous
+        tc_fence_after();
+        float4* dst = reinterpret_cast<float4*>(a.ws) + (static_cast<int64_t>(it.slot + it.part) * 2 + x) * 33 * BM + r;
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+          float v[32];
+          fetch(k, v);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) dst[(8 * k + c) * BM] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        }
+        dst[32 * BM] = make_float4(m, l, 0.0f, 0.0f);
+        __threadfence();
+      } else if (done || (nkv == 0 && poll_wait_warp(&bars[GEO::bQReady + x], 0, abort, a.status, lim))) {
+        // (no tiles: Q_x has landed before its buffer is reused below)
+        tc_fence_after();
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        store_lse(n, m, l);
+        const uint32_t stage = sbase + q_at(x);  // Q_x is no longer read
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+          float v[32];
+          fetch(k, v);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) stage_chunk(stage, r, 4 * k + c, v + 8 * c, inv);
+        }
+        __syncwarp();
+        store_rows(warp * 32, 32);
+      }
     }
   } else if (warp < kProdWarp) {
     // ------------------------------------------------------------ converters
@@ -560,8 +624,8 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     // little early, so that softmax step j finds V's exponents as well as K's. A barrier is
     // not reused early: K(j+4) and V(j+4) are converted only after S(j) has completed.
     const int is_v = (warp >> 1) & 1;
-    const int rows = 64 / n_conv;  // of this warp
-    const int t = lane & 3, r0 = ((warp & 1) + (warp < kConvWarp0 ? 2 : 0)) * rows + (lane >> 2);
+    constexpr int rows = 32;  // of this warp
+    const int t = lane & 3, r0 = (warp & 1) * rows + (lane >> 2);
     auto convert = [&](auto conv, uint32_t codes, uint32_t tiles, int n_ld, int n_kv, uint64_t* ld_full, uint64_t* ld_empty,
                        uint64_t* kv_empty, uint8_t* exps, uint8_t* wide, int n_exp, int rec, int stage_bytes) {
       conv.init(t);
@@ -621,10 +685,10 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     // one copy of the loop where K and V have the same format: the instruction caches
     // hold four different loops per sub-partition as it is
     if (KB == VB || !is_v)
-      convert(Converter<L, KB>{}, codes, dst, is_v ? LV : LK, is_v ? NV : NK, ld_full, ld_empty, kv_empty, exps, wide, n_exp,
+      convert(Converter<L, KB>{}, codes, dst, is_v ? LV : LK, is_v ? n_vs : NK, ld_full, ld_empty, kv_empty, exps, wide, n_exp,
               GEO::kRecK, GEO::kStageK);
     else
-      convert(Converter<L, VB>{}, codes, dst, LV, NV, ld_full, ld_empty, kv_empty, exps, wide, n_exp, GEO::kRecV,
+      convert(Converter<L, VB>{}, codes, dst, LV, n_vs, ld_full, ld_empty, kv_empty, exps, wide, n_exp, GEO::kRecV,
               GEO::kStageV);
   } else if (warp == kProdWarp || warp == kProdWarpV) {
     // ------------------------------------------------------------ producers
@@ -655,52 +719,57 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   } else {
     // ------------------------------------------------------------ MMA issuers
     const int x = warp - kMmaWarp;
-    if (lane == 0 && x < nq) {
+    if (lane == 0) {
       constexpr uint32_t idS = idesc_f16(BM, BN, 0);
       constexpr uint32_t idPV = idesc_f16(BM, D, 1);
       const uint32_t tS0 = tmem + kColS + 128 * x, tO = tmem + kColO + 128 * x;
       // descriptors address shared memory in units of 16 bytes
-      const uint64_t dq = smem_desc_sw128(sbase + GEO::kOffQ + x * kQTile, 16, 1024);
+      const uint64_t dq = smem_desc_sw128(sbase + q_at(shared ? 0 : x), 16, 1024);
       const uint64_t dk = smem_desc_sw128(sbase + GEO::kOffK, 16, 1024);
       const uint64_t dv = smem_desc_sw128(sbase + GEO::kOffV, kAtom, 1024);
-      auto issue_s = [&](int j) {
-        const uint64_t k = dk + static_cast<uint64_t>((j % NK) * (kKVTile >> 4));
+      const int n_mine = shared ? (nkv - x + 1) / 2 : nkv;
+      auto tile = [&](int i) { return shared ? 2 * i + x : i; };
+      auto issue_s = [&](int i) {
+        const uint64_t k = dk + static_cast<uint64_t>((tile(i) % NK) * (kKVTile >> 4));
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          mma_bf16_ss(tS0 + 64 * (j & 1), dq + (((kk >> 2) * kQAtom + (kk & 3) * 32) >> 4),
+          mma_bf16_ss(tS0 + 64 * (i & 1), dq + (((kk >> 2) * kQAtom + (kk & 3) * 32) >> 4),
                       k + (((kk >> 2) * kAtom + (kk & 3) * 32) >> 4), idS, kk > 0);
-        mma_commit(&bars[GEO::bSFull + 2 * x + (j & 1)]);
+        mma_commit(&bars[GEO::bSFull + 2 * x + (i & 1)]);
       };
-      auto issue_pv = [&](int j) {
-        const uint64_t v = dv + static_cast<uint64_t>((j % NV) * (kKVTile >> 4));
-        const uint32_t p = tS0 + 64 * (j & 1);
+      int vs = shared ? x : 0;
+      auto issue_pv = [&](int i) {
+        const uint64_t v = dv + static_cast<uint64_t>(vs * (kKVTile >> 4));
+        const uint32_t p = tS0 + 64 * (i & 1);
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          mma_bf16_ts(tO, p + 8 * kk, v + ((kk * 2048) >> 4), idPV, (j > 0 || kk > 0) ? 1u : 0u);
+          mma_bf16_ts(tO, p + 8 * kk, v + ((kk * 2048) >> 4), idPV, (i > 0 || kk > 0) ? 1u : 0u);
+        vs += stride;
+        if (vs >= n_vs) vs -= n_vs;
       };
-      auto wait_ready = [&](int j) {
-        return poll_wait(&bars[GEO::bReady + j % GEO::kReady], (j / GEO::kReady) & 1, abort, a.status, lim);
-      };
-      bool ok = nkv > 0 && poll_wait(&bars[GEO::bQReady + x], 0, abort, a.status, lim);
-      for (int j = 0; j < 2 && j < nkv && ok; ++j) {
-        if (!(ok = wait_ready(j))) break;
+      auto ready_at = [&](int i) { return &bars[GEO::bReady + tile(i) % GEO::kReady]; };
+      auto ready_phase = [&](int i) { return static_cast<uint32_t>((tile(i) / GEO::kReady) & 1); };
+      auto wait_ready = [&](int i) { return poll_wait(ready_at(i), ready_phase(i), abort, a.status, lim); };
+      bool ok = n_mine > 0 && poll_wait(&bars[GEO::bQReady + x], 0, abort, a.status, lim);
+      for (int i = 0; i < 2 && i < n_mine && ok; ++i) {
+        if (!(ok = wait_ready(i))) break;
         tc_fence_after();
-        issue_s(j);
+        issue_s(i);
       }
       // A test of a barrier takes this thread over 100 cycles even where its phase has
       // completed, and a tile's issue is what it has time for: the next tile's is tested
-      // before S(j+2) is issued, and waited for only if that failed.
-      bool ready = nkv > 2 && ok && mbar_test(&bars[GEO::bReady + 2], 0);
-      for (int j = 0; j < nkv && ok; ++j) {
-        if (!(ok = poll_wait(&bars[GEO::bPFull + 2 * x + (j & 1)], (j >> 1) & 1, abort, a.status, lim))) break;
+      // before S(i+2) is issued, and waited for only if that failed.
+      bool ready = n_mine > 2 && ok && mbar_test(ready_at(2), ready_phase(2));
+      for (int i = 0; i < n_mine && ok; ++i) {
+        if (!(ok = poll_wait(&bars[GEO::bPFull + 2 * x + (i & 1)], (i >> 1) & 1, abort, a.status, lim))) break;
         tc_fence_after();
-        issue_pv(j);
-        if (j + 2 < nkv) {
-          if (!ready && !(ok = wait_ready(j + 2))) break;
-          ready = j + 3 < nkv && mbar_test(&bars[GEO::bReady + (j + 3) % GEO::kReady], ((j + 3) / GEO::kReady) & 1);
+        issue_pv(i);
+        if (i + 2 < n_mine) {
+          if (!ready && !(ok = wait_ready(i + 2))) break;
+          ready = i + 3 < n_mine && mbar_test(ready_at(i + 3), ready_phase(i + 3));
           tc_fence_after();
-          issue_s(j + 2);
-        } else if (j + 2 == nkv) {
+          issue_s(i + 2);
+        } else if (i + 2 == n_mine) {
           mma_commit(&bars[GEO::bOReady + x]);
         }
       }
@@ -744,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       }
       const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
       if (c0 == 0) store_lse(n, mx, lsum);
-      const uint32_t stage = sbase + GEO::kOffQ + x * kQTile;
+      const uint32_t stage = sbase + q_at(x);
 #pragma unroll 1
       for (int g = c0; g < c0 + n_col; g += 8) {
         float acc[32];
