@@ -6,7 +6,7 @@
 // storage blocks; a KV tile is four consecutive entries of that list (64 tokens), so the
 // kept first tokens and a sliding window need no tokens between them.
 //   warps 0-3 / 4-7  softmax of Q tile 0 / 1: thread r owns row r (TMEM lane r); all
-//                    eight first gather the Q rows (cp.async into the MMA's layout)
+//                    eight first gather the Q rows into the MMA's layout
 //   warps 8-9/10-11  converters of K / V: four lanes per row, 32 channels each, codes and
 //                    scales from the staged records to 128B-swizzled fp16 tiles
 //   warps 12 / 15    producers of K / V: a storage block is contiguous, one bulk copy
@@ -15,7 +15,9 @@
 // The pipeline is that of the contiguous-window attention kernel (S double-buffered,
 // S_x(j+2) issued behind PV_x(j), one commit per tile and Q tile, K and V as separate
 // streams): see there for what was measured. What differs: rows of different lengths
-// of sight. A tile that some row of the Q tile does not see whole takes a masked step
+// of sight, and items of one Q tile, whose two softmax sets take turns with the KV tiles and
+// join their results at the end (24 to 72 rows over 12480 tokens, int4: 188 us for 148 such
+// items; one set, the other's warps converting too: 218). A tile that some row of the Q tile does not see whole takes a masked step
 // (a 64-bit mask per row; a masked logit is -inf); the running maximum starts at -1e30,
 // so a row without any visible token ends with l = 0 and is stored as 0.
 // Roundings: Q, K, V and P are fp16 for the MMAs (K and V exact for int4 codes; see
@@ -111,30 +113,38 @@ struct Converter {
       }
     }
   }
-  // One row: record block `rec`, row `rr` of it, to row r of the tile at dst. EXACT: takes a
-  // power of two out of a row beyond (kScaleLeast, kScaleMost) and returns its exponent;
-  // else converts as if there were none and keeps this lane's extremes of live rows' scales.
-  template <bool EXACT>
-  __device__ __forceinline__ int row(uint32_t rec, int rr, uint32_t dst, int r, int t, bool live, uint32_t& least,
-                                     uint32_t& most) const {
+  // This lane's codes and scales of one row: row rr of record block `rec`.
+  struct Raw {
+    uint32_t w[BITS], x[KG];  // 4 or 8 words of codes
+  };
+  __device__ __forceinline__ Raw load(uint32_t rec, int rr, int t) const {
     using R = Rec<L, BITS>;
-    uint32_t w[BITS];  // 4 or 8 words of codes
+    Raw u;
     const uint32_t src = rec + rr * R::CW + t * (R::CW / 4);
 #pragma unroll
     for (int i = 0; i < BITS / 4; ++i) {
       const uint4 v = ld_shared_v4(src + 16 * i);
-      w[4 * i] = v.x;
-      w[4 * i + 1] = v.y;
-      w[4 * i + 2] = v.z;
-      w[4 * i + 3] = v.w;
+      u.w[4 * i] = v.x;
+      u.w[4 * i + 1] = v.y;
+      u.w[4 * i + 2] = v.z;
+      u.w[4 * i + 3] = v.w;
     }
     const uint32_t sc = rec + R::kCodes + rr * L::G * 2;
-    uint32_t x[KG], top = 0;
 #pragma unroll
-    for (int q = 0; q < KG; ++q) {
-      x[q] = ld_shared_u16(sc + 2 * (KG == 1 ? base : min(base + q, L::G - 1)));
-      top = max(top, x[q]);
-    }
+    for (int q = 0; q < KG; ++q) u.x[q] = ld_shared_u16(sc + 2 * (KG == 1 ? base : min(base + q, L::G - 1)));
+    return u;
+  }
+  // One loaded row, to row r of the tile at dst. EXACT: takes a power of two out of a row
+  // beyond (kScaleLeast, kScaleMost) and returns its exponent; else converts as if there
+  // were none and keeps this lane's extremes of live rows' scales.
+  template <bool EXACT>
+  __device__ __forceinline__ int row(const Raw& u, uint32_t dst, int r, int t, bool live, uint32_t& least,
+                                     uint32_t& most) const {
+    const uint32_t (&w)[BITS] = u.w;
+    const uint32_t (&x)[KG] = u.x;
+    uint32_t top = 0;
+#pragma unroll
+    for (int q = 0; q < KG; ++q) top = max(top, x[q]);
     float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int q = 0; q < KG; ++q) f[q] = live ? __uint_as_float(x[q] << 16) : 0.0f;  // rows past the end hold anything
@@ -641,15 +651,19 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         }
         const uint32_t dst = tiles + ks * kKVTile;
         uint32_t least = kScaleLeast, most = 0;
-        auto convert_rows = [&](auto exact) {
+        auto convert_rows = [&](auto exact, auto unroll) {
           constexpr bool EXACT = decltype(exact)::value;
           int any = 0;
-#pragma unroll(EXACT ? 1 : 2)
+          auto load = [&](int r) { return conv.load(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, t); };
+          auto next = load(r0);
+#pragma unroll(decltype(unroll)::value)
           for (int p = 0; p < rows; p += 8) {
+            // the next row's loads are in flight while this one is converted
             const int r = r0 + p, e = it.jb + 4 * j + (r >> 4);
+            const auto raw = next;
+            if (p + 8 < rows) next = load(r + 8);
             const bool live = e < it.je && it.block_at(e) * kBlock + (r & 15) < it.kv_len;
-            const int x = conv.template row<EXACT>(codes + ls * stage_bytes + (r >> 4) * rec, r & 15, dst, r, t, live, least,
-                                                   most);
+            const int x = conv.template row<EXACT>(raw, dst, r, t, live, least, most);
             if constexpr (EXACT) {
               any |= x;
               if (t == 0) exps[slot * BN + r] = static_cast<uint8_t>(x);
@@ -657,9 +671,14 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
           }
           return any;
         };
-        int any = convert_rows(std::false_type{});
+        // The conversion is what items of one Q tile wait for, and four rows at a time have the
+        // most in flight (165 us, one at a time 205, for 195 tiles in each of 148 items); two Q
+        // tiles wait for their softmax, and the shorter loop is easier on the instruction
+        // caches (2000 new tokens over 18720: 797 us, four at a time 814).
+        int any = shared ? convert_rows(std::false_type{}, std::integral_constant<int, 4>{})
+                         : convert_rows(std::false_type{}, std::integral_constant<int, 1>{});
         if (__any_sync(0xffffffffu, most > kScaleMost || least < kScaleLeast))
-          any = __any_sync(0xffffffffu, convert_rows(std::true_type{}) != 0);
+          any = __any_sync(0xffffffffu, convert_rows(std::true_type{}, std::integral_constant<int, 1>{}) != 0);
         if (lane == 0) wide[4 * slot + r0 / rows] = static_cast<uint8_t>(any);
         uint64_t* const read = &ld_empty[ls];
         if (++ls == n_ld) ls = 0, ld_phase ^= 1;
