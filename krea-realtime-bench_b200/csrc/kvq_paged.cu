@@ -111,7 +111,10 @@ __device__ __noinline__ void fix_slow(const uint4* tin, int r, uint32_t slow_mas
   }
 }
 
-// Bound by memory at many tokens, by latency at few. One CTA per tile of 16 tokens
+// Bound by latency at few tokens; at many by memory and the quantization's instructions
+// alike (4680 tokens of 40 heads, bands4: 123 MB in 30 us, 4.1 TB/s, 69 % of the issue
+// slots; 24 single tokens of 8 heads, with the read of what was stored: 6.7 us on the
+// device). One CTA per tile of 16 tokens
 // (one storage block) x 8 heads of K or V: the rows arrive by cp.async (a token's heads
 // are contiguous: 2 KB runs), thread r quantizes row r = 16 head + token, and each head's
 // record, contiguous in its page, is written with 16-byte stores; a block that the step
@@ -215,7 +218,8 @@ struct ReadArgs {
   int64_t stride[2];
 };
 
-// Bound by memory: one CTA per storage block, K and V of all heads, 16 lanes per row and
+// Bound by memory (32760 tokens of 40 heads, bands4: 902 MB in 165 us, 5.46 TB/s, 83 % of
+// what a copy reaches). One CTA per storage block and tensor, all heads, 16 lanes per row and
 // eight channels per lane, so a warp reads contiguous codes and writes 256-byte rows.
 // kHeadsAtOnce heads are loaded before the first is converted. An aligned run of eight
 // channels meets at most two groups.

@@ -1,5 +1,12 @@
 // Attention of many query rows per KV head over the paged quantized cache (sm_100a):
-// prompt chunks, denoising blocks. Tensor-bound: tcgen05.mma with TMEM accumulators.
+// prompt chunks, denoising blocks, drafts of grouped heads: tcgen05.mma with TMEM
+// accumulators. Bound by the softmax step of a warp (~1700 of a 64-token tile's ~2000
+// cycles: S out of TMEM, maximum, exponentials, P into TMEM), which the MMAs of the other Q
+// tile overlap, and under a long load by the power limit. Measured: 4680 queries of 40
+// heads over 32760 tokens 3.4 to 3.75 ms by the clock that the power left (835 to 925
+// TFLOP/s), 2000 queries of 40 heads over 18720 tokens, causal, 0.79 to 0.85 ms; 12
+// sequences with 4 to 6 new tokens, 8 query heads per KV head, 2705 to 6240 tokens, int8:
+// 40.5 us, of which ~15 are launch, set-up, first tiles and the join.
 //
 // One CTA of 16 warps per item of the plan: up to 256 rows (two Q tiles of 128) of a
 // sequence and KV head, row = query * group + grouped head, over its list of 16-token
