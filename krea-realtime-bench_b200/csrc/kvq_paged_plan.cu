@@ -41,13 +41,27 @@ struct Plan {
   int units = 0, slots = 0, tile_slots = 0, row_tile = 8, row_ctas = 0;
 };
 
-// Few rows. With more work than the resident blocks can share in pieces of kMinBlocks
-// storage blocks, the units are one line of blocks (an empty unit counts as one), cut
-// into equal pieces, one per resident block: every block streams the same number of
-// bytes whatever the lengths are; a piece is made of the whole or partial units it meets.
-// With less, each unit is cut by itself into equal parts, so that a block has one item and
-// waits for its data once. No unit gets more than kMaxParts parts.
-constexpr int kMinBlocks = 16;
+// Few rows. Two ways to cut the units, by an estimate in microseconds of the blocks'
+// work: rounds of kRound storage blocks (two for each warp of a block of threads), the
+// join of a unit's parts, and what any join costs; for 8 and 16 rows, fitted to graph
+// replays of 1 to 8 sequences of 400 to 8000 tokens, 8 KV heads.
+// - Each unit by itself into equal parts, of which all are resident at once: a block of
+//   threads has one item and waits for its data once.
+// - The units as one line of storage blocks (an empty unit counts as one), cut into equal
+//   pieces, one per resident block of threads: each streams the same number of bytes
+//   whatever the lengths are; a piece is made of the whole or partial units it meets, two
+//   joins in the common case.
+// Measured: 8 sequences of 3000 tokens by units 15.7 us, as a line 18.9; one of 8000 in 16
+// parts a head 11.8, in 32 12.9; one of 400 whole 7.3, in two parts 8.6; one of 1561 in 7
+// parts 8.5, in 4 11.0. No unit gets more than kMaxParts parts.
+constexpr int kRound = 8;
+constexpr double kRoundCost[2] = {1.4, 1.9}, kRowPart[2] = {0.17, 0.44}, kRowJoin = 3.0;
+
+static double row_cost(int row_tile, int64_t piece, int64_t parts) {
+  const int w = row_tile > 8;
+  return kRoundCost[w] * static_cast<double>((piece + kRound - 1) / kRound) +
+         (parts > 1 ? kRowJoin + kRowPart[w] * static_cast<double>(parts) : 0.0);
+}
 
 static void cut_rows(const std::vector<Unit>& units, int n_heads, int64_t n_resident, Plan* p) {
   int64_t total = 0, longest = 0;
@@ -56,14 +70,30 @@ static void cut_rows(const std::vector<Unit>& units, int n_heads, int64_t n_resi
     longest = std::max<int64_t>(longest, u.n);
   }
   if (total == 0) return;
-  const int64_t piece = std::max<int64_t>(
-      {(total + n_resident - 1) / n_resident, kMinBlocks, (longest + kMaxParts - 2) / (kMaxParts - 1)});
+  int64_t piece = std::max<int64_t>(
+      {(total + n_resident - 1) / n_resident, 2 * kRound, (longest + kMaxParts - 2) / (kMaxParts - 1)});
   const int64_t n_ctas = (total + piece - 1) / piece;
+  // the line, as two items a block of threads
+  double least = row_cost(p->row_tile, piece + kRound, (longest + piece - 1) / piece + 1) + kRowJoin;
+  int64_t by_unit = 0;  // piece of the first way
+  if (static_cast<int64_t>(units.size()) * n_heads <= n_resident) {
+    for (int64_t c = 2 * kRound; c < longest + kRound; c += kRound) {
+      const int64_t parts = (longest + c - 1) / c;
+      const double cost = row_cost(p->row_tile, (longest + parts - 1) / parts, parts);
+      if (parts > kMaxParts || cost >= least) continue;
+      int64_t all = 0;
+      for (const Unit& u : units) all += std::max<int64_t>(1, (u.n + c - 1) / c) * n_heads;
+      if (all > n_resident) continue;
+      least = cost;
+      by_unit = c;
+    }
+    if (longest == 0) by_unit = kRound;  // nothing to see: the rows still have to be written
+  }
   p->rows.reserve(units.size() * n_heads + n_ctas);
-  if (total < n_resident * kMinBlocks) {
+  if (by_unit) {
     for (const Unit& u : units)
       for (int h = 0; h < n_heads; ++h) {
-        const int64_t parts = std::max<int64_t>(1, (u.n + piece - 1) / piece);
+        const int64_t parts = std::max<int64_t>(1, (u.n + by_unit - 1) / by_unit);
         for (int64_t k = 0; k < parts; ++k)
           p->rows.push_back(make_item(u, h, u.n * k / parts, u.n * (k + 1) / parts, static_cast<int>(k),
                                       static_cast<int>(parts), p->units, p->slots));
@@ -190,27 +220,53 @@ static void cut_tiles(std::vector<Unit>& units, int n_heads, int n_sms, Plan* p)
   }
 }
 
-// Up to kFewRows rows of a sequence and KV head go to the kernel for few rows.
-constexpr int kFewRows = 16;
+// Up to kFewRows rows of a sequence and KV head go to the kernel for few rows: 16 rows,
+// 64 sequences of 946 to 16384 tokens, 8 KV heads 253 us, on the other kernel 401. Up to
+// kMidRows do, in tiles of 16 rows that each read the cache, where all sequences are such
+// and the work is at most kMidBlocks storage blocks per resident block of threads: 24 rows,
+// one sequence of 1561 tokens 13.1 us, on the other kernel 21.9; of 8000 tokens 19.5, 32.6;
+// 8 sequences of 3000 tokens (81 blocks) 34.7 both; 64 long ones 487, 402.
+constexpr int kFewRows = 16, kMidRows = 64, kMidBlocks = 48;
 
 static int make_plan(const kvq_paged_cache* c, int layout, const int32_t* kv_lens, const int32_t* q_lens, int n_seqs,
                      int group, int causal, int64_t window, int64_t sink, int n_sms, Plan* p) {
-  std::vector<Unit> few, many;
-  int64_t q_first = 0;
+  auto resident = [&](int row_tile) {
+    return static_cast<int64_t>(n_sms) * rows_ctas_per_sm(layout, c->k_bits, c->v_bits, row_tile);
+  };
+  int64_t most = 0, q_sum = 0;  // rows of a sequence and KV head, queries
   for (int s = 0; s < n_seqs; ++s) {
-    const int64_t rows = static_cast<int64_t>(q_lens[s]) * group;
-    const int tile = rows <= kFewRows ? kFewRows : kTileRows;
-    for (int64_t r = 0; r < rows; r += tile) {
-      const int n = static_cast<int>(std::min<int64_t>(tile, rows - r));
-      (rows <= kFewRows ? few : many)
-          .push_back(make_unit(s, kv_lens[s], q_lens[s], q_first, group, static_cast<int>(r), n, causal, window, sink));
-      if (rows <= kFewRows && rows > 8) p->row_tile = 16;
-    }
-    q_first += q_lens[s];
+    most = std::max(most, static_cast<int64_t>(q_lens[s]) * group);
+    q_sum += q_lens[s];
   }
-  KVQ_REQUIRE(static_cast<int64_t>(few.size() + many.size()) * c->n_heads < (1 << 24) && q_first < ((int64_t)1 << 31),
-              KVQ_ERR_ARG, "too many rows for one launch");
-  cut_rows(few, c->n_heads, static_cast<int64_t>(n_sms) * rows_ctas_per_sm(layout, c->k_bits, c->v_bits, p->row_tile), p);
+  KVQ_REQUIRE(q_sum < ((int64_t)1 << 31), KVQ_ERR_ARG, "too many rows for one launch");
+  std::vector<Unit> few, many;
+  auto split = [&](int64_t limit) {
+    few.clear();
+    many.clear();
+    int64_t q_first = 0, blocks = 0;
+    for (int s = 0; s < n_seqs; ++s) {
+      const int64_t rows = static_cast<int64_t>(q_lens[s]) * group;
+      const int tile = rows <= limit ? kFewRows : kTileRows;
+      for (int64_t r = 0; r < rows; r += tile) {
+        const int n = static_cast<int>(std::min<int64_t>(tile, rows - r));
+        const Unit u = make_unit(s, kv_lens[s], q_lens[s], q_first, group, static_cast<int>(r), n, causal, window, sink);
+        (rows <= limit ? few : many).push_back(u);
+        if (rows <= limit) blocks += u.n;
+        if (rows <= limit && rows > 8) p->row_tile = 16;
+      }
+      q_first += q_lens[s];
+    }
+    return blocks * c->n_heads;
+  };
+  if (most <= kFewRows || most > kMidRows) {
+    split(kFewRows);
+  } else if (split(kMidRows) > kMidBlocks * resident(16)) {
+    p->row_tile = 8;
+    split(kFewRows);
+  }
+  KVQ_REQUIRE(static_cast<int64_t>(few.size() + many.size()) * c->n_heads < (1 << 24), KVQ_ERR_ARG,
+              "too many rows for one launch");
+  cut_rows(few, c->n_heads, resident(p->row_tile), p);
   cut_tiles(many, c->n_heads, n_sms, p);
   return KVQ_OK;
 }

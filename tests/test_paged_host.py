@@ -125,7 +125,7 @@ def test_plan_covers_every_row_and_block_once(libkvq, kv, q, group, causal, wind
         for it in items:
             s, h, row0, n_rows, n_sink, first, jb, je, part, parts, unit, slot, kv_len, start, qf, _ = (int(x) for x in it)
             assert 1 <= n_rows <= most and kv_len == kv[s] and start == kv[s] - q[s] and qf == q_first[s]
-            assert (q[s] * group <= 16) == (kind == 0)
+            assert kind == 0 if q[s] * group <= 16 else q[s] * group <= 64 or kind == 1
             by_unit.setdefault((s, h, row0, n_rows), []).append((part, parts, jb, je, n_sink, first, unit, slot))
         for (s, h, row0, n_rows), parts in by_unit.items():
             seen[s, h][row0:row0 + n_rows] += 1
@@ -165,10 +165,10 @@ def start_of(kv, q):
 
 
 def test_plan_shares_the_work(libkvq):
-    """A long sequence with one row occupies every block that can be resident, and a
-    ragged batch gives each the same number of storage blocks."""
+    """A long sequence with one row is shared by about as many blocks of threads as there
+    are SMs, and a ragged batch gives each the same number of storage blocks."""
     _, info, few, _, cta_first = plan_of(libkvq, [200000], [1], n_heads=1)
-    assert info.n_row_ctas >= 120 and len(few) == info.n_row_ctas
+    assert info.n_row_ctas >= 100 and len(few) == info.n_row_ctas
     lens = (np.arange(1, 200) * 977) % 9000 + 1
     _, info, few, _, cta_first = plan_of(libkvq, lens, [1] * len(lens), n_heads=2)
     work = np.add.reduceat(few[:, 7] - few[:, 6], cta_first[:-1])
