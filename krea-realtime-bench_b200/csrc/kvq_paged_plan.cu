@@ -224,9 +224,11 @@ static void cut_tiles(std::vector<Unit>& units, int n_heads, int n_sms, Plan* p)
 // 64 sequences of 946 to 16384 tokens, 8 KV heads 253 us, on the other kernel 401. Up to
 // kMidRows do, in tiles of 16 rows that each read the cache, where all sequences are such
 // and the work is at most kMidBlocks storage blocks per resident block of threads: 24 rows,
-// one sequence of 1561 tokens 13.1 us, on the other kernel 21.9; of 8000 tokens 19.5, 32.6;
-// 8 sequences of 3000 tokens (81 blocks) 34.7 both; 64 long ones 487, 402.
-constexpr int kFewRows = 16, kMidRows = 64, kMidBlocks = 48;
+// one sequence of 1561 tokens 13.1 us, on the other kernel 21.9; 64 rows, one of 8000 tokens
+// (54 blocks) 24.4, 33.4; 8 sequences of 3000 tokens, 24 rows (81 blocks) 31.7, 34.6; 8 of
+// 1500, 64 rows (81) 27.5, 25.7; 12 with 32 to 48 rows, int8 (126) 44.8, 39.3. Rows on both
+// sides of 16 cost two launches else: 12 sequences with 16 to 24 rows 31.1, 51.7.
+constexpr int kFewRows = 16, kMidRows = 64, kMidBlocks = 80;
 
 static int make_plan(const kvq_paged_cache* c, int layout, const int32_t* kv_lens, const int32_t* q_lens, int n_seqs,
                      int group, int causal, int64_t window, int64_t sink, int n_sms, Plan* p) {
