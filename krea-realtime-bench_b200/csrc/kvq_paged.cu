@@ -112,9 +112,9 @@ __device__ __noinline__ void fix_slow(const uint4* tin, int r, uint32_t slow_mas
 }
 
 // Bound by latency at few tokens; at many by memory and the quantization's instructions
-// alike (4680 tokens of 40 heads, bands4: 123 MB in 30 us, 4.1 TB/s, 69 % of the issue
-// slots; 24 single tokens of 8 heads, with the read of what was stored: 6.7 us on the
-// device). One CTA per tile of 16 tokens
+// alike (4680 tokens of 40 heads, bands4: 129 MB in 29.4 us, 4.4 TB/s, 69 % of the issue
+// slots; 9 prompts of 129 to 1531 tokens, 10 heads, int8: 14.0 us; 24 single tokens of 8
+// heads 3.5 us on the device). One CTA per tile of 16 tokens
 // (one storage block) x 8 heads of K or V: the rows arrive by cp.async (a token's heads
 // are contiguous: 2 KB runs), thread r quantizes row r = 16 head + token, and each head's
 // record, contiguous in its page, is written with 16-byte stores; a block that the step

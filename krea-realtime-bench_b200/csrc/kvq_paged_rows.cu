@@ -2,7 +2,7 @@
 // single tokens, short drafts. Every K and V record of a KV head is read once for all its
 // rows. Memory-bound with int8 records; with int4 ones, of half the bytes and as many
 // instructions, bound by the issue slots (64 % used, and the ALU 53 %). Measured, 64
-// sequences of 946 to 16384 tokens, 8 KV heads, 40 query heads: int4 636 MB in 173 us
+// sequences of 946 to 16384 tokens, 8 KV heads, 40 query heads: int4 636 MB in 173 to 177 us
 // (3.7 TB/s), int8 5.75 TB/s of the 6.55 that a copy reaches; two sequences of 107 and 131
 // thousand tokens, int8 K and int4 V: 571 MB in 131 us (4.3 TB/s).
 //

@@ -3,8 +3,8 @@
 // accumulators. Bound by the softmax step of a warp (~1700 of a 64-token tile's ~2000
 // cycles: S out of TMEM, maximum, exponentials, P into TMEM), which the MMAs of the other Q
 // tile overlap, and under a long load by the power limit. Measured: 4680 queries of 40
-// heads over 32760 tokens 3.4 to 3.75 ms by the clock that the power left (835 to 925
-// TFLOP/s), 2000 queries of 40 heads over 18720 tokens, causal, 0.79 to 0.85 ms; 12
+// heads over 32760 tokens 3.4 to 3.85 ms by the clock that the power left (815 to 925
+// TFLOP/s), 2000 queries of 40 heads over 18720 tokens, causal, 0.79 to 0.87 ms; 12
 // sequences with 4 to 6 new tokens, 8 query heads per KV head, 2705 to 6240 tokens, int8:
 // 40.5 us, of which ~15 are launch, set-up, first tiles and the join.
 //
