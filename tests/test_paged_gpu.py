@@ -537,3 +537,29 @@ def test_refusals():
             paged.attention(q, cache, fresh)
         y = q + 1
     assert y.shape == q.shape
+
+
+@pytest.mark.parametrize("group", [5, 8, 11, 21])
+@pytest.mark.parametrize("kv", [[300, 17, 1000, 0, 3], [2500, 4000, 90, 1, 64], [40000, 30000, 35000, 38000, 2]])
+@pytest.mark.parametrize("k_bits,v_bits,mode", [(4, 4, "blind32"), (8, 8, "bands")])
+def test_rows_between_the_two_kernels(group, kv, k_bits, v_bits, mode):
+    """10 to 63 rows per KV head beside sequences with none and with one query: tiles of 16
+    rows or of 128, by the lengths, whole and in parts."""
+    q = [2, 3, 3, 0, 1]
+    cache, batch, table = make(kv, q, heads=1 if kv[0] > 10000 else 2, page=32, k_bits=k_bits, v_bits=v_bits, mode=mode)
+    k, v = fill(cache, table, kv)
+    x = torch.randn(sum(q), cache.n_heads * group, 128).bfloat16().cuda()
+    check(x, cache, batch, k, v)
+    check(x, cache, batch, k, v, window=333, sink=40)
+
+
+@pytest.mark.parametrize("rows", [17, 64, 65, 127, 128, 129])
+@pytest.mark.parametrize("n", [64, 65, 128, 129, 192, 640, 9000])
+def test_one_q_tile_takes_turns(rows, n):
+    """Few and many key tiles, odd and even, whole and in parts; more sequences than the kernel
+    for few rows takes at the longer ones."""
+    seqs = 24 if n == 9000 else 3
+    kv = [n] * seqs
+    cache, batch, table = make(kv, [rows] * seqs, heads=1, page=64, mode="bands2", k_bits=8)
+    k, v = fill(cache, table, kv)
+    check(torch.randn(rows * seqs, 1, 128).bfloat16().cuda(), cache, batch, k, v)
