@@ -58,12 +58,12 @@ struct Geo {
   static constexpr int kStageK = 4 * kRecK, kStageV = 4 * kRecV;
   static constexpr int NK = 3, NV = VB == 8 ? 4 : 5;
   static constexpr int LK = KB == 8 ? 2 : 3, LV = KB == 8 ? 2 : 3;
-  static constexpr int kReady = 4;
-  static_assert(NK <= 4 && NV <= 5, "no tile may be converted before the barrier of the one kReady before it completes");
+  static constexpr int kReady = 8;  // see at the converters
   static constexpr int kOffK = 0;
   static constexpr int kOffV = kOffK + NK * kKVTile;
   // Q tile 1, then Q tile 0: an item of one Q tile has two more stages of V in the other's place
   static constexpr int NV1 = NV + kQTile / kKVTile;
+  static_assert(NK < kReady && NV1 < kReady, "no tile may be converted before the barrier of the one kReady before it completes");
   static constexpr int kOffQ = kOffV + NV * kKVTile;
   static constexpr int kOffCK = kOffQ + 2 * kQTile;
   static constexpr int kOffCV = kOffCK + LK * kStageK;
@@ -638,8 +638,11 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   } else if (warp < kProdWarp) {
     // ------------------------------------------------------------ converters
     // K(j) and V(j) count on one barrier, which the MMA threads wait for before S(j): V a
-    // little early, so that softmax step j finds V's exponents as well as K's. A barrier is
-    // not reused early: K(j+4) and V(j+4) are converted only after S(j) has completed.
+    // little early, so that softmax step j finds V's exponents as well as K's. An arrival
+    // does not say whose it is, so no warp may arrive for tile j + kReady before all four
+    // have for tile j: with fewer stages than kReady, a tile j + kReady takes a stage that a
+    // tile behind j had, which is free only after that tile's S, and all four warps, each
+    // in the order of the tiles, have arrived for it.
     const int is_v = (warp >> 1) & 1;
     constexpr int rows = 32;  // of this warp
     const int t = lane & 3, r0 = (warp & 1) * rows + (lane >> 2);
