@@ -105,11 +105,14 @@ __device__ __forceinline__ uint32_t int8_pair(uint32_t x) {
 // The attention multiplies in fp16 rather than bf16: an int4 code times a bf16 scale has
 // eleven significant bits, which fp16 holds and bf16 rounds to eight; with bf16 products
 // the output's error against 64 bits was 3.7e-3, of which the rounding of the output is
-// 1.7e-3. fp16 ends at 65504 and thins out below 2^-14, so a token whose largest key or
-// value scale lies beyond [kScaleLeast, kScaleMost] is multiplied as if its scales were
-// 2^-e times as large, and a query row likewise: logits get the power of two back in
-// fp32, softmax weights get a value's, relative to a power of two F that each output row
-// keeps for itself. Tokens and rows that have none keep their bits.
+// 1.7e-3. fp16 ends at 65504 and thins out below 2^-14, so a token with a key or value
+// scale beyond [kScaleLeast, kScaleMost] is multiplied as if its scales were 2^-e times
+// as large, and a query row likewise: logits get the power of two back in fp32, softmax
+// weights get a value's, relative to a power of two F that each output row keeps for
+// itself. Tokens and rows that have none keep their bits. Groups down to 2^-22 of a
+// token's largest so keep all that fp16 has of them (int4: down to 2^-25 all their bits),
+// those below 2^-33 become 0. A group whose codes are all zero is stored with the scale 1,
+// which does not count.
 __device__ __forceinline__ uint32_t h16mul2(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
@@ -144,13 +147,18 @@ constexpr uint32_t kQueryLeast = 0x3B80, kQueryMost = 0x4700;        // bf16 2^-
 __device__ __forceinline__ bool beyond(uint32_t bits, uint32_t least, uint32_t most) { return bits - least > most - least; }
 // 2^e, |e| <= 126
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
-// Exponents to take out of a token whose largest scale has these bits, and of a query row
-// whose largest magnitude has: to [256, 512) and [2^14, 2^15) above, to [1, 2) below.
-__device__ __forceinline__ int scale_exponent(uint32_t bits) {
-  if (bits == 0 || !beyond(bits, kScaleLeast, kScaleMost)) return 0;
-  const int e = static_cast<int>(bits >> 7) - 127;
-  return bits > kScaleMost ? min(e - 8, 119) : max(e, -110);
+// Exponent to take out of a token whose largest and least scales (of groups that are not
+// zero) have these bits: the largest ends below 512, the least at 2^-14 or above if the
+// largest leaves room for that; 0 where both do.
+__device__ __forceinline__ int scale_exponent(uint32_t most, uint32_t least) {
+  if (most <= kScaleMost && least >= kScaleLeast) return 0;
+  const int down = static_cast<int>(most >> 7) - 127 - 8, up = static_cast<int>(least >> 7) - 127 + 14;
+  return most > kScaleMost ? min(down, 119) : max(max(down, up), -110);
 }
+// What a token without any such group has: its weight counts nowhere but in the sum.
+constexpr int kNoScale = -110;
+// Exponent to take out of a query row whose largest magnitude has these bits: to
+// [2^14, 2^15) above, to [1, 2) below.
 __device__ __forceinline__ int query_exponent(uint32_t bits) {
   if (bits == 0 || !beyond(bits, kQueryLeast, kQueryMost)) return 0;
   const int e = static_cast<int>(bits >> 7) - 127;
@@ -197,6 +205,26 @@ __host__ __device__ constexpr int most_groups() {
     most = n > most ? n : most;
   }
   return most;
+}
+
+// Bit q: group base + q has a code other than zero's among the N channels from ch on, whose
+// codes are at `src` in shared memory. Groups are made of channel pairs. Rarely called, and
+// a function of its own: inlined it cost the loops around it 2 to 3 % in registers and
+// instruction cache.
+template <class L, int BITS, int N>
+__device__ __noinline__ uint32_t used_groups(uint32_t src, int ch, int base) {
+  constexpr int kPerWord = 32 / BITS;
+  uint32_t used = 0;
+#pragma unroll 1
+  for (int i = 0; i < N * BITS / 32; ++i, src += 4, ch += kPerWord) {
+    uint32_t x;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(src));
+    x ^= BITS == 4 ? 0x88888888u : 0x80808080u;
+#pragma unroll
+    for (int c = 0; c < kPerWord; c += 2)
+      if ((x >> (BITS * c)) & ((1u << (2 * BITS)) - 1)) used |= 1u << (group_at<L>(ch + c) - base);
+  }
+  return used;
 }
 
 }  // namespace paged

@@ -259,24 +259,32 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
             kw[r][4 * w + 3] = v.w;
           }
           const uint32_t from = k_scales + off + 8 * r * L::G * 2;
-          uint32_t x[GEO::kKG], top = 0;
+          uint32_t x[GEO::kKG], top = 0, low = 0xFFFFu;
           float f[GEO::kKG];
+          uint32_t used = ~0u;
+          if constexpr (EXACT) used = used_groups<L, KB, 32>(src, 32 * t, kbase);
 #pragma unroll
           for (int q = 0; q < GEO::kKG; ++q) {
             x[q] = ld_shared_u16(from + 2 * (GEO::kKG == 1 ? kbase : min(kbase + q, L::G - 1)));
+            if (EXACT && !((used >> q) & 1u)) continue;
             top = max(top, x[q]);
-            f[q] = __uint_as_float(x[q] << 16);
+            low = min(low, x[q]);
           }
+#pragma unroll
+          for (int q = 0; q < GEO::kKG; ++q) f[q] = (used >> q) & 1u ? __uint_as_float(x[q] << 16) : 0.0f;
           if constexpr (EXACT) {
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = scale_exponent(top);
+#pragma unroll
+            for (int d = 1; d < 4; d <<= 1) {
+              top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+              low = min(low, __shfl_xor_sync(0xffffffffu, low, d));
+            }
+            const int e = top == 0 ? 0 : scale_exponent(top, low);
             back[r] = pow2i(e);
 #pragma unroll
             for (int q = 0; q < GEO::kKG; ++q) f[q] *= pow2i(-e);
           } else {
             most = max(most, top);
-            least = min(least, top);
+            least = min(least, low);
           }
           ks01[r] = pack_f16x2(f[0], f[GEO::kKG > 1 ? 1 : 0]);
           ks23[r] = 0;
@@ -329,23 +337,31 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           const uint32_t from = ((u & 1) ? v_scales1 : v_scales0) + off + (u >> 1) * 8 * L::G * 2;
           // rows past the end hold anything: as zeros they add nothing
           const bool live = whole || (any_live && first_token + ((u & 1) ? vt1 : vt0) + (u >> 1) * 8 < it.kv_len);
-          uint32_t top = 0;
+          uint32_t used = live ? ~0u : 0u, top = 0, low = 0xFFFFu;
+          if constexpr (EXACT) {
+            const uint32_t src = ((u & 1) ? v_codes1 : v_codes0) + off + (u >> 1) * 8 * Rec<L, VB>::CW;
+            used &= used_groups<L, VB, 16>(src, 16 * g, vbase);
+          }
 #pragma unroll
           for (int q = 0; q < GEO::kVG; ++q) {
             uint32_t x = ld_shared_u16(from + 2 * (GEO::kVG == 1 ? vbase : min(vbase + q, L::G - 1)));
-            x = live ? x : 0;
+            x = (used >> q) & 1u ? x : 0;
             top = max(top, x);
+            if (!EXACT || ((used >> q) & 1u)) low = min(low, x);
             f[u][q] = __uint_as_float(x << 16);
           }
           if constexpr (EXACT) {
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-            ex[u] = scale_exponent(top);
+            for (int d = 4; d < 32; d <<= 1) {
+              top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+              low = min(low, __shfl_xor_sync(0xffffffffu, low, d));
+            }
+            ex[u] = !live ? 0 : top == 0 ? kNoScale : scale_exponent(top, low);
 #pragma unroll
             for (int q = 0; q < GEO::kVG; ++q) f[u][q] *= pow2i(-ex[u]);
           } else {
             most = max(most, top);
-            least = min(least, live ? top : kScaleLeast);
+            least = min(least, live ? low : kScaleLeast);
           }
         }
         if constexpr (EXACT) {

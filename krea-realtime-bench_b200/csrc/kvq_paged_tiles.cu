@@ -123,11 +123,12 @@ struct Converter {
   // This lane's codes and scales of one row: row rr of record block `rec`.
   struct Raw {
     uint32_t w[BITS], x[KG];  // 4 or 8 words of codes
+    uint32_t src;             // and where they are
   };
   __device__ __forceinline__ Raw load(uint32_t rec, int rr, int t) const {
     using R = Rec<L, BITS>;
     Raw u;
-    const uint32_t src = rec + rr * R::CW + t * (R::CW / 4);
+    const uint32_t src = u.src = rec + rr * R::CW + t * (R::CW / 4);
 #pragma unroll
     for (int i = 0; i < BITS / 4; ++i) {
       const uint4 v = ld_shared_v4(src + 16 * i);
@@ -149,24 +150,31 @@ struct Converter {
                                      uint32_t& most) const {
     const uint32_t (&w)[BITS] = u.w;
     const uint32_t (&x)[KG] = u.x;
-    uint32_t top = 0;
+    uint32_t top = 0, low = 0xFFFFu, used = live ? ~0u : 0u;  // rows past the end hold anything
+    if constexpr (EXACT) used &= used_groups<L, BITS, 32>(u.src, 32 * t, base);
 #pragma unroll
-    for (int q = 0; q < KG; ++q) top = max(top, x[q]);
+    for (int q = 0; q < KG; ++q) {
+      if (EXACT && !((used >> q) & 1u)) continue;
+      top = max(top, x[q]);
+      low = min(low, x[q]);
+    }
     float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int q = 0; q < KG; ++q) f[q] = live ? __uint_as_float(x[q] << 16) : 0.0f;  // rows past the end hold anything
+    for (int q = 0; q < KG; ++q) f[q] = (used >> q) & 1u ? __uint_as_float(x[q] << 16) : 0.0f;
     uint32_t s01, s23 = 0;
     int e = 0;
     if constexpr (EXACT) {
-      top = live ? top : 0;
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      e = scale_exponent(top);
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+        low = min(low, __shfl_xor_sync(0xffffffffu, low, d));
+      }
+      e = !live ? 0 : top == 0 ? kNoScale : scale_exponent(top, low);
 #pragma unroll
       for (int q = 0; q < KG; ++q) f[q] *= pow2i(-e);
     } else if (live) {
       most = max(most, top);
-      least = min(least, top);
+      least = min(least, low);
     }
     s01 = pack_f16x2(f[0], f[KG == 1 ? 0 : 1]);
     if constexpr (KG > 2) s23 = pack_f16x2(f[2], f[3]);
