@@ -176,11 +176,17 @@ __device__ __forceinline__ uint32_t most_of(const uint4& v) {
   }
   return m;
 }
+// A row's running maximum m stands kBias below the logit it was taken from and moves only
+// when some logit lies more than kLag + kBias above it, so the softmax weights 2^(x - m)
+// end at 2^15, and the largest of a row is 2^7 at least. fp16 holds weights of 2^-21 of that
+// with all their bits, and those of 2^-32 at all: without the bias 200 tokens under a first
+// token that leads by 17 nats and has the value 0 came out 7 % off.
+constexpr float kBias = 7.0f, kLag = 8.0f;
 // The F of an output row once a weight times its value's power of two has been 2^top, given
 // F so far; a row that has seen nothing yet (fresh) may take a lower one than 0. Leaves
 // room below fp16's end; 0 where that does, so that ordinary rows end up there.
 __device__ __forceinline__ float next_f(float f, float top, bool fresh) {
-  const float need = ceilf(top) - 14.0f;
+  const float need = ceilf(top) - (kBias + kLag);
   const float n = fresh ? need : fmaxf(f, need);
   return top == -INFINITY ? f : (n > -15.0f && n < 0.0f ? 0.0f : n);
 }

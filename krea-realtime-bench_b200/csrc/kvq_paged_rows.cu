@@ -12,9 +12,9 @@
 // copies (no tensor map) while the other stage is worked on; the warps never wait for
 // each other inside a piece. Per block (tokens j, rows n, channels c; mma.sync m16n8k16, fp32 out):
 //   S^T[j, n] = sum_c K[j, c] q[n, c]      A = K from registers, B = q held in registers
-//   p = 2^(S^T scale - m_n)                m_n lags the true maximum by at most 8: it moves
-//                                          (and O, l are rescaled) only when some logit
-//                                          exceeds it by more, one vote per block otherwise
+//   p = 2^(S^T scale - m_n)                m_n moves (and O, l are rescaled) only when some
+//                                          logit exceeds it by more than kLag + kBias, one
+//                                          vote per block otherwise
 //   O^T[c, n] += sum_j V[j, c] p[j, n]     A = V from registers, B = p (transposed, movmatrix)
 // Tokens are the M side, so 8 rows cost one N = 8 instruction. tcgen05 would need
 // the dequantized tile in shared memory (2 x 256 bytes per row through the shared-
@@ -428,15 +428,15 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
         const float mx1 = fmaxf(fmaxf(s[0][nt][1], s[0][nt][3]), fmaxf(s[1][nt][1], s[1][nt][3])) * sc[nt][1];
         fresh[nt][0] = m[nt][0] < -1.0e29f;
         fresh[nt][1] = m[nt][1] < -1.0e29f;
-        if (__any_sync(0xffffffffu, mx0 > m[nt][0] + 8.0f || mx1 > m[nt][1] + 8.0f)) {
+        if (__any_sync(0xffffffffu, mx0 - m[nt][0] > kBias + kLag || mx1 - m[nt][1] > kBias + kLag)) {
           float n0 = mx0, n1 = mx1;
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) {
             n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
             n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
           }
-          n0 = fmaxf(n0, m[nt][0]);
-          n1 = fmaxf(n1, m[nt][1]);
+          n0 = fmaxf(n0 - kBias, m[nt][0]);
+          n1 = fmaxf(n1 - kBias, m[nt][1]);
           const float a0 = ex2f(m[nt][0] - n0), a1 = ex2f(m[nt][1] - n1);
           m[nt][0] = n0;
           m[nt][1] = n1;

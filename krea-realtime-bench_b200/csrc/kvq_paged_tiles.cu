@@ -434,11 +434,11 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       const bool fresh = m < -1.0e29f;
       float alpha = 1.0f;
       if (i_ == 0) {
-        m = fmaxf(m, mt);
-      } else if (mt > m + 8.0f) {
+        m = fmaxf(m, mt - kBias);
+      } else if (mt - m > kBias + kLag) {
         rescale = true;
-        alpha = ex2f(m - mt);
-        m = mt;
+        alpha = ex2f(m - (mt - kBias));
+        m = mt - kBias;
         l *= alpha;
       }
       const float nm = -m;

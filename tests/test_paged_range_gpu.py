@@ -61,3 +61,36 @@ def test_groups_of_zeros_beside_small_ones(q, k_bits, v_bits, mode, size):
     kk[17] = vv[18] = 0
     k, v = append(cache, table, kk, vv)
     check(torch.randn(q, 4, 128).bfloat16().cuda(), cache, batch, k, v, scale=0.09 / size)
+
+
+@pytest.mark.parametrize("q", [1, 70])
+@pytest.mark.parametrize("k_bits,v_bits", [(4, 4), (8, 8)])
+@pytest.mark.parametrize("n,lead", [(200, 5.0), (200, 13.0), (200, 16.5), (200, 17.2), (131072, 16.5), (131072, 17.2)])
+def test_weights_under_one_dominating_token(q, k_bits, v_bits, n, lead):
+    """The first token leads by `lead` nats and has the value zero: the output is the sum of the
+    others' small weights. 200 tokens in one part, 131072 in many.
+
+    Bound per element: the output's rounding (2^-8), and of each weight either fp16's relative
+    rounding (2^-11) or, below its normal range, 2^-32 of the row's largest (fp16 ends at 2^-24,
+    and the largest is stored as 2^7 at least), a value's rounding (2^-11) and a logit's by
+    those of the keys (twice d)."""
+    cache, batch, table = make([n], [q], heads=1, page=128, k_bits=k_bits, v_bits=v_bits, mode="blind64", garbage=False)
+    kk = torch.randn(n, 1, 128) * 0.03
+    vv = 1 + 0.3 * torch.randn(n, 1, 128)
+    kk[:, 0, 0] = 0
+    kk[0] = vv[0] = 0
+    kk[0, 0, 0] = lead
+    x = torch.randn(q, 1, 128)
+    x[:, :, 0] = 1
+    x = x.bfloat16()
+    k, v = append(cache, table, kk.bfloat16(), vv.bfloat16())
+    out, lse = paged.attention(x.cuda(), cache, batch, causal=False, softmax_scale=1.0, return_lse=True)
+    k, v, xd = k[:, 0], v[:, 0], x[:, 0].double()
+    logits = xd @ k.T
+    w = torch.softmax(logits, 1)
+    ref = w @ v
+    d = (2.0 ** -11 * (xd.abs() @ k.abs().T)).amax(1, keepdim=True)
+    most = w.amax(1, keepdim=True)
+    bound = 2.0 ** -8 * ref.abs() + (2 * 2.0 ** -11 + 2 * d + 2e-5) * (w @ v.abs()) + 2.0 ** -32 * most * v.abs().sum(0)
+    assert ((out[:, 0].double().cpu() - ref).abs() <= bound).all()
+    assert ((lse[:, 0].double().cpu() - torch.logsumexp(logits, 1)).abs() <= d[:, 0] + 2e-5).all()
