@@ -382,7 +382,35 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
       value_scales(at, ta, true, vs[0], ve[0], std::false_type{});
       value_scales(at + GEO::kStage / 2, tz, two, vs[1], ve[1], std::false_type{});
       bool wide_v = false;
-      if (__any_sync(0xffffffffu, most > kScaleMost || least < kScaleLeast)) {
+      // Rows past the end hold anything, zeros where nothing was written yet, and those of K
+      // have counted above (a test per row there cost 3 % of a decode batch): where there are
+      // some, the live rows' scales are looked at again.
+      auto live_beyond = [&]() {
+        bool far = false;
+#pragma unroll 1
+        for (int bb = 0; bb < (two ? 2 : 1); ++bb) {
+          const uint32_t off = at + bb * (GEO::kStage / 2);
+          const int n_live = it.kv_len - (bb ? tz : ta);
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int q = 0; q < GEO::kKG; ++q) {
+              const uint32_t x = ld_shared_u16(k_scales + off + 8 * r * L::G * 2 + 2 * min(kbase + q, L::G - 1));
+              far |= token_of(g) + 8 * r < n_live && beyond(x, kScaleLeast, kScaleMost);
+            }
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int q = 0; q < GEO::kVG; ++q) {
+              const uint32_t x = ld_shared_u16(((u & 1) ? v_scales1 : v_scales0) + off + (u >> 1) * 8 * L::G * 2 +
+                                               2 * min(vbase + q, L::G - 1));
+              far |= ((u & 1) ? vt1 : vt0) + (u >> 1) * 8 < n_live && beyond(x, kScaleLeast, kScaleMost);
+            }
+        }
+        return far;
+      };
+      if (__any_sync(0xffffffffu, most > kScaleMost || least < kScaleLeast) &&
+          (whole || __any_sync(0xffffffffu, live_beyond()))) {
         // rare: once more, with the powers of two
 #pragma unroll 1
         for (int bb = 0; bb < 2; ++bb) {
