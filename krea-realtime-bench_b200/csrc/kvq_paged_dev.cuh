@@ -155,6 +155,19 @@ __device__ __forceinline__ int scale_exponent(uint32_t most, uint32_t least) {
   const int down = static_cast<int>(most >> 7) - 127 - 8, up = static_cast<int>(least >> 7) - 127 + 14;
   return most > kScaleMost ? min(down, 119) : max(max(down, up), -110);
 }
+// The largest and least of the scales that lanes differing in the bits FIRST, 2 FIRST, ... ,
+// LAST of their number have, in one exchange.
+template <int FIRST, int LAST>
+__device__ __forceinline__ void extremes_of_lanes(uint32_t& most, uint32_t& least) {
+  uint32_t x = most << 16 | (0xFFFFu - least);
+#pragma unroll
+  for (int d = FIRST; d <= LAST; d <<= 1) x = __vmaxu2(x, __shfl_xor_sync(0xffffffffu, x, d));
+  most = x >> 16;
+  least = 0xFFFFu - (x & 0xFFFFu);
+}
+// Bits of the scale that a group of zeros is stored with: no other group needs a look at its
+// codes to tell.
+constexpr uint32_t kScaleOne = 0x3F80;
 // What a token without any such group has: its weight counts nowhere but in the sum.
 constexpr int kNoScale = -110;
 // Exponent to take out of a query row whose largest magnitude has these bits: to
@@ -214,9 +227,9 @@ __host__ __device__ constexpr int most_groups() {
 }
 
 // Bit q: group base + q has a code other than zero's among the N channels from ch on, whose
-// codes are at `src` in shared memory. Groups are made of channel pairs. Rarely called, and
-// a function of its own: inlined it cost the loops around it 2 to 3 % in registers and
-// instruction cache.
+// codes are at `src` in shared memory; bits of groups whose scale is not 1 are of no use.
+// Groups are made of channel pairs. Rarely called, and a function of its own: inlined it cost
+// the loops around it 2 to 3 % in registers and instruction cache.
 template <class L, int BITS, int N>
 __device__ __noinline__ uint32_t used_groups(uint32_t src, int ch, int base) {
   constexpr int kPerWord = 32 / BITS;

@@ -262,10 +262,15 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           uint32_t x[GEO::kKG], top = 0, low = 0xFFFFu;
           float f[GEO::kKG];
           uint32_t used = ~0u;
-          if constexpr (EXACT) used = used_groups<L, KB, 32>(src, 32 * t, kbase);
+          bool one = false;
 #pragma unroll
           for (int q = 0; q < GEO::kKG; ++q) {
             x[q] = ld_shared_u16(from + 2 * (GEO::kKG == 1 ? kbase : min(kbase + q, L::G - 1)));
+            one |= x[q] == kScaleOne;
+          }
+          if (EXACT && __any_sync(0xffffffffu, one)) used = used_groups<L, KB, 32>(src, 32 * t, kbase);
+#pragma unroll
+          for (int q = 0; q < GEO::kKG; ++q) {
             if (EXACT && !((used >> q) & 1u)) continue;
             top = max(top, x[q]);
             low = min(low, x[q]);
@@ -273,11 +278,7 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
 #pragma unroll
           for (int q = 0; q < GEO::kKG; ++q) f[q] = (used >> q) & 1u ? __uint_as_float(x[q] << 16) : 0.0f;
           if constexpr (EXACT) {
-#pragma unroll
-            for (int d = 1; d < 4; d <<= 1) {
-              top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-              low = min(low, __shfl_xor_sync(0xffffffffu, low, d));
-            }
+            extremes_of_lanes<1, 2>(top, low);
             const int e = top == 0 ? 0 : scale_exponent(top, low);
             back[r] = pow2i(e);
 #pragma unroll
@@ -337,25 +338,24 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           const uint32_t from = ((u & 1) ? v_scales1 : v_scales0) + off + (u >> 1) * 8 * L::G * 2;
           // rows past the end hold anything: as zeros they add nothing
           const bool live = whole || (any_live && first_token + ((u & 1) ? vt1 : vt0) + (u >> 1) * 8 < it.kv_len);
-          uint32_t used = live ? ~0u : 0u, top = 0, low = 0xFFFFu;
-          if constexpr (EXACT) {
-            const uint32_t src = ((u & 1) ? v_codes1 : v_codes0) + off + (u >> 1) * 8 * Rec<L, VB>::CW;
-            used &= used_groups<L, VB, 16>(src, 16 * g, vbase);
-          }
+          uint32_t used = live ? ~0u : 0u, top = 0, low = 0xFFFFu, xs[GEO::kVG];
+          bool one = false;
 #pragma unroll
           for (int q = 0; q < GEO::kVG; ++q) {
-            uint32_t x = ld_shared_u16(from + 2 * (GEO::kVG == 1 ? vbase : min(vbase + q, L::G - 1)));
-            x = (used >> q) & 1u ? x : 0;
+            xs[q] = ld_shared_u16(from + 2 * (GEO::kVG == 1 ? vbase : min(vbase + q, L::G - 1)));
+            one |= xs[q] == kScaleOne;
+          }
+          if (EXACT && __any_sync(0xffffffffu, one))
+            used &= used_groups<L, VB, 16>(((u & 1) ? v_codes1 : v_codes0) + off + (u >> 1) * 8 * Rec<L, VB>::CW, 16 * g, vbase);
+#pragma unroll
+          for (int q = 0; q < GEO::kVG; ++q) {
+            const uint32_t x = (used >> q) & 1u ? xs[q] : 0;
             top = max(top, x);
             if (!EXACT || ((used >> q) & 1u)) low = min(low, x);
             f[u][q] = __uint_as_float(x << 16);
           }
           if constexpr (EXACT) {
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) {
-              top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-              low = min(low, __shfl_xor_sync(0xffffffffu, low, d));
-            }
+            extremes_of_lanes<4, 16>(top, low);
             ex[u] = !live ? 0 : top == 0 ? kNoScale : scale_exponent(top, low);
 #pragma unroll
             for (int q = 0; q < GEO::kVG; ++q) f[u][q] *= pow2i(-ex[u]);

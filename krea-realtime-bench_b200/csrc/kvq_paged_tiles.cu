@@ -151,7 +151,12 @@ struct Converter {
     const uint32_t (&w)[BITS] = u.w;
     const uint32_t (&x)[KG] = u.x;
     uint32_t top = 0, low = 0xFFFFu, used = live ? ~0u : 0u;  // rows past the end hold anything
-    if constexpr (EXACT) used &= used_groups<L, BITS, 32>(u.src, 32 * t, base);
+    if constexpr (EXACT) {
+      bool one = false;
+#pragma unroll
+      for (int q = 0; q < KG; ++q) one |= x[q] == kScaleOne;
+      if (__any_sync(0xffffffffu, one)) used &= used_groups<L, BITS, 32>(u.src, 32 * t, base);
+    }
 #pragma unroll
     for (int q = 0; q < KG; ++q) {
       if (EXACT && !((used >> q) & 1u)) continue;
@@ -164,11 +169,7 @@ struct Converter {
     uint32_t s01, s23 = 0;
     int e = 0;
     if constexpr (EXACT) {
-#pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-        low = min(low, __shfl_xor_sync(0xffffffffu, low, d));
-      }
+      extremes_of_lanes<1, 2>(top, low);
       e = !live ? 0 : top == 0 ? kNoScale : scale_exponent(top, low);
 #pragma unroll
       for (int q = 0; q < KG; ++q) f[q] *= pow2i(-e);
