@@ -177,6 +177,10 @@ __device__ __forceinline__ int query_exponent(uint32_t bits) {
   const int e = static_cast<int>(bits >> 7) - 127;
   return bits > kQueryMost ? e - 14 : max(e, -110);
 }
+// What a row's logits are multiplied with: the softmax scale with the power of two taken out
+// of the row's query. Never 0, which would make a masked logit NaN; logits of so small a
+// scale are 0 either way.
+__device__ __forceinline__ float row_scale_of(float scale_log2, int e) { return fmaxf(scale_log2 * pow2i(e), 0x1p-126f); }
 // Largest finite magnitude among eight bf16, as bits.
 __device__ __forceinline__ uint32_t most_of(const uint4& v) {
   uint32_t m = 0;

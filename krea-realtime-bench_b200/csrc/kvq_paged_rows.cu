@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
       most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
       const int e = query_exponent(most);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) sc[nt][i] = a.scale_log2 * pow2i(__shfl_sync(0xffffffffu, e, 4 * (2 * t + i)));
+      for (int i = 0; i < 2; ++i) sc[nt][i] = row_scale_of(a.scale_log2, __shfl_sync(0xffffffffu, e, 4 * (2 * t + i)));
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const uint4 v = 8 * nt + g < it.n_rows ? to_f16(qv[nt][w], e) : make_uint4(0, 0, 0, 0);

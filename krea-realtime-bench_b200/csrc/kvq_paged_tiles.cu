@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       uint32_t most = 0;
 #pragma unroll 4
       for (int c = 0; c < 16; ++c) most = max(most, most_of(ld_global_nc_v4(src + c)));
-      row_scale *= pow2i(query_exponent(most));
+      row_scale = row_scale_of(a.scale_log2, query_exponent(most));
     }
     // wide_k, wide_v: a byte per converter warp of the tile, and whose rows' exponents count
     auto exps16 = [&](uint32_t wide, uint32_t at, int block) {

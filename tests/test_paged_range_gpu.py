@@ -134,3 +134,16 @@ def test_slots_that_were_never_written_cost_nothing():
 
     ratios = [t[0] / t[1] for t in (fastest() for _ in range(5))]
     assert min(ratios) < 1.07, ratios
+
+
+@pytest.mark.parametrize("q", [1, 12, 150])
+@pytest.mark.parametrize("scale,size", [(1e-20, 1e-30), (1e-38, 1e-25), (1e-38, 1.0), (1e-30, 1e-6)])
+def test_tiny_scale_and_queries(q, scale, size):
+    """Logits of no size: the mean of the values that a row sees, where the product of the
+    softmax scale and the power of two taken out of a query is below fp32's range too."""
+    n = 217
+    cache, batch, table = make([n], [q], heads=2, page=32)
+    k, v = append(cache, table, rows_of(n, 2, 3), rows_of(n, 2, 4))
+    x = (torch.randn(q, 4, 128) * size).bfloat16()
+    check(x.cuda(), cache, batch, k, v, scale=scale)
+    check(x.cuda(), cache, batch, k, v, scale=scale, window=50, sink=7)
