@@ -33,15 +33,21 @@ HEAD_DIM = 128
 # calls return, without making a Stream object at every launch
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
-def _launch(index: int, raw: int, fn, what: str, *args) -> None:
-    """One C call on device `index` and its stream `raw`."""
-    if _current_device() == index:
+def _launch(cache: "PagedKVCache", batch: "PagedBatch", raw: int, fn, what: str, *args) -> None:
+    """One C call on the cache's device and its stream `raw`. A captured one holds addresses
+    of the batch's uploads, so the cache, whose pages it holds too, keeps the batch."""
+    if _current_device() == cache.device.index:
         rc = fn(*args, raw)
+        captured = _capturing()
     else:
-        with torch.cuda.device(index):
+        with torch.cuda.device(cache.device):
             rc = fn(*args, raw)
+            captured = _capturing()
+    if captured:
+        cache._captured.add(batch)
     if rc:
         _lib.check(rc, what)
 
@@ -73,7 +79,11 @@ class PagedBatch:
     (new ones included) and how many of those are new. Shared by all layers and by
     append, read and attention. block_table [B, most pages], kv_lens [B] and q_lens
     [B] are host data; row b's first ceil(kv_lens[b] / page_size) entries are used.
-    Tensors with one row per new token are ordered sequence after sequence."""
+    Tensors with one row per new token are ordered sequence after sequence.
+
+    A CUDA graph into which a call was captured keeps this batch's lengths, table and work
+    list, whose memory belongs to the batch: the cache holds the batch until its
+    release_captured(), so only the cache has to be kept as long as the graph."""
 
     def __init__(self, block_table, kv_lens, q_lens, page_size: int, device="cuda"):
         dev = _cuda_device(device)
@@ -253,6 +263,7 @@ class PagedKVCache:
                                       self._map.ctypes.data)
         self._ref = ctypes.byref(self._c)
         self._format = (self.n_heads, self.k_bits, self.v_bits, group_mode)
+        self._captured = set()
 
     def _row_bytes(self, bits: int) -> int:
         return self._code_bytes(bits) + 2 * len(self.bands)
@@ -278,6 +289,12 @@ class PagedKVCache:
     def storage_bytes(self) -> int:
         return self._k_pages.numel() + self._v_pages.numel()
 
+    def release_captured(self) -> None:
+        """Drops the batches that were kept for CUDA graphs: a graph into which a call was
+        captured reads the batch's table, lengths and plan at every replay. Call it when no
+        such graph will be replayed again; the cache itself has to outlive them."""
+        self._captured.clear()
+
     def _check(self, batch: PagedBatch) -> None:
         if not isinstance(batch, PagedBatch):
             raise TypeError(f"expected a PagedBatch, got {type(batch).__name__}")
@@ -298,7 +315,7 @@ class PagedKVCache:
         shape = (batch.n_new, self.n_heads, self.head_dim)
         k, ks = _rows(k, shape, self.device, "k")
         v, vs = _rows(v, shape, self.device, "v")
-        _launch(self.device.index, batch._use(), _lib.load().kvq_paged_append, "kvq_paged_append", k.data_ptr(), ks,
+        _launch(self, batch, batch._use(), _lib.load().kvq_paged_append, "kvq_paged_append", k.data_ptr(), ks,
                 v.data_ptr(), vs, self._ref, batch._ref)
 
     def read(self, batch: PagedBatch, new_only: bool = False):
@@ -311,7 +328,7 @@ class PagedKVCache:
         shape, row = (n, self.n_heads, self.head_dim), self.n_heads * self.head_dim
         k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
         v = torch.empty_like(k)
-        _launch(self.device.index, batch._use(), _lib.load().kvq_paged_read, "kvq_paged_read", self._ref, batch._ref,
+        _launch(self, batch, batch._use(), _lib.load().kvq_paged_read, "kvq_paged_read", self._ref, batch._ref,
                 1 if new_only else 0, k.data_ptr(), row, v.data_ptr(), row)
         return k, v
 
@@ -380,7 +397,7 @@ def attention(q: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, causal: b
     lse = torch.empty(shape[:2], dtype=torch.float32, device=device) if return_lse else None
     plan = batch._plan(cache, heads, bool(causal), window, sink)
     raw = batch._use()
-    _launch(device.index, raw, _lib.load().kvq_paged_attention, "kvq_paged_attention", q.data_ptr(), qs, cache._ref,
+    _launch(cache, batch, raw, _lib.load().kvq_paged_attention, "kvq_paged_attention", q.data_ptr(), qs, cache._ref,
             batch._ref, out.data_ptr(), os_, lse.data_ptr() if return_lse else None, heads, 1 if causal else 0, window, sink,
             scale, *plan.args(raw))
     return (out, lse) if return_lse else out
