@@ -75,8 +75,9 @@ struct alignas(16) Item {
 static_assert(sizeof(Item) == 64, "the plan's layout");
 constexpr int kItemWords = 16;
 
-// Workspace of one part: O [rows][128] unnormalised, then m, l per row (fp32).
-__host__ __device__ constexpr int slot_floats(int rows) { return rows * (D + 2); }
+// Workspace of one part: O [rows][128] unnormalised, then m, l, F and an unused one per row
+// (fp32): the running maximum, the sum, and the power of two that O is kept divided by.
+__host__ __device__ constexpr int slot_floats(int rows) { return rows * (D + 4); }
 // Most parts of a unit: joining them is serial work of one block.
 constexpr int kMaxParts = 128;
 
@@ -116,7 +117,7 @@ __device__ __forceinline__ Seen seen_by(const AttnArgs& a, int pos, int kv_len) 
 }
 
 // Workspace of one part in the kernel for many rows: two Q tiles of float4 [33][128 rows],
-// 32 columns of O and one of (m, l).
+// 32 columns of O and one of (m, l, F).
 constexpr int kTileRows = 256;
 constexpr int64_t kTileSlotBytes = 2 * 33 * 128 * 16;
 

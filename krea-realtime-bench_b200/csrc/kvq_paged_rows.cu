@@ -26,7 +26,7 @@
 // of tokens inside a fragment is free as long as A and B agree: lane (g, t) = (lane /
 // 4, lane % 4) holds channels 32t..32t+31 of K rows and channels 16g..16g+15 of V
 // rows, 8 or 16 contiguous bytes of shared memory.
-// The warps' (m, l, O) are joined in shared memory, parts of a unit in the workspace.
+// The warps' (m, l, F, O) are joined in shared memory, parts of a unit in the workspace.
 #include <cmath>
 
 #include "kvq_paged_dev.cuh"
@@ -48,7 +48,7 @@ struct RowGeo {
   static constexpr int kStages = 2;
   static constexpr int kRing = kStages * kStage;  // one warp's
   static constexpr int kOffML = kWarps * kRing;
-  static constexpr int kOffBar = kOffML + kWarps * 8 * NT * 8;
+  static constexpr int kOffBar = kOffML + kWarps * 8 * NT * 16;
   static constexpr int kOffMisc = kOffBar + kWarps * kStages * 8;
   static constexpr int kSmemBytes = kOffMisc + 16;
   // resident blocks: shared memory, and registers (168 a thread for three, 255 for two; with
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
   volatile int* abort = reinterpret_cast<volatile int*>(smem + GEO::kOffMisc);
   volatile int* last = abort + 1;
   uint8_t* ring = smem + warp * GEO::kRing;
-  float* sm_ml = reinterpret_cast<float*>(smem + GEO::kOffML);  // [warp][row][2]
+  float4* sm_ml = reinterpret_cast<float4*>(smem + GEO::kOffML);  // [warp][row] (m, l, F)
   if (lane == 0) {
     for (int i = 0; i < GEO::kStages; ++i) mbar_init(&bars[i], 1);
     fence_mbar_init();
@@ -576,7 +576,9 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
     }
     step = step0 + n_mine;
 
-    // ---- join the warps: each leaves (m, l, O) in its own ring, whose copies are all consumed
+    // ---- join the warps: each leaves (m, l, F, O) in its own ring, whose copies are all
+    // consumed. Sums and O each have their own greatest term, m and m + F: O times 2^F may
+    // be beyond fp32 until it is divided by the sum.
     float* mine = reinterpret_cast<float*>(ring);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -586,28 +588,23 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
         const int n = 8 * nt + 2 * t + e;
-        if (g == 0) {
-          sm_ml[(warp * kRows + n) * 2] = m[nt][e];
-          sm_ml[(warp * kRows + n) * 2 + 1] = x;
-        }
-        const float of = ex2f(F[nt][e]);
+        if (g == 0) sm_ml[warp * kRows + n] = make_float4(m[nt][e], x, F[nt][e], 0.0f);
         float4* dst = reinterpret_cast<float4*>(mine + n * D + 16 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          dst[i] = make_float4(o[nt][2 * i][e] * of, o[nt][2 * i][2 + e] * of, o[nt][2 * i + 1][e] * of,
-                               o[nt][2 * i + 1][2 + e] * of);
+          dst[i] = make_float4(o[nt][2 * i][e], o[nt][2 * i][2 + e], o[nt][2 * i + 1][e], o[nt][2 * i + 1][2 + e]);
       }
     }
     __syncthreads();
     float* slot = it.parts > 1 ? a.ws + static_cast<int64_t>(it.slot + it.part) * slot_floats(kRows) : nullptr;
     // Rows are dealt to the warps, lane i has channels 4i..4i+3.
-    auto finish = [&](int n, float4 acc, float mm, float total) {
+    auto finish = [&](int n, float4 acc, float mm, float total, float f) {
       const int row = it.row0 + n, i = row / a.group;
       const int64_t tok = it.q_first + i;
       const int h = it.head * a.group + row - i * a.group;
-      const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+      const float inv = total == 0.0f ? 0.0f : 1.0f / total, of = ex2f(f);
       *reinterpret_cast<uint2*>(a.out + tok * a.out_stride + h * D + 4 * lane) =
-          make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+          make_uint2(pack_bf16x2(acc.x * inv * of, acc.y * inv * of), pack_bf16x2(acc.z * inv * of, acc.w * inv * of));
       if (a.lse && lane == 0)
         a.lse[tok * a.n_q_heads + h] = total == 0.0f ? -INFINITY : 0.69314718055994531f * (mm + log2f(total));
     };
@@ -615,24 +612,30 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
       acc = make_float4(fmaf(f, v.x, acc.x), fmaf(f, v.y, acc.y), fmaf(f, v.z, acc.z), fmaf(f, v.w, acc.w));
     };
     for (int n = warp; n < it.n_rows; n += kWarps) {
-      float mw[kWarps], mm = -1.0e30f, total = 0.0f;
+      float mm = -1.0e30f, total = 0.0f;
+      float4 ml[kWarps];
+      bool wide = false;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        mw[w] = sm_ml[(w * kRows + n) * 2];
-        mm = fmaxf(mm, mw[w]);
+        ml[w] = sm_ml[w * kRows + n];
+        mm = fmaxf(mm, ml[w].x);
+        wide = wide || ml[w].z != 0.0f;
       }
+      float mf = -1.0e30f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mf = fmaxf(mf, ml[w].x + ml[w].z);
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2f(mw[w] - mm);
-        total += f * sm_ml[(w * kRows + n) * 2 + 1];
-        add(acc, f, reinterpret_cast<const float4*>(smem + w * GEO::kRing + n * D * 4)[lane]);
+        const float f = ex2f(ml[w].x - mm);
+        total += f * ml[w].y;
+        add(acc, ex2f(ml[w].x + ml[w].z - mf), reinterpret_cast<const float4*>(smem + w * GEO::kRing + n * D * 4)[lane]);
       }
       if (slot) {
         reinterpret_cast<float4*>(slot + n * D)[lane] = acc;
-        if (lane == 0) reinterpret_cast<float2*>(slot + kRows * D)[n] = make_float2(mm, total);
+        if (lane == 0) reinterpret_cast<float4*>(slot + kRows * D)[n] = make_float4(mm, total, mf - mm, 0.0f);
       } else {
-        finish(n, acc, mm, total);
+        finish(n, acc, mm, total, mf - mm);
       }
     }
     if (slot) {
@@ -651,34 +654,39 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
         constexpr int kAtOnce = 16;
         const float* base = a.ws + static_cast<int64_t>(it.slot) * slot_floats(kRows);
         for (int n = warp; n < it.n_rows; n += kWarps) {
-          float mm = -1.0e30f, total = 0.0f;
+          float mm = -1.0e30f, mf = -1.0e30f, total = 0.0f;
           float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           for (int p0 = 0; p0 < it.parts; p0 += kAtOnce) {
             const float* sp = base + static_cast<int64_t>(p0) * slot_floats(kRows);
             const int np = it.parts - p0;
-            float2 ml = make_float2(-1.0e30f, 0.0f);
+            float4 ml = make_float4(-1.0e30f, 0.0f, 0.0f, 0.0f);
             if (lane < min(np, kAtOnce))
-              ml = __ldcg(reinterpret_cast<const float2*>(sp + lane * slot_floats(kRows) + kRows * D) + n);
+              ml = __ldcg(reinterpret_cast<const float4*>(sp + lane * slot_floats(kRows) + kRows * D) + n);
             float4 v[kAtOnce];
 #pragma unroll
             for (int q = 0; q < kAtOnce; ++q)
               v[q] = q < np ? __ldcg(reinterpret_cast<const float4*>(sp + q * slot_floats(kRows) + n * D) + lane)
                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float top = fmaxf(ml.x, mm);
+            float top = fmaxf(ml.x, mm), top_f = fmaxf(ml.x + ml.z, mf);
 #pragma unroll
-            for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            for (int x = 8; x > 0; x >>= 1) {
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              top_f = fmaxf(top_f, __shfl_xor_sync(0xffffffffu, top_f, x));
+            }
             top = __shfl_sync(0xffffffffu, top, 0);  // lanes 0-15 hold the parts
-            const float f0 = ex2f(mm - top), f = ex2f(ml.x - top);
-            float sum = f * ml.y;
+            top_f = __shfl_sync(0xffffffffu, top_f, 0);
+            const float f0 = ex2f(mf - top_f), f = ex2f(ml.x + ml.z - top_f);
+            float sum = ex2f(ml.x - top) * ml.y;
 #pragma unroll
             for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            total = total * f0 + __shfl_sync(0xffffffffu, sum, 0);
+            total = total * ex2f(mm - top) + __shfl_sync(0xffffffffu, sum, 0);
             acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
 #pragma unroll
             for (int q = 0; q < kAtOnce; ++q) add(acc, __shfl_sync(0xffffffffu, f, q), v[q]);
             mm = top;
+            mf = top_f;
           }
-          finish(n, acc, mm, total);
+          finish(n, acc, mm, total, mf - mm);
         }
       }
     }

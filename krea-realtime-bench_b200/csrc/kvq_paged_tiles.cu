@@ -269,10 +269,10 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         st_global_v4(a.out + to + 8 * c, ld_shared_v4(stage + (c >> 3) * kQAtom + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)));
     }
   };
-  auto stage_chunk = [&](uint32_t stage, int r, int ch, const float* v, float inv) {
+  auto stage_chunk = [&](uint32_t stage, int r, int ch, const float* v, float f) {
     st_shared_v4(stage + (ch >> 3) * kQAtom + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
-                 pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv),
-                 pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
+                 pack_bf16x2(v[0] * f, v[1] * f), pack_bf16x2(v[2] * f, v[3] * f), pack_bf16x2(v[4] * f, v[5] * f),
+                 pack_bf16x2(v[6] * f, v[7] * f));
   };
   auto store_lse = [&](int n, float m, float l) {
     if (a.lse && n < it.n_rows) {
@@ -556,12 +556,13 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                : step(i, j, wide_k, wide_v, std::true_type{});
       if (!ok) break;
     }
-    float of = ex2f(F);  // what the row of O is multiplied by, and the other set's
-    float of1 = 0.0f;
+    // what the rows of O, of this set and of the other, are multiplied with when they are joined
+    float of = 1.0f, of1 = 0.0f;
     bool done = ok && n_mine > 0 && poll_wait_warp(&bars[GEO::bOFinal + x], 0, abort, a.status, lim);
     // Shared tiles: set 1 leaves its row in the stages of K and V, float4 column c of row r
-    // at [c][r] and (m, l) behind them, and set 0 adds it to its own. No MMA reads the
-    // stages any more.
+    // at [c][r] and (m, l, F) behind them, and set 0 adds it to its own. No MMA reads the
+    // stages any more. Sums and O each have their own greatest term, m and m + F: O times
+    // 2^F may be beyond fp32 until it is divided by the sum.
     const uint32_t other = sbase + GEO::kOffK + r * 16;
     if (shared && nkv > 0) {
       if (x == 1) {
@@ -575,22 +576,23 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
             for (int c = 0; c < 8; ++c)
               st_shared_v4(other + (8 * k + c) * BM * 16, o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
           }
-          st_shared_v4(other + 32 * BM * 16, __float_as_uint(m), __float_as_uint(l), __float_as_uint(of), 0);
+          st_shared_v4(other + 32 * BM * 16, __float_as_uint(m), __float_as_uint(l), __float_as_uint(F), 0);
         }
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (x == 0) {
         const uint4 u = ld_shared_v4(other + 32 * BM * 16);
-        const float m1 = __uint_as_float(u.x), l1 = __uint_as_float(u.y), mx = fmaxf(m, m1);
-        const float f = ex2f(m - mx), f1 = ex2f(m1 - mx);
+        const float m1 = __uint_as_float(u.x), l1 = __uint_as_float(u.y), mf1 = m1 + __uint_as_float(u.z);
+        const float mx = fmaxf(m, m1), mf = fmaxf(m + F, mf1);
+        l = l * ex2f(m - mx) + l1 * ex2f(m1 - mx);
+        of = ex2f(m + F - mf);
+        of1 = ex2f(mf1 - mf);
         m = mx;
-        l = l * f + l1 * f1;
-        of *= f;
-        of1 = __uint_as_float(u.z) * f1;
+        F = mf - mx;
       }
     }
     const bool both = shared && nkv > 1;  // set 1 had tiles
-    // 32 columns of the row of O, unnormalised
+    // 32 columns of the joined row of O, divided by 2^F
     auto fetch = [&](int k, float (&v)[32]) {
       if (done) {
         uint32_t o[32];
@@ -625,12 +627,14 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
 #pragma unroll
           for (int c = 0; c < 8; ++c) dst[(8 * k + c) * BM] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
         }
-        dst[32 * BM] = make_float4(m, l, 0.0f, 0.0f);
+        dst[32 * BM] = make_float4(m, l, F, 0.0f);
         __threadfence();
       } else if (done || (nkv == 0 && poll_wait_warp(&bars[GEO::bQReady + x], 0, abort, a.status, lim))) {
         // (no tiles: Q_x has landed before its buffer is reused below)
         tc_fence_after();
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l, pow_f = ex2f(F);
+        of *= inv;
+        of1 *= inv;
         store_lse(n, m, l);
         const uint32_t stage = sbase + q_at(x);  // Q_x is no longer read
 #pragma unroll 1
@@ -638,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
           float v[32];
           fetch(k, v);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) stage_chunk(stage, r, 4 * k + c, v + 8 * c, inv);
+          for (int c = 0; c < 4; ++c) stage_chunk(stage, r, 4 * k + c, v + 8 * c, pow_f);
         }
         __syncwarp();
         store_rows(warp * 32, 32);
@@ -841,15 +845,19 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       const int n_col = 16 * nq / 2, c0 = (tid / (nq * BM)) * n_col;  // float4 columns of this thread
       const int64_t pstride = static_cast<int64_t>(2) * 33 * BM;
       const float4* src = reinterpret_cast<const float4*>(a.ws) + (static_cast<int64_t>(it.slot) * 2 + x) * 33 * BM + r;
-      float mx = -1.0e30f, lsum = 0.0f;
+      float mx = -1.0e30f, mf = -1.0e30f, lsum = 0.0f;
 #pragma unroll 4
-      for (int p = 0; p < it.parts; ++p) mx = fmaxf(mx, __ldcg(src + p * pstride + 32 * BM).x);
+      for (int p = 0; p < it.parts; ++p) {
+        const float4 ml = __ldcg(src + p * pstride + 32 * BM);
+        mx = fmaxf(mx, ml.x);
+        mf = fmaxf(mf, ml.x + ml.z);
+      }
 #pragma unroll 4
       for (int p = 0; p < it.parts; ++p) {
         const float4 ml = __ldcg(src + p * pstride + 32 * BM);
         lsum = fmaf(ml.y, ex2f(ml.x - mx), lsum);
       }
-      const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+      const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum, pow_f = ex2f(mf - mx);
       if (c0 == 0) store_lse(n, mx, lsum);
       const uint32_t stage = sbase + q_at(x);
 #pragma unroll 1
@@ -859,7 +867,8 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         for (int i = 0; i < 32; ++i) acc[i] = 0.0f;
 #pragma unroll 2
         for (int p = 0; p < it.parts; ++p) {
-          const float f = ex2f(__ldcg(src + p * pstride + 32 * BM).x - mx);
+          const float4 ml = __ldcg(src + p * pstride + 32 * BM);
+          const float f = ex2f(ml.x + ml.z - mf);
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             const float4 v = __ldcg(src + p * pstride + (g + c) * BM);
@@ -870,7 +879,9 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
           }
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) stage_chunk(stage, r, g / 2 + c, acc + 8 * c, inv);
+        for (int i = 0; i < 32; ++i) acc[i] *= inv;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) stage_chunk(stage, r, g / 2 + c, acc + 8 * c, pow_f);
       }
       __syncthreads();
       store_rows(warp * 8 * nq, 8 * nq);

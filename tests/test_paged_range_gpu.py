@@ -147,3 +147,23 @@ def test_tiny_scale_and_queries(q, scale, size):
     x = (torch.randn(q, 4, 128) * size).bfloat16()
     check(x.cuda(), cache, batch, k, v, scale=scale)
     check(x.cuda(), cache, batch, k, v, scale=scale, window=50, sink=7)
+
+
+@pytest.mark.parametrize("q", [1, 12, 40, 150])
+@pytest.mark.parametrize("k_bits,v_bits,mode", [(4, 4, "blind32"), (8, 8, "bands4")])
+@pytest.mark.parametrize("n", [217, 9000])
+def test_values_near_the_end_of_fp32(q, k_bits, v_bits, mode, n):
+    """The mean of values is in range where their sum is not."""
+    cache, batch, table = make([n], [q], heads=2, page=32, k_bits=k_bits, v_bits=v_bits, mode=mode)
+    kk, vv = rows_of(n, 2, 3), (1e38 * (1 + 0.2 * torch.randn(n, 2, 128))).bfloat16()
+    vv[5::7] *= 1e-30
+    k, v = append(cache, table, kk, vv)
+    x = torch.randn(q, 4, 128).bfloat16()
+    check(x.cuda(), cache, batch, k, v)
+    check(x.cuda(), cache, batch, k, v, window=150, sink=20)
+    # an infinity is stored as 3e38: rows that see it are finite
+    vv = rows_of(n, 2, 4)
+    vv[n - 3 * q // 4 - 1, 1, 77] = float("inf")
+    cache.append(kk.cuda(), vv.cuda(), paged.PagedBatch(table, [n], [n], 32, device="cuda:0"))
+    out = paged.attention(x.cuda(), cache, batch).float()
+    assert torch.isfinite(out).all() and out[-1, 2:, 77].min() > 1e30
