@@ -200,11 +200,11 @@ __device__ __forceinline__ uint32_t most_of(const uint4& v) {
 // token that leads by 17 nats and has the value 0 came out 7 % off.
 constexpr float kBias = 7.0f, kLag = 8.0f;
 // The F of an output row once a weight times its value's power of two has been 2^top, given
-// F so far; a row that has seen nothing yet (fresh) may take a lower one than 0. Leaves
-// room below fp16's end; 0 where that does, so that ordinary rows end up there.
-__device__ __forceinline__ float next_f(float f, float top, bool fresh) {
-  const float need = ceilf(top) - (kBias + kLag);
-  const float n = fresh ? need : fmaxf(f, need);
+// what F has to be for the row so far: F less what the maximum has risen since, which for a
+// row that had seen nothing is all it can be. Leaves room below fp16's end; 0 where that
+// does, so that ordinary rows end up there.
+__device__ __forceinline__ float next_f(float f, float top) {
+  const float n = fmaxf(f, ceilf(top) - (kBias + kLag));
   return top == -INFINITY ? f : (n > -15.0f && n < 0.0f ? 0.0f : n);
 }
 // Eight bf16 times 2^-e -> fp16 (exact for normal results).

@@ -439,7 +439,6 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
 
       // ---- softmax weights
       uint32_t pf[NT][2][2];
-      bool fresh[NT][2];  // rows that have seen nothing yet
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if (!whole) {
@@ -454,8 +453,6 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
         }
         const float mx0 = fmaxf(fmaxf(s[0][nt][0], s[0][nt][2]), fmaxf(s[1][nt][0], s[1][nt][2])) * sc[nt][0];
         const float mx1 = fmaxf(fmaxf(s[0][nt][1], s[0][nt][3]), fmaxf(s[1][nt][1], s[1][nt][3])) * sc[nt][1];
-        fresh[nt][0] = m[nt][0] < -1.0e29f;
-        fresh[nt][1] = m[nt][1] < -1.0e29f;
         if (__any_sync(0xffffffffu, mx0 - m[nt][0] > kBias + kLag || mx1 - m[nt][1] > kBias + kLag)) {
           float n0 = mx0, n1 = mx1;
 #pragma unroll
@@ -466,17 +463,22 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           n0 = fmaxf(n0 - kBias, m[nt][0]);
           n1 = fmaxf(n1 - kBias, m[nt][1]);
           const float a0 = ex2f(m[nt][0] - n0), a1 = ex2f(m[nt][1] - n1);
-          m[nt][0] = n0;
-          m[nt][1] = n1;
           l[nt][0] *= a0;
           l[nt][1] *= a1;
+          if (wide_v || f_any) {  // F follows, and O below
+            F[nt][0] += m[nt][0] - n0;
+            F[nt][1] += m[nt][1] - n1;
+          } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            o[nt][i][0] *= a0;
-            o[nt][i][1] *= a1;
-            o[nt][i][2] *= a0;
-            o[nt][i][3] *= a1;
+            for (int i = 0; i < 8; ++i) {
+              o[nt][i][0] *= a0;
+              o[nt][i][1] *= a1;
+              o[nt][i][2] *= a0;
+              o[nt][i][3] *= a1;
+            }
           }
+          m[nt][0] = n0;
+          m[nt][1] = n1;
         }
 #pragma unroll
         for (int bb = 0; bb < 2; ++bb) {
@@ -507,7 +509,7 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
           for (int i = 0; i < 2; ++i) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], d));
-            const float Fn = next_f(F[nt][i], top[i], fresh[nt][i]);
+            const float Fn = next_f(F[nt][i], top[i]);
             const float back = ex2f(F[nt][i] - Fn);
             F[nt][i] = Fn;
 #pragma unroll

@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       const float mt =
           fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * row_scale;
       bool rescale = false;
-      const bool fresh = m < -1.0e29f;
+      const float m_old = m;
       float alpha = 1.0f;
       if (i_ == 0) {
         m = fmaxf(m, mt - kBias);
@@ -483,12 +483,11 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
               top = fmax3(top, __uint_as_float(s0[c + i]), __uint_as_float(s1[c + i]));
             }
           }
-          const float Fn = next_f(F, top, fresh);
-          if (Fn != F) {
-            alpha_o *= ex2f(F - Fn);
-            rescale = i_ > 0;
-            F = Fn;
-          }
+          F += m_old - m;
+          const float Fn = next_f(F, top);
+          alpha_o = ex2f(F - Fn);  // alpha's part in F has been taken
+          rescale = rescale || (i_ > 0 && Fn != F);
+          F = Fn;
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             pw[c] = pack_f16x2(ex2f(__uint_as_float(s0[2 * c]) - F), ex2f(__uint_as_float(s0[2 * c + 1]) - F));

@@ -167,3 +167,32 @@ def test_values_near_the_end_of_fp32(q, k_bits, v_bits, mode, n):
     cache.append(kk.cuda(), vv.cuda(), paged.PagedBatch(table, [n], [n], 32, device="cuda:0"))
     out = paged.attention(x.cuda(), cache, batch).float()
     assert torch.isfinite(out).all() and out[-1, 2:, 77].min() > 1e30
+
+
+@pytest.mark.parametrize("q", [1, 12, 40, 150])
+@pytest.mark.parametrize("k_bits,v_bits,mode", [(4, 4, "blind32"), (8, 8, "bands4")])
+@pytest.mark.parametrize("n", [600, 5000])
+@pytest.mark.parametrize("size,other", [(1e-20, 1.0), (1e-30, 1e-9), (1.0, 1e18)])
+def test_small_values_behind_large_ones_of_no_weight(q, k_bits, v_bits, mode, n, size, other):
+    """The first half's values are 1e18 to 1e21 times as large as the second half's, and their
+    weights 1e-26 times: the row's power of two follows the maximum down.
+
+    Bound per element: roundings as above, of each weight; below fp16's normal range 2^-32 of
+    the largest product of a weight and its value."""
+    cache, batch, table = make([n], [q], heads=1, page=32, k_bits=k_bits, v_bits=v_bits, mode=mode)
+    kk, vv = 0.03 * torch.randn(n, 1, 128), 1 + 0.2 * torch.randn(n, 1, 128)
+    kk[:, 0, 0] = 0
+    kk[n // 2:, 0, 0] = 60
+    vv[: n // 2] *= other
+    vv[n // 2:] *= size
+    x = torch.randn(q, 4, 128)
+    x[:, :, 0] = 1
+    k, v = append(cache, table, kk.bfloat16(), vv.bfloat16())
+    out = paged.attention(x.bfloat16().cuda(), cache, batch, causal=False, softmax_scale=1.0)[:, 0].double().cpu()
+    k, v, xd = k[:, 0], v[:, 0], x[:, 0].bfloat16().double()
+    w = torch.softmax(xd @ k.T, 1)
+    ref = w @ v
+    d = (2.0 ** -11 * (xd.abs() @ k.abs().T)).amax(1, keepdim=True)
+    most = (w * v.abs().amax(1)).amax(1, keepdim=True)
+    bound = 2.0 ** -8 * ref.abs() + (2 * 2.0 ** -11 + 2 * d + 2e-5) * (w @ v.abs()) + 2.0 ** -32 * n * most
+    assert ((out - ref).abs() <= bound).all()
