@@ -142,7 +142,7 @@ __device__ __forceinline__ uint32_t int8_pair_f16(uint32_t x) {
   return h16add2(and_or(x, 0x00FF00FFu, 0x64006400u), 0xE480E480u);
 }
 constexpr uint32_t kScaleLeast = 0x3880, kScaleMost = 0x4400;  // bf16 2^-14, 512 (127 * 512 < 65504)
-constexpr uint32_t kQueryLeast = 0x3B80, kQueryMost = 0x4700;        // bf16 2^-8, 2^15
+constexpr uint32_t kQueryLeast = 0x3880, kQueryMost = 0x4700;  // bf16 2^-14, 2^15
 // bits of a bf16 >= 0 outside [least, most]
 __device__ __forceinline__ bool beyond(uint32_t bits, uint32_t least, uint32_t most) { return bits - least > most - least; }
 // 2^e, |e| <= 126
@@ -170,12 +170,11 @@ __device__ __forceinline__ void extremes_of_lanes(uint32_t& most, uint32_t& leas
 constexpr uint32_t kScaleOne = 0x3F80;
 // What a token without any such group has: its weight counts nowhere but in the sum.
 constexpr int kNoScale = -110;
-// Exponent to take out of a query row whose largest magnitude has these bits: to
-// [2^14, 2^15) above, to [1, 2) below.
-__device__ __forceinline__ int query_exponent(uint32_t bits) {
-  if (bits == 0 || !beyond(bits, kQueryLeast, kQueryMost)) return 0;
-  const int e = static_cast<int>(bits >> 7) - 127;
-  return bits > kQueryMost ? e - 14 : max(e, -110);
+// Exponent to take out of a query row whose largest and least magnitudes (of elements that
+// are not 0) have these bits: the largest goes to [2^14, 2^15) where either lies beyond.
+__device__ __forceinline__ int query_exponent(uint32_t most, uint32_t least) {
+  if (most <= kQueryMost && least >= kQueryLeast) return 0;
+  return max(static_cast<int>(most >> 7) - 127 - 14, -110);
 }
 // What a row's logits are multiplied with: the softmax scale with the power of two taken out
 // of the row's query. Never 0, which would make a masked logit NaN; logits of so small a
@@ -192,6 +191,14 @@ __device__ __forceinline__ uint32_t most_of(const uint4& v) {
     m = max(m, hi < 0x7F80u ? hi : 0u);
   }
   return m;
+}
+// Least magnitude other than 0 among eight bf16, as bits, or one less (0xFFFE or more: none).
+__device__ __forceinline__ uint32_t least_of(const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t m = 0xFFFFFFFFu;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __vminu2(m, (w[i] & 0x7FFF7FFFu) - 0x00010001u);
+  return min(m & 0xFFFFu, m >> 16) + 1;
 }
 // A row's running maximum m stands kBias below the logit it was taken from and moves only
 // when some logit lies more than kLag + kBias above it, so the softmax weights 2^(x - m)

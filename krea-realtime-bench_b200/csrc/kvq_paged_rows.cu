@@ -177,9 +177,9 @@ __global__ void __launch_bounds__(kRowThreads, (RowGeo<L, KB, VB, NT>::kCtas)) r
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       uint32_t most = max(max(most_of(qv[nt][0]), most_of(qv[nt][1])), max(most_of(qv[nt][2]), most_of(qv[nt][3])));
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      const int e = query_exponent(most);
+      uint32_t least = min(min(least_of(qv[nt][0]), least_of(qv[nt][1])), min(least_of(qv[nt][2]), least_of(qv[nt][3])));
+      extremes_of_lanes<1, 2>(most, least);
+      const int e = query_exponent(most, least);
 #pragma unroll
       for (int i = 0; i < 2; ++i) sc[nt][i] = row_scale_of(a.scale_log2, __shfl_sync(0xffffffffu, e, 4 * (2 * t + i)));
 #pragma unroll

@@ -84,7 +84,8 @@ struct Geo {
   static_assert(kExpK >= NK + 5 && kExpV >= NV1 + 1, "rings of exponents");
   static constexpr int kOffExpK = kOffMisc + 32, kOffExpV = kOffExpK + kExpK * BN;
   static constexpr int kOffWideK = kOffExpV + kExpV * BN, kOffWideV = kOffWideK + 4 * kExpK;
-  static constexpr int kSmemBytes = kOffWideV + 4 * kExpV;
+  static constexpr int kOffExpQ = kOffWideV + 4 * kExpV;  // the exponent taken out of each query row
+  static constexpr int kSmemBytes = kOffExpQ + 2 * BM;
   static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM must fit");
   static_assert(kOffCK % 16 == 0 && kOffCV % 16 == 0, "bulk copies");
 };
@@ -284,11 +285,10 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   };
 
   // The exponent to take out of a query row of which each lane of half a warp has a part.
-  auto row_exponent = [&](uint32_t most) {
-    if (!__any_sync(0xffffffffu, beyond(most, kQueryLeast, kQueryMost))) return 0;
-#pragma unroll
-    for (int x = 8; x > 0; x >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
-    return query_exponent(most);
+  auto row_exponent = [&](uint32_t most, uint32_t least) {
+    if (!__any_sync(0xffffffffu, most > kQueryMost || least < kQueryLeast)) return 0;
+    extremes_of_lanes<1, 8>(most, least);
+    return query_exponent(most, least);
   };
   // Ahead of the set-up of the barriers: the Q rows, gathered by the eight softmax warps
   // (two rows at a time) and converted to fp16, and the producers' first look-ups.
@@ -308,8 +308,9 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       const uint32_t dst = sbase + q_at(n >> 7) + (c >> 3) * kQAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4);
       uint4 v = make_uint4(0, 0, 0, 0);
       if (n < it.n_rows) v = ld_global_nc_v4(a.q + from + 8 * c);
-      const int e = row_exponent(most_of(v));
+      const int e = row_exponent(most_of(v), least_of(v));
       q_wide |= e;
+      if (c == 0) smem[GEO::kOffExpQ + n] = static_cast<uint8_t>(e);
       if (n < it.n_rows) v = to_f16(v, e);
       st_shared_v4(dst, v.x, v.y, v.z, v.w);
     }
@@ -373,16 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     bool ok = true, s_ready = false;  // s_ready: S of the coming tile was already found complete
     // this row's softmax scale, with the power of two taken out of its query
     float row_scale = a.scale_log2;
-    if (q_wide) {
-      int64_t tok;
-      int h;
-      place(min(n, it.n_rows - 1), tok, h);
-      const uint4* src = reinterpret_cast<const uint4*>(a.q + tok * a.q_stride + h * D);
-      uint32_t most = 0;
-#pragma unroll 4
-      for (int c = 0; c < 16; ++c) most = max(most, most_of(ld_global_nc_v4(src + c)));
-      row_scale = row_scale_of(a.scale_log2, query_exponent(most));
-    }
+    if (q_wide) row_scale = row_scale_of(a.scale_log2, static_cast<int8_t>(smem[GEO::kOffExpQ + n]));
     // wide_k, wide_v: a byte per converter warp of the tile, and whose rows' exponents count
     auto exps16 = [&](uint32_t wide, uint32_t at, int block) {
       return (wide >> (8 * (block >> 1))) & 255u ? ld_shared_v4(at + 16 * block) : make_uint4(0, 0, 0, 0);

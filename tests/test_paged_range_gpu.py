@@ -196,3 +196,21 @@ def test_small_values_behind_large_ones_of_no_weight(q, k_bits, v_bits, mode, n,
     most = (w * v.abs().amax(1)).amax(1, keepdim=True)
     bound = 2.0 ** -8 * ref.abs() + (2 * 2.0 ** -11 + 2 * d + 2e-5) * (w @ v.abs()) + 2.0 ** -32 * n * most
     assert ((out - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("q", [1, 12, 40, 150])
+@pytest.mark.parametrize("k_bits,v_bits", FORMATS)
+@pytest.mark.parametrize("mode", ["bands", "blind32"])
+@pytest.mark.parametrize("ratio", [1e3, 2.0 ** 15, 1e6])
+@pytest.mark.parametrize("size", [1.0, 2e-3, 1e-9])
+def test_queries_with_groups_of_different_magnitude(q, k_bits, v_bits, mode, ratio, size):
+    """Queries that are small in the channels where keys are large: each group has its share of
+    the logits."""
+    n = 217
+    cache, batch, table = make([n], [q], heads=2, page=32, k_bits=k_bits, v_bits=v_bits, mode=mode)
+    large = torch.ones(128)
+    for lo, hi in cache.bands[1::2]:
+        large[lo:hi] = ratio
+    k, v = append(cache, table, (rows_of(n, 2, 3).float() * large).bfloat16(), rows_of(n, 2, 4))
+    x = (torch.randn(q, 4, 128) / large * size).bfloat16()
+    check(x.cuda(), cache, batch, k, v, scale=0.09 / size)
