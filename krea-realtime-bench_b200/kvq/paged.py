@@ -27,6 +27,7 @@ from .ops import _require_cuda
 BLOCK = 16  # tokens of one storage block
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIM = 128
+_FAR = 2 ** 32  # a window or sink beyond all positions
 
 
 # the current stream of a device as an integer, and the current device: what the public
@@ -382,6 +383,7 @@ def attention(q: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, causal: b
         raise ValueError("window and sink must be >= 0")
     if sink and not window:
         raise ValueError("sink keeps the first tokens of a window: give window too")
+    window, sink = min(window, _FAR), min(sink, _FAR)
     scale = 0.0 if softmax_scale is None else float(softmax_scale)
     # least: the kernels hold it in fp32, where a smaller one is 0
     if softmax_scale is not None and not 1e-38 <= scale <= 1e38:

@@ -214,3 +214,14 @@ def test_queries_with_groups_of_different_magnitude(q, k_bits, v_bits, mode, rat
     k, v = append(cache, table, (rows_of(n, 2, 3).float() * large).bfloat16(), rows_of(n, 2, 4))
     x = (torch.randn(q, 4, 128) / large * size).bfloat16()
     check(x.cuda(), cache, batch, k, v, scale=0.09 / size)
+
+
+@pytest.mark.parametrize("q", [1, 150])
+def test_windows_longer_than_any_sequence(q):
+    """Whole numbers of any size are windows and sinks."""
+    cache, batch, table = make([200], [q], heads=1)
+    append(cache, table, rows_of(200, 1, 3), rows_of(200, 1, 4))
+    x = torch.randn(q, 2, 128).bfloat16().cuda()
+    want = paged.attention(x, cache, batch)
+    for window, sink in ((2 ** 31, 0), (2 ** 63 - 1, 2 ** 63 - 1), (2 ** 63, 0), (2 ** 64 + 5, 2 ** 64), (9, 2 ** 64 + 3)):
+        assert torch.equal(paged.attention(x, cache, batch, window=window, sink=sink), want), (window, sink)
