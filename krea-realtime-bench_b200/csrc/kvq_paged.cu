@@ -40,7 +40,8 @@ int check_cache(const kvq_paged_cache* c, const kvq_paged_batch* b, int* layout)
               KVQ_ERR_ALIGN, "pages must be 16-byte aligned");
   const int64_t lim = ((int64_t)1 << 31) - 1;
   KVQ_REQUIRE(b->n_seqs >= 0 && b->n_new >= 0 && b->n_tokens >= 0 && b->n_new_blocks >= 0 && b->n_blocks >= 0 &&
-                  b->n_new <= lim && b->n_tokens <= lim && b->table_stride >= 0,
+                  b->n_new <= lim && b->n_tokens <= lim && b->n_new_blocks <= lim && b->n_blocks <= lim &&
+                  b->table_stride >= 0,
               KVQ_ERR_ARG, "bad batch");
   KVQ_REQUIRE(b->n_seqs == 0 || (b->table && b->seqs), KVQ_ERR_ARG, "NULL table or sequence pointer");
   KVQ_REQUIRE((reinterpret_cast<uintptr_t>(b->table) & 3) == 0 && (reinterpret_cast<uintptr_t>(b->seqs) & 15) == 0,

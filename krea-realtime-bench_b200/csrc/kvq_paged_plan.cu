@@ -235,12 +235,14 @@ static int make_plan(const kvq_paged_cache* c, int layout, const int32_t* kv_len
   auto resident = [&](int row_tile) {
     return static_cast<int64_t>(n_sms) * rows_ctas_per_sm(layout, c->k_bits, c->v_bits, row_tile);
   };
-  int64_t most = 0, q_sum = 0;  // rows of a sequence and KV head, queries
+  int64_t most = 0, q_sum = 0, n_least = 0;  // rows of a sequence and KV head, queries, fewest units
   for (int s = 0; s < n_seqs; ++s) {
-    most = std::max(most, static_cast<int64_t>(q_lens[s]) * group);
+    const int64_t rows = static_cast<int64_t>(q_lens[s]) * group;
+    most = std::max(most, rows);
     q_sum += q_lens[s];
+    n_least += (rows + kTileRows - 1) / kTileRows;
   }
-  KVQ_REQUIRE(q_sum < ((int64_t)1 << 31), KVQ_ERR_ARG, "too many rows for one launch");
+  KVQ_REQUIRE(q_sum < ((int64_t)1 << 31) && n_least * c->n_heads < (1 << 24), KVQ_ERR_ARG, "too many rows for one launch");
   std::vector<Unit> few, many;
   auto split = [&](int64_t limit) {
     few.clear();

@@ -216,3 +216,21 @@ def test_attention_entry_refuses_bad_arguments(libkvq):
     assert attend(info=None) == -1 and attend(items=None) == -1 and attend(items=p + 4) == -4
     assert attend(ws=None) == -1 and attend(ctr=None) == -1 and attend(ws=p + 128) == -4
     assert attend(batch=_lib.PagedBatchArgs(p, 2, p, 0, 20, 0, 3, 2, 0)) == 0  # no new tokens
+
+
+def test_plan_and_entries_refuse_sizes_before_they_work_on_them(libkvq):
+    """More rows than a launch has are refused before their work list is made (it would fill the
+    host's memory), and block counts beyond a grid before they are cut to 32 bits."""
+    c, keep = format_args(n_heads=1)
+    q = np.full(3, (2 ** 31 - 1) // 65535, dtype=np.int32)
+    info = _lib.PagedPlanInfo()
+    assert libkvq.kvq_paged_plan(ctypes.byref(c), q.ctypes.data, q.ctypes.data, 3, 65535, 1, 0, 0, 148, None, 0,
+                                 ctypes.byref(info)) == -1
+    assert b"too many rows" in libkvq.kvq_last_error()
+    p = 4096
+    for kw in (dict(n_new_blocks=1 << 32), dict(n_blocks=(1 << 32) + 3)):
+        b = dict(table=p, table_stride=2, seqs=p, n_new=2, n_tokens=20, n_new_blocks=2, n_blocks=3, n_seqs=2)
+        b = ctypes.byref(_lib.PagedBatchArgs(**{**b, **kw}))
+        c2 = ctypes.byref(format_args()[0])
+        assert libkvq.kvq_paged_append(p, 256, p, 256, c2, b, None) == -1
+        assert libkvq.kvq_paged_read(c2, b, 0, p, 256, p, 256, None) == -1
