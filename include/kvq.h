@@ -399,7 +399,8 @@ KVQ_API int kvq_paged_plan(const kvq_paged_cache* cache, const int32_t* kv_lens,
  *   j < kv_len,  j <= p if causal,  j > p - window or j < sink if window > 0;
  * out = sum_j w_j V_j, w = softmax(q . K_j * softmax_scale) over the tokens it sees
  * (softmax_scale <= 0: 1/sqrt(head_dim); at most 1e38); 0 (lse -inf) where it sees
- * none. Logits beyond fp32's range give NaN.
+ * none. Logits beyond 1e8 in magnitude, and products q . K_j beyond fp32's range
+ * before the scale, may give NaN or 0.
  *   q, out  bf16 [n_new][n_q_heads][head_dim], token strides in elements; query head
  *           h reads KV head h / (n_q_heads / n_heads)
  *   lse     fp32 [n_new][n_q_heads] or NULL: natural log of the sum of exponentials

@@ -365,11 +365,13 @@ def attention(q: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, causal: b
     sequences' cached tokens (append the step's k and v first): bf16 like q, and with
     return_lse also fp32 [n_new, n_q_heads], the natural log of the sum of exponentials.
 
-    Query i of a sequence stands at position p = kv_len - q_len + i; it sees tokens
-    j <= p if causal (else all), of those the last `window` (0: all) and the first
-    `sink`. A query that sees nothing gives 0, and -inf. Query head h reads KV head
-    h / (n_q_heads / n_heads); softmax_scale defaults to 1 / sqrt(128). Logits beyond
-    fp32's range give NaN."""
+    Query i of a sequence stands at position p = kv_len - q_len + i. It sees tokens j <= p
+    if causal (else all); with a window, of those only j > p - window, and the first `sink`
+    (so without causal a window bounds how far a query looks back, and all later tokens are
+    seen). A query that sees nothing gives 0, and -inf. Query head h reads KV head
+    h / (n_q_heads / n_heads); softmax_scale defaults to 1 / sqrt(128). Logits beyond 1e8 in
+    magnitude, where fp32 no longer tells neighbours apart, may give NaN or 0, and so may
+    products q . K_j beyond fp32's range before the scale."""
     if not isinstance(cache, PagedKVCache):
         raise TypeError(f"expected a PagedKVCache, got {type(cache).__name__}")
     cache._check(batch)

@@ -1,12 +1,14 @@
-"""Paged attention on the GPU where fp16 operands are short of range: channel groups of
-different magnitude inside a token. Against its definition in 64 bits, with the tolerances of
-test_paged_gpu.py, which hold every K and V value to fp16's relative rounding."""
+"""Paged cache on the GPU where fp16 operands are short of range (channel groups of different
+magnitude inside a token, small weights, values and scales near fp32's ends), and what
+test_paged_gpu.py holds loosely. Against definitions in 64 bits, with its tolerances where no
+other is derived: they hold every K and V value to fp16's relative rounding."""
 import numpy as np
 import pytest
 import torch
 
 from kvq import paged
-from test_paged_gpu import FORMATS, check, make, rows_of, stored
+from oracle import c_oracle
+from test_paged_gpu import FORMATS, check, fill, make, rows_of, stored, u16
 
 pytestmark = pytest.mark.gpu
 
@@ -225,3 +227,80 @@ def test_windows_longer_than_any_sequence(q):
     want = paged.attention(x, cache, batch)
     for window, sink in ((2 ** 31, 0), (2 ** 63 - 1, 2 ** 63 - 1), (2 ** 63, 0), (2 ** 64 + 5, 2 ** 64), (9, 2 ** 64 + 3)):
         assert torch.equal(paged.attention(x, cache, batch, window=window, sink=sink), want), (window, sink)
+
+
+@pytest.mark.parametrize("q", [1, 12, 150])
+@pytest.mark.parametrize("most", [1e4, 1e6, 3e7, 1e8])
+def test_logits_up_to_1e8(q, most):
+    """One token of a row leads by 20 nats and by far more than logits' spacing in fp32: its value,
+    and 300 e^-20 of others at most."""
+    n = 300
+    cache, batch, table = make([n], [q], heads=1, page=32)
+    k, v = append(cache, table, rows_of(n, 1, 3), rows_of(n, 1, 4))
+    x = torch.randn(q, 2, 128).bfloat16()
+    logits = (x.double().flatten(0, 1) @ k[:, 0].T)
+    scale = most / float(logits.abs().max())
+    first, second = (logits * scale).topk(2, -1).values.T
+    out = paged.attention(x.cuda(), cache, batch, causal=False, softmax_scale=scale).double().cpu().flatten(0, 1)
+    assert torch.isfinite(out).all()
+    clear = first - second > max(20.0, 100 * most * 2.0 ** -23)
+    assert clear.float().mean() > 0.8
+    want = v[logits.argmax(-1), 0]
+    assert ((out - want).abs() <= 2.0 ** -8 * want.abs() + n * 2.1e-9 * 2 * v.abs().max())[clear].all()
+
+
+@pytest.mark.parametrize("q", [1, 12, 150])
+@pytest.mark.parametrize("k_bits,v_bits,mode", [(4, 4, "blind32"), (8, 4, "bands4"), (8, 8, "bands2")])
+def test_log_sum_exp(q, k_bits, v_bits, mode):
+    """To the error that the keys' roundings allow (d per logit; none for int4) and fp32's."""
+    kv = [700, 9001]
+    cache, batch, table = make(kv, [q, q], heads=2, page=32, k_bits=k_bits, v_bits=v_bits, mode=mode)
+    k, v = fill(cache, table, kv)
+    x = torch.randn(2 * q, 4, 128).bfloat16()
+    for window, sink in ((0, 0), (200, 30)):
+        _, lse = paged.attention(x.cuda(), cache, batch, window=window, sink=sink, return_lse=True)
+        first = token = 0
+        for n in kv:
+            p, j = torch.arange(n - q, n)[:, None], torch.arange(n)[None]
+            see = (j <= p) & ((j > p - window) | (j < sink)) if window else j <= p
+            for h in range(4):
+                xh, kh = x[first:first + q, h].double(), k[token:token + n, h // 2]
+                want = torch.logsumexp((xh @ kh.T / 128 ** 0.5).masked_fill(~see, -np.inf), 1)
+                mass = xh.abs() @ kh.abs().T / 128 ** 0.5
+                d = (2.0 ** -11 * (k_bits == 8) + 2.0 ** -22) * mass.masked_fill(~see, 0).amax(1)
+                err = (lse[first:first + q, h].double().cpu() - want).abs()
+                assert (err <= d + 1e-5).all(), float((err - d).max())
+            first, token = first + q, token + n
+
+
+@pytest.mark.parametrize("heads", [7, 9, 12, 16, 17, 40])
+@pytest.mark.parametrize("k_bits,v_bits", FORMATS)
+def test_append_and_read_of_more_heads_than_a_tile(heads, k_bits, v_bits):
+    kv, q = [50, 33], [19, 33]
+    cache, batch, table = make(kv, q, heads=heads, page=16, k_bits=k_bits, v_bits=v_bits, mode="bands4")
+    k, v = rows_of(52, heads, 1), rows_of(52, heads, 2)
+    cache.append(k.cuda(), v.cuda(), batch)
+    rk, rv = cache.read(batch, new_only=True)
+    assert torch.equal(rk.cpu(), stored(k, k_bits, cache.bands).bfloat16())
+    assert torch.equal(rv.cpu(), stored(v, v_bits, cache.bands).bfloat16())
+
+
+@pytest.mark.parametrize("mode", ["bands", "blind64"])
+def test_append_extreme_rows_int8(mode):
+    """All-zero, tiny and huge rows as the oracle stores them; non-finite ones finite."""
+    cache, batch, table = make([8], [8], heads=1, k_bits=8, v_bits=8, mode=mode)
+    x = torch.randn(8, 1, 128).bfloat16()
+    x[0] = 0
+    x[1] *= 1e-38
+    x[2] *= 2.0 ** -120
+    x[3] *= 1e37
+    cache.append(x.cuda(), x.cuda(), batch)
+    rc, rs = c_oracle.quantize(u16(x), cache.bands, 8)
+    at = (int(table[0, 0]), 0, 0, slice(0, 8))
+    for codes, scales in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)):
+        assert np.array_equal(codes[at].cpu().numpy(), rc[:, 0]) and np.array_equal(u16(scales[at]), rs[:, 0])
+    x[4, 0, 3], x[5, 0, 50], x[6, 0, 127], x[7] = np.nan, np.inf, -np.inf, np.nan
+    cache.append(x.cuda(), x.cuda(), batch)
+    k, v = (t.float().cpu()[:, 0] for t in cache.read(batch))
+    assert torch.isfinite(k).all() and torch.equal(k, v)
+    assert k[4, 3] == 0 and (k[7] == 0).all() and k[5, 50] > 2.9e38 and k[6, 127] < -2.9e38
