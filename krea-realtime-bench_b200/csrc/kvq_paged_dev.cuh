@@ -171,10 +171,12 @@ constexpr uint32_t kScaleOne = 0x3F80;
 // What a token without any such group has: its weight counts nowhere but in the sum.
 constexpr int kNoScale = -110;
 // Exponent to take out of a query row whose largest and least magnitudes (of elements that
-// are not 0) have these bits: the largest goes to [2^14, 2^15) where either lies beyond.
+// are not 0) have these bits: the largest ends below 2^15, the least at 2^-14 or above if the
+// largest leaves room for that. No further, so that products with huge keys stay in range.
 __device__ __forceinline__ int query_exponent(uint32_t most, uint32_t least) {
   if (most <= kQueryMost && least >= kQueryLeast) return 0;
-  return max(static_cast<int>(most >> 7) - 127 - 14, -110);
+  const int down = static_cast<int>(most >> 7) - 127 - 14, up = static_cast<int>(least >> 7) - 127 + 14;
+  return most > kQueryMost ? down : max(max(down, up), -110);
 }
 // What a row's logits are multiplied with: the softmax scale with the power of two taken out
 // of the row's query. Never 0, which would make a masked logit NaN; logits of so small a

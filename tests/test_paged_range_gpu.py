@@ -304,3 +304,15 @@ def test_append_extreme_rows_int8(mode):
     k, v = (t.float().cpu()[:, 0] for t in cache.read(batch))
     assert torch.isfinite(k).all() and torch.equal(k, v)
     assert k[4, 3] == 0 and (k[7] == 0).all() and k[5, 50] > 2.9e38 and k[6, 127] < -2.9e38
+
+
+@pytest.mark.parametrize("q", [1, 12, 150])
+@pytest.mark.parametrize("k_bits,v_bits", FORMATS)
+@pytest.mark.parametrize("ks,qs", [(1e34, 1e-30), (1e36, 1.0), (1e-35, 1e30), (1e-30, 1e34)])
+def test_huge_keys_and_tiny_queries(q, k_bits, v_bits, ks, qs):
+    """Products in range of factors near both ends of it."""
+    n = 217
+    cache, batch, table = make([n], [q], heads=2, page=32, k_bits=k_bits, v_bits=v_bits, mode="bands")
+    k, v = append(cache, table, rows_of(n, 2, 3, ks), rows_of(n, 2, 4))
+    x = (torch.randn(q, 4, 128) * qs).bfloat16()
+    check(x.cuda(), cache, batch, k, v, scale=max(0.09 / (ks * qs), 2e-38))
