@@ -42,11 +42,11 @@ def _launch(cache: "PagedKVCache", batch: "PagedBatch", raw: int, fn, what: str,
     of the batch's uploads, so the cache, whose pages it holds too, keeps the batch."""
     if _current_device() == cache.device.index:
         rc = fn(*args, raw)
-        captured = _capturing()
+        captured = raw and _capturing()  # the legacy default stream, 0, cannot be captured
     else:
         with torch.cuda.device(cache.device):
             rc = fn(*args, raw)
-            captured = _capturing()
+            captured = raw and _capturing()
     if captured:
         cache._captured.add(batch)
     if rc:
