@@ -410,6 +410,8 @@ KVQ_API int kvq_paged_plan(const kvq_paged_cache* cache, const int32_t* kv_lens,
  *   counters     device uint32[info->n_units], 0 before the first call that uses them;
  *           a launch leaves them 0. Launches that may overlap need workspaces and
  *           counters of their own.
+ * A call captured into a CUDA graph reads the batch's table and sequences, the plan, the
+ * workspace and the counters at every replay.
  */
 KVQ_API int kvq_paged_attention(const void* q, int64_t q_token_stride, const kvq_paged_cache* cache,
                                 const kvq_paged_batch* batch, void* out, int64_t out_token_stride, float* lse,

@@ -44,7 +44,10 @@ struct Plan {
 // Few rows. Two ways to cut the units, by an estimate in microseconds of the blocks'
 // work: rounds of kRound storage blocks (two for each warp of a block of threads), the
 // join of a unit's parts, and what any join costs; for 8 and 16 rows, fitted to graph
-// replays of 1 to 8 sequences of 400 to 8000 tokens, 8 KV heads.
+// replays of 1 to 8 sequences of 400 to 8000 tokens, 8 KV heads. It says nothing of what an
+// item costs, and the first way is not tried below 9 storage blocks: batches of short
+// contexts, whose whole units become items one after the other on a line, are far from
+// one wave's latency (64 sequences of 16 tokens 49 us, of 20 to 300 tokens 31, one of 100 14).
 // - Each unit by itself into equal parts, of which all are resident at once: a block of
 //   threads has one item and waits for its data once.
 // - The units as one line of storage blocks (an empty unit counts as one), cut into equal
@@ -226,8 +229,10 @@ static void cut_tiles(std::vector<Unit>& units, int n_heads, int n_sms, Plan* p)
 // and the work is at most kMidBlocks storage blocks per resident block of threads: 24 rows,
 // one sequence of 1561 tokens 13.1 us, on the other kernel 21.9; 64 rows, one of 8000 tokens
 // (54 blocks) 24.4, 33.4; 8 sequences of 3000 tokens, 24 rows (81 blocks) 31.7, 34.6; 8 of
-// 1500, 64 rows (81) 27.5, 25.7; 12 with 32 to 48 rows, int8 (126) 44.8, 39.3. Rows on both
-// sides of 16 cost two launches else: 12 sequences with 16 to 24 rows 31.1, 51.7.
+// 1500, 64 rows (81) 27.5, 25.7; 12 with 32 to 48 rows, int8 (126) 44.8, 39.3: at the limit
+// each is a tenth faster for one of two batches. Rows on both sides of 16 cost two launches
+// else: 12 sequences with 16 to 24 rows 31.1, 51.7. (17 to 64 rows beside a sequence with
+// more go to the other kernel without a measurement.)
 constexpr int kFewRows = 16, kMidRows = 64, kMidBlocks = 80;
 
 static int make_plan(const kvq_paged_cache* c, int layout, const int32_t* kv_lens, const int32_t* q_lens, int n_seqs,

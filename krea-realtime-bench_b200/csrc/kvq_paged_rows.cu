@@ -2,9 +2,10 @@
 // single tokens, short drafts. Every K and V record of a KV head is read once for all its
 // rows. Memory-bound with int8 records; with int4 ones, of half the bytes and as many
 // instructions, bound by the issue slots (64 % used, and the ALU 53 %). Measured, 64
-// sequences of 946 to 16384 tokens, 8 KV heads, 40 query heads: int4 636 MB in 173 to 177 us
-// (3.7 TB/s), int8 5.75 TB/s of the 6.55 that a copy reaches; two sequences of 107 and 131
-// thousand tokens, int8 K and int4 V: 571 MB in 131 us (4.3 TB/s).
+// sequences of 946 to 16384 tokens, 8 KV heads, 40 query heads: int4 636 MB in 174 to 177 us
+// (3.6 TB/s), int8 1203 MB in 212 us (5.7 of the 6.55 that a copy reaches); two sequences of
+// 107 and 131 thousand tokens, int8 K and int4 V: 571 MB in 123 us (4.6 TB/s). A step with
+// scales beyond fp16's range is repeated: the int4 batch takes 2.3 times as long if all are.
 //
 // A CTA of four warps streams its pieces of the plan (kvq_paged_plan) one after the
 // other; warp w takes every fourth pair of 16-token storage blocks of a piece. A block's K
