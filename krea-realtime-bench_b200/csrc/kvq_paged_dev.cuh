@@ -211,10 +211,10 @@ constexpr float kBias = 7.0f, kLag = 8.0f;
 // The F of an output row once a weight times its value's power of two has been 2^top, given
 // what F has to be for the row so far: F less what the maximum has risen since, which for a
 // row that had seen nothing is all it can be. Leaves room below fp16's end; 0 where that
-// does, so that ordinary rows end up there.
+// leaves what an ordinary row has (top = kBias at least), so that those end up there.
 __device__ __forceinline__ float next_f(float f, float top) {
   const float n = fmaxf(f, ceilf(top) - (kBias + kLag));
-  return top == -INFINITY ? f : (n > -15.0f && n < 0.0f ? 0.0f : n);
+  return top == -INFINITY ? f : (n >= -kLag && n < 0.0f ? 0.0f : n);
 }
 // Eight bf16 times 2^-e -> fp16 (exact for normal results).
 __device__ __forceinline__ uint4 to_f16(const uint4& v, int e) {

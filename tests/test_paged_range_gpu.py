@@ -316,3 +316,32 @@ def test_huge_keys_and_tiny_queries(q, k_bits, v_bits, ks, qs):
     k, v = append(cache, table, rows_of(n, 2, 3, ks), rows_of(n, 2, 4))
     x = (torch.randn(q, 4, 128) * qs).bfloat16()
     check(x.cuda(), cache, batch, k, v, scale=max(0.09 / (ks * qs), 2e-38))
+
+
+@pytest.mark.parametrize("q", [1, 70])
+@pytest.mark.parametrize("k_bits,v_bits", [(4, 4), (8, 8)])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-4, 1e-5, 3e-6, 1e-6])
+def test_small_weights_of_small_values(q, k_bits, v_bits, size):
+    """As under a dominating token (17 nats), whose value lies in the other channels, with
+    values of any size: their power of two leaves the weights as much room as there is."""
+    n = 200
+    cache, batch, table = make([n], [q], heads=1, page=128, k_bits=k_bits, v_bits=v_bits, mode="blind64", garbage=False)
+    kk = torch.randn(n, 1, 128) * 0.03
+    vv = (1 + 0.3 * torch.randn(n, 1, 128)) * size
+    kk[:, 0, 0] = 0
+    kk[0] = 0
+    kk[0, 0, 0] = 17.0
+    vv[0, :, 64:] = 0
+    vv[1:, :, :64] = 0
+    x = torch.randn(q, 1, 128)
+    x[:, :, 0] = 1
+    x = x.bfloat16()
+    k, v = append(cache, table, kk.bfloat16(), vv.bfloat16())
+    out = paged.attention(x.cuda(), cache, batch, causal=False, softmax_scale=1.0)
+    k, v, xd = k[:, 0], v[:, 0], x[:, 0].double()
+    w = torch.softmax(xd @ k.T, 1)
+    ref = w @ v
+    d = (2.0 ** -11 * (xd.abs() @ k.abs().T)).amax(1, keepdim=True)
+    bound = 2.0 ** -8 * ref.abs() + (2 * 2.0 ** -11 + 2 * d + 2e-5) * (w @ v.abs())
+    bound += 2.0 ** -32 * w.amax(1, keepdim=True) * v.abs().sum(0)
+    assert ((out[:, 0].double().cpu() - ref).abs() <= bound).all()
