@@ -194,13 +194,14 @@ __device__ __forceinline__ uint32_t most_of(const uint4& v) {
   }
   return m;
 }
-// Least magnitude other than 0 among eight bf16, as bits, or one less (0xFFFE or more: none).
+// Least magnitude other than 0 among eight bf16, as bits, or one less (0x8000 or more: none).
+// A 0 in a low half takes one from the high half, where a 1 then counts as none.
 __device__ __forceinline__ uint32_t least_of(const uint4& v) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   uint32_t m = 0xFFFFFFFFu;
 #pragma unroll
   for (int i = 0; i < 4; ++i) m = __vminu2(m, (w[i] & 0x7FFF7FFFu) - 0x00010001u);
-  return min(m & 0xFFFFu, m >> 16) + 1;
+  return min(min(m & 0xFFFFu, m >> 16), 0xFFFEu) + 1;
 }
 // A row's running maximum m stands kBias below the logit it was taken from and moves only
 // when some logit lies more than kLag + kBias above it, so the softmax weights 2^(x - m)

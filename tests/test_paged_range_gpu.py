@@ -345,3 +345,19 @@ def test_small_weights_of_small_values(q, k_bits, v_bits, size):
     bound = 2.0 ** -8 * ref.abs() + (2 * 2.0 ** -11 + 2 * d + 2e-5) * (w @ v.abs())
     bound += 2.0 ** -32 * w.amax(1, keepdim=True) * v.abs().sum(0)
     assert ((out[:, 0].double().cpu() - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("q", [1, 12, 150])
+@pytest.mark.parametrize("bits", [1, 2, 0x7F, 0x80])
+def test_queries_of_the_smallest_numbers(q, bits):
+    """Zeros beside bf16's smallest magnitudes, in every second channel, in both orders: logits of
+    no size."""
+    n = 217
+    cache, batch, table = make([n], [q], heads=2, page=32)
+    k, v = append(cache, table, rows_of(n, 2, 3), rows_of(n, 2, 4))
+    for first in (0, 1):
+        x = torch.zeros(q, 4, 128, dtype=torch.int16)
+        x[..., first::2] = bits
+        x[:, 1, :64] = 0
+        x[:, 2, 8:] = 0
+        check(x.view(torch.bfloat16).cuda(), cache, batch, k, v)
